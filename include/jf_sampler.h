@@ -557,6 +557,171 @@ typedef struct jf_tree_gather_args {
 
 int jf_tree_gather(const jf_tree_gather_args *args, void *stream);
 
+/* ---- scoring ------------------------------------------------------------- */
+
+/* Operators over rows of logits that hand out what the selection keeps to
+ * itself: the processed logits, log-probabilities with the best alternatives,
+ * and the training of a draft model on a teacher's best tokens. None has a
+ * counterpart in the reference. Rows are f32 or bf16 at any element's
+ * alignment; row r starts at r * stride elements, and one row needs no stride.
+ * Sums, maxima and probabilities are held in fp32, and each result is rounded
+ * once to the type it is stored in; the same call gives the same bits.
+ *
+ * A scorer owns the scratch of calls of up to max_rows rows (1..4194304) over
+ * one vocabulary (1..524288 tokens). Its calls are ordered by the caller, as a
+ * sampler's are. Creates on the current HIP device. */
+typedef struct jf_scorer jf_scorer;
+
+int jf_scorer_create(uint32_t vocabulary, uint32_t max_rows, jf_scorer **out);
+int jf_scorer_destroy(jf_scorer *scorer);
+uint64_t jf_scorer_workspace_bytes(const jf_scorer *scorer);
+
+/* Requests' logit biases on the device, one row a request, each of at most
+ * max_entries distinct tokens. A bias is finite, or -infinity for a ban. */
+typedef struct jf_bias_table jf_bias_table;
+
+int jf_bias_table_create(uint32_t vocabulary, uint32_t rows,
+                         uint32_t max_entries, jf_bias_table **out);
+int jf_bias_table_destroy(jf_bias_table *table);
+/* Replaces row `row` by `count` host pairs in any order (0 clears it); uploads
+ * on `stream`. A token outside the vocabulary or given twice, or a bias that
+ * is NaN or +infinity, fails before the row changes. */
+int jf_bias_table_set(jf_bias_table *table, uint32_t row,
+                      const uint32_t *tokens, const float *biases,
+                      uint64_t count, void *stream);
+
+/* out[r][v] = mask(bias(penalize(logits[r][v]))) for every token v: the
+ * selection's penalties (jf_sample: the same table, extra tokens and rules, of
+ * rows whose policy has any), plus the row's bias of the token, or -infinity
+ * where a constrained row's mask or a stop exclusion drops it. Temperatures
+ * and cuts are the sampler's. A ban is -infinity whatever the logit; other
+ * edits follow fp32 (a NaN logit of a penalized token becomes -FLT_MAX, as in
+ * the selection), and a value past the range of a bf16 `out` is an infinity
+ * there. `out` may be the logits themselves, with the same dtype and
+ * stride: then only edited and dropped tokens are written. Otherwise the two
+ * share no element. Row records are uploaded when they differ from the last
+ * call's (as jf_sample's); a call that repeats them may be captured. */
+typedef struct jf_process_args {
+  uint32_t rows;
+  uint32_t dtype;
+  const void *logits;
+  uint64_t logits_stride;
+  void *out;
+  uint32_t out_dtype;
+  uint64_t out_stride;
+  const uint32_t *masks;         /* device; constrained rows */
+  uint64_t mask_stride;
+  const uint32_t *mask_rows;     /* host, rows entries, or NULL: row r's mask
+                                    is masks + mask_rows[r] * mask_stride */
+  const jf_policy *policies;     /* host, rows entries */
+  uint32_t stop_token_0;
+  uint32_t stop_token_1;
+  const jf_penalty_table *penalties;
+  const uint32_t *penalty_rows;  /* host, rows entries, or NULL */
+  const uint32_t *extra_tokens;  /* device */
+  const uint32_t *extra_counts;  /* host, rows entries (<= 16), or NULL */
+  uint64_t extra_stride;
+  const uint64_t *extra_offsets; /* host, rows entries, or NULL */
+  const jf_bias_table *biases;
+  const uint32_t *bias_rows;     /* host, rows entries (JF_NO_TOKEN: none), or
+                                    NULL */
+} jf_process_args;
+
+int jf_process_logits(jf_scorer *scorer, const jf_process_args *args,
+                      void *stream);
+
+/* Log-probabilities of row r at temperature T = temperatures[r] (NULL, or an
+ * entry that is no positive finite float of at least FLT_MIN, such as a greedy
+ * row's 0: 1), with m the row's largest logit:
+ *   lse = m / T + ln sum_v exp((x_v - m) / T)
+ *   lp_v = (x_v - m) / T - ln sum_v exp((x_v - m) / T)
+ * Writes, each when set: out_lse[r]; out_logprobs[r * token_count + i], the
+ * log-probability of tokens[r * token_stride + i]; out_ranks[r], the place
+ * (from 1) of the row's first such token in the order (logit down, id up);
+ * and the `top` (<= 128) first tokens of that order with theirs, in
+ * out_top_ids and out_top_logprobs [r][top].
+ * A token of logit -infinity has log-probability -infinity, whatever else its
+ * row holds, and is not listed;
+ * lists end in JF_NO_TOKEN with -infinity, and a row that leaves nothing has
+ * lse -infinity. An id outside the vocabulary scores -infinity, rank 0. A row
+ * that holds NaN or +infinity has NaN for lse and log-probabilities; its list
+ * is that of its other tokens (+infinity first), and NaN is ahead of nothing. */
+#define JF_TOP_LOGPROBS 128u
+
+typedef struct jf_logprobs_args {
+  uint32_t rows;
+  uint32_t dtype;
+  const void *logits;
+  uint64_t logits_stride;
+  const float *temperatures; /* device, rows entries, or NULL */
+  const uint32_t *tokens;    /* device, or NULL */
+  uint32_t token_count;      /* tokens a row */
+  uint64_t token_stride;
+  float *out_lse;            /* device, or NULL */
+  float *out_logprobs;       /* device; with tokens */
+  uint32_t *out_ranks;       /* device, or NULL */
+  uint32_t top;
+  uint32_t *out_top_ids;     /* device; with top */
+  float *out_top_logprobs;   /* device; with top */
+} jf_logprobs_args;
+
+int jf_logprobs(jf_scorer *scorer, const jf_logprobs_args *args, void *stream);
+
+/* Distillation of a student (the draft model) from a teacher's best tokens.
+ * Row r of the teacher's list holds teacher_count (1..256) slots, an id and a
+ * value u each; an id outside the vocabulary (JF_NO_TOKEN) is an absent slot,
+ * and a token listed again counts at its first slot. With `normalize` the
+ * values are logits, p = softmax(u / T) over the listed tokens; without, they
+ * are log-probabilities at T, p = exp(u), whose mass may be below 1. With
+ * q = softmax(logits / T) over the whole vocabulary:
+ *   out_loss[r] = sum_k p_k (ln p_k - ln q_{id_k})
+ *   grad[r][j]  = grad_loss[r * grad_loss_stride] / T
+ *                 * (q_j sum_k p_k - [j = id_k] p_k)
+ * (terms of p_k = 0 are 0; a factor of T^2 is the caller's, in grad_loss). The
+ * list and T get no gradient. A list of one token with normalize is cross
+ * entropy with that token.
+ * A row with no listed probability has loss 0; its gradient, and that of a row
+ * whose grad_loss is 0, is 0 whatever its logits. A listed token of logit
+ * -infinity with p > 0 makes the loss +infinity (its gradient stays finite);
+ * a student row that leaves nothing has q = 0 everywhere. NaN or +infinity in
+ * a row makes its loss and gradient NaN.
+ *
+ * jf_distill: the losses (and out_lse, the rows' logsumexp of logits / T, when
+ * set), and what the backward pass takes into `saved` when set:
+ * [rows][2 + teacher_count] floats. jf_distill_backward: the gradients, in the
+ * logits' dtype, from the same logits, ids and T and from `saved`.
+ * jf_distill_step: both, for a trainer that has the losses' gradients before
+ * the losses (a mean's); `saved` may be NULL. grad_loss_stride 0 gives every
+ * row the same. `grad` may be the logits themselves with the same stride,
+ * otherwise the two share no element. */
+#define JF_TEACHER_TOKENS 256u
+
+typedef struct jf_distill_args {
+  uint32_t rows;
+  uint32_t dtype;
+  const void *logits;
+  uint64_t logits_stride;
+  float temperature;
+  uint32_t normalize;
+  const uint32_t *teacher_ids;   /* device */
+  const float *teacher_values;   /* device; not read by the backward pass */
+  uint64_t teacher_stride;
+  uint32_t teacher_count;
+  float *out_loss;               /* device, rows entries */
+  float *out_lse;                /* device, rows entries, or NULL */
+  float *saved;                  /* device */
+  const float *grad_loss;        /* device */
+  uint64_t grad_loss_stride;
+  void *grad;                    /* device */
+  uint64_t grad_stride;
+} jf_distill_args;
+
+int jf_distill(jf_scorer *scorer, const jf_distill_args *args, void *stream);
+int jf_distill_backward(jf_scorer *scorer, const jf_distill_args *args,
+                        void *stream);
+int jf_distill_step(jf_scorer *scorer, const jf_distill_args *args,
+                    void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,7 @@ OUT = os.path.join(HERE, "jf_sampler", "libjf_sampler.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["jf_kernels.hip", "jf_draft.hip", "jf_gather.hip", "jf_noalloc.hip", "jf_penalty.hip",
+           "jf_process.hip", "jf_score.hip", "jf_distill.hip", "jf_scorer.cpp",
            "jf_sampler.cpp", "jf_host.cpp",
            "jf_tree.cpp", "jf_mask_wire.cpp", "sampling.cpp"]
 # jf_kernels.hip compiles as four objects (its JF_PART sections), in parallel.

@@ -1,0 +1,133 @@
+// Device access to rows of logits, f32 (DT 0) or bf16 (DT 1), for the
+// operators that read or write whole rows: 16-byte vectors at any element's
+// alignment, a chunk of 8192 tokens a block at a time. Token
+// chunk * 8192 + j * SLAB + tid * VEC + e is element e of thread tid's j-th
+// vector.
+#pragma once
+
+#include "jf_device.h"
+#include "jf_scorer.h"
+
+namespace jf {
+
+typedef uint32_t LogitWords __attribute__((ext_vector_type(4)));
+typedef LogitWords LogitWordsAt4 __attribute__((aligned(4)));
+typedef LogitWords LogitWordsAt2 __attribute__((aligned(2)));
+
+template <int DT>
+struct Logits;
+template <>
+struct Logits<0> {
+  using Element = float;
+  using Words = LogitWordsAt4;
+  static constexpr uint32_t VEC = 4;
+};
+template <>
+struct Logits<1> {
+  using Element = uint16_t;
+  using Words = LogitWordsAt2;
+  static constexpr uint32_t VEC = 8;
+};
+template <int DT>
+constexpr uint32_t kSlab = 256 * Logits<DT>::VEC;
+template <int DT>
+constexpr uint32_t kLoads = kScoreChunk / kSlab<DT>;
+
+template <int DT>
+__device__ __forceinline__ const typename Logits<DT>::Element *row_of(const void *logits,
+                                                                      uint64_t at) {
+  return (const typename Logits<DT>::Element *)logits + at;
+}
+template <int DT>
+__device__ __forceinline__ typename Logits<DT>::Element *row_of(void *logits, uint64_t at) {
+  return (typename Logits<DT>::Element *)logits + at;
+}
+
+__device__ __forceinline__ float logit_value(float x) { return x; }
+__device__ __forceinline__ float logit_value(uint16_t x) { return bf16_to_float(x); }
+
+// Rounds to nearest, ties to even; a NaN stays one (its top mantissa bit set).
+__device__ __forceinline__ uint32_t float_to_bf16(float x) {
+  const uint32_t u = f2u(x);
+  const uint32_t r = (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+  return x == x ? r : (u >> 16) | 0x40u;
+}
+template <int DT>
+__device__ __forceinline__ typename Logits<DT>::Element logit_of(float x) {
+  if constexpr (DT == 0)
+    return x;
+  else
+    return (uint16_t)float_to_bf16(x);
+}
+
+// The VEC values of one vector.
+template <int DT>
+__device__ __forceinline__ void unpack(const LogitWords &w, float (&v)[Logits<DT>::VEC]) {
+  if constexpr (DT == 0) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = u2f(w[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[2 * e] = u2f(w[e] << 16);
+      v[2 * e + 1] = u2f(w[e] & 0xffff0000u);
+    }
+  }
+}
+template <int DT>
+__device__ __forceinline__ LogitWords pack(const float (&v)[Logits<DT>::VEC]) {
+  LogitWords w;
+  if constexpr (DT == 0) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = f2u(v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = float_to_bf16(v[2 * e]) | float_to_bf16(v[2 * e + 1]) << 16;
+  }
+  return w;
+}
+
+// The vector at `token` of a row of `vocabulary` tokens; those past its end
+// hold the bits `past`.
+template <int DT>
+__device__ __forceinline__ LogitWords load_words(const typename Logits<DT>::Element *row,
+                                                 uint32_t token, uint32_t vocabulary,
+                                                 uint32_t past) {
+  if (token + Logits<DT>::VEC <= vocabulary) return *(const typename Logits<DT>::Words *)(row + token);
+  LogitWords w;
+#pragma unroll
+  for (uint32_t e = 0; e < 4; ++e) {
+    if constexpr (DT == 0) {
+      w[e] = token + e < vocabulary ? f2u(row[token + e]) : past;
+    } else {
+      const uint32_t lo = token + 2 * e < vocabulary ? row[token + 2 * e] : past;
+      const uint32_t hi = token + 2 * e + 1 < vocabulary ? row[token + 2 * e + 1] : past;
+      w[e] = lo | hi << 16;
+    }
+  }
+  return w;
+}
+// The bits of -infinity for `past`.
+template <int DT>
+constexpr uint32_t kPastMinusInfinity = DT == 0 ? 0xff800000u : 0xff80u;
+
+// The values of a vector into tokens [token, token + VEC) of a row, those
+// past its end left out.
+template <int DT>
+__device__ __forceinline__ void store_words(typename Logits<DT>::Element *row, uint32_t token,
+                                            uint32_t vocabulary, const LogitWords &w) {
+  if (token + Logits<DT>::VEC <= vocabulary) {
+    *(typename Logits<DT>::Words *)(row + token) = w;
+    return;
+  }
+#pragma unroll
+  for (uint32_t e = 0; e < Logits<DT>::VEC; ++e)
+    if (token + e < vocabulary) {
+      if constexpr (DT == 0)
+        row[token + e] = u2f(w[e]);
+      else
+        row[token + e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+    }
+}
+
+}  // namespace jf

@@ -1,0 +1,520 @@
+// Host side of the operators over rows of logits (include/jf_sampler.h,
+// "scoring"): argument checks, the bias table, the scorer's scratch and row
+// records, and the launches of jf_process.hip, jf_score.hip and
+// jf_distill.hip.
+#include "jf_scorer.h"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <string>
+#include <utility>
+#include <vector>
+
+#include "jf_objects.h"
+#include "jf_sampler.h"
+
+namespace {
+
+using namespace jf::host;
+
+constexpr uint32_t kMaxVocabulary = 524288;
+constexpr uint32_t kMaxRows = 1u << 22;
+// Blocks of one launch at most: its threads stay below 2^32.
+constexpr uint32_t kMaxBlocks = 1u << 23;
+
+uint32_t chunks_of(uint32_t vocabulary) {
+  return (vocabulary + jf::kScoreChunk - 1) / jf::kScoreChunk;
+}
+size_t element_size(uint32_t dtype) { return dtype == JF_DTYPE_F32 ? 4 : 2; }
+
+const void *rows_at(const void *p, uint64_t row, uint64_t stride, uint32_t dtype) {
+  return (const uint8_t *)p + row * stride * element_size(dtype);
+}
+template <class T>
+T *at(T *p, uint64_t offset) {
+  return p ? p + offset : nullptr;
+}
+
+}  // namespace
+
+struct jf_bias_table {
+  uint32_t vocabulary = 0;
+  uint32_t rows = 0;
+  uint32_t max_entries = 0;
+  uint32_t buckets = 0;
+  int device = 0;
+  jf::PenaltyEntry *entries = nullptr;  // [rows][max_entries] {token, bits of the bias}
+  uint32_t *offsets = nullptr;          // [rows][buckets + 1]
+  // Rows that a failed upload may have left half changed: refused until set.
+  std::vector<uint8_t> stale;
+  StagingRing staging;
+};
+
+struct jf_scorer {
+  uint32_t vocabulary = 0;
+  uint32_t max_rows = 0;
+  uint32_t chunks = 0;
+  int device = 0;
+  jf::ProcessRow *rows = nullptr;  // [max_rows]
+  float2 *partials = nullptr;      // [max_rows][chunks]
+  uint32_t *aheads = nullptr;      // [max_rows][chunks]
+  float *maxima = nullptr;         // [min(max_rows, kTopRows)][chunks * kScoreChunkGroups]
+  float *saved = nullptr;          // [max_rows][2 + kTeacherTokens]
+  uint64_t workspace_bytes = 0;
+  std::vector<jf::ProcessRow> last_rows;  // what the device's rows hold
+  std::vector<jf::ProcessRow> host_rows;  // the call's rows, reused across calls
+  StagingRing staging;
+};
+
+extern "C" {
+
+// ---- biases ------------------------------------------------------------------
+
+int jf_bias_table_destroy(jf_bias_table *t) {
+  if (!t) return JF_OK;
+  t->staging.release();
+  (void)hipFree(t->entries);
+  (void)hipFree(t->offsets);
+  delete t;
+  return JF_OK;
+}
+
+int jf_bias_table_create(uint32_t vocabulary, uint32_t rows, uint32_t max_entries,
+                         jf_bias_table **out) {
+  if (!out) return fail(JF_ERR_INVALID_ARGUMENT, "output pointer is null");
+  *out = nullptr;
+  if (!vocabulary || !rows || !max_entries || max_entries > 0x7fffffffu)
+    return fail(JF_ERR_INVALID_ARGUMENT, "invalid bias table geometry");
+  jf_bias_table *t = new (std::nothrow) jf_bias_table;
+  if (!t) return fail(JF_ERR_NO_MEMORY, "bias table allocation failed");
+  t->vocabulary = vocabulary;
+  t->rows = rows;
+  t->max_entries = max_entries;
+  t->buckets = (vocabulary + jf::kPenaltyBucket - 1) / jf::kPenaltyBucket;
+  int rc = JF_OK;
+  try {
+    t->stale.assign(rows, 0);
+  } catch (const std::bad_alloc &) {
+    rc = fail(JF_ERR_NO_MEMORY, "bias table allocation failed");
+  }
+  hipError_t e = hipGetDevice(&t->device);
+  if (rc == JF_OK && e != hipSuccess) rc = hip_fail(e, "hipGetDevice");
+  const size_t offsets = (size_t)rows * (t->buckets + 1);
+  if (rc == JF_OK) rc = device_alloc(&t->entries, (size_t)rows * max_entries, "bias entries");
+  if (rc == JF_OK) rc = device_alloc(&t->offsets, offsets, "bias offsets");
+  if (rc == JF_OK) {
+    e = hipMemset(t->offsets, 0, offsets * sizeof(uint32_t));
+    if (e == hipSuccess) e = hipDeviceSynchronize();
+    if (e != hipSuccess) rc = hip_fail(e, "bias table init");
+  }
+  if (rc != JF_OK) {
+    jf_bias_table_destroy(t);
+    return rc;
+  }
+  *out = t;
+  return JF_OK;
+}
+
+int jf_bias_table_set(jf_bias_table *t, uint32_t row, const uint32_t *tokens, const float *biases,
+                      uint64_t count, void *stream) {
+  if (!t) return fail(JF_ERR_INVALID_ARGUMENT, "bias table is null");
+  if (row >= t->rows) return fail(JF_ERR_INVALID_ARGUMENT, "bias row is outside the table");
+  if (count && (!tokens || !biases)) return fail(JF_ERR_INVALID_ARGUMENT, "null buffer");
+  if (count > t->max_entries)
+    return fail(JF_ERR_INVALID_ARGUMENT, "biases exceed the table row");
+  int rc = check_device(t->device);
+  if (rc != JF_OK) return rc;
+  try {
+    std::vector<std::pair<uint32_t, float>> sorted(count);
+    for (uint64_t i = 0; i < count; ++i) {
+      if (tokens[i] >= t->vocabulary)
+        return fail(JF_ERR_INVALID_ARGUMENT, "biased token is outside the vocabulary");
+      if (!(biases[i] <= FLT_MAX))
+        return fail(JF_ERR_INVALID_ARGUMENT, "a bias is finite or -infinity");
+      sorted[i] = {tokens[i], biases[i]};
+    }
+    std::sort(sorted.begin(), sorted.end(),
+              [](const auto &x, const auto &y) { return x.first < y.first; });
+    for (uint64_t i = 1; i < count; ++i)
+      if (sorted[i].first == sorted[i - 1].first)
+        return fail(JF_ERR_INVALID_ARGUMENT, "a token is biased twice in one row");
+    std::vector<jf::PenaltyEntry> entries(count);
+    std::vector<uint32_t> offsets(t->buckets + 1, 0u);
+    for (uint64_t i = 0; i < count; ++i) {
+      uint32_t bits;
+      std::memcpy(&bits, &sorted[i].second, sizeof(bits));
+      entries[i] = {sorted[i].first, bits};
+      ++offsets[sorted[i].first / jf::kPenaltyBucket + 1];
+    }
+    for (uint32_t b = 0; b < t->buckets; ++b) offsets[b + 1] += offsets[b];
+    const hipStream_t st = (hipStream_t)stream;
+    t->stale[row] = 1;
+    rc = t->staging.upload(t->entries + (size_t)row * t->max_entries, entries.data(),
+                           count * sizeof(jf::PenaltyEntry), st);
+    if (rc == JF_OK)
+      rc = t->staging.upload(t->offsets + (size_t)row * (t->buckets + 1), offsets.data(),
+                             offsets.size() * sizeof(uint32_t), st);
+    if (rc == JF_OK) t->stale[row] = 0;
+  } catch (const std::bad_alloc &) {
+    return fail(JF_ERR_NO_MEMORY, "bias row allocation failed");
+  }
+  return rc;
+}
+
+// ---- scorer ------------------------------------------------------------------
+
+int jf_scorer_destroy(jf_scorer *s) {
+  if (!s) return JF_OK;
+  s->staging.release();
+  (void)hipFree(s->rows);
+  (void)hipFree(s->partials);
+  (void)hipFree(s->aheads);
+  (void)hipFree(s->maxima);
+  (void)hipFree(s->saved);
+  delete s;
+  return JF_OK;
+}
+
+int jf_scorer_create(uint32_t vocabulary, uint32_t max_rows, jf_scorer **out) {
+  if (!out) return fail(JF_ERR_INVALID_ARGUMENT, "output pointer is null");
+  *out = nullptr;
+  if (!vocabulary) return fail(JF_ERR_INVALID_ARGUMENT, "invalid scoring geometry");
+  if (vocabulary > kMaxVocabulary)
+    return fail(JF_ERR_INVALID_ARGUMENT, "vocabulary exceeds 524288 tokens");
+  if (!max_rows || max_rows > kMaxRows)
+    return fail(JF_ERR_INVALID_ARGUMENT, "scoring row count is not in 1..4194304");
+  jf_scorer *s = new (std::nothrow) jf_scorer;
+  if (!s) return fail(JF_ERR_NO_MEMORY, "scorer allocation failed");
+  s->vocabulary = vocabulary;
+  s->max_rows = max_rows;
+  s->chunks = chunks_of(vocabulary);
+  int rc = JF_OK;
+  const hipError_t e = hipGetDevice(&s->device);
+  if (e != hipSuccess) rc = hip_fail(e, "hipGetDevice");
+  const uint64_t parts = (uint64_t)max_rows * s->chunks;
+  const uint64_t maxima = (uint64_t)std::min(max_rows, jf::kTopRows) * s->chunks *
+                          jf::kScoreChunkGroups;
+  const uint64_t saved = (uint64_t)max_rows * (2 + jf::kTeacherTokens);
+  if (rc == JF_OK) rc = device_alloc(&s->rows, max_rows, "row records");
+  if (rc == JF_OK) rc = device_alloc(&s->partials, parts, "row partials");
+  if (rc == JF_OK) rc = device_alloc(&s->aheads, parts, "rank partials");
+  if (rc == JF_OK) rc = device_alloc(&s->maxima, maxima, "group maxima");
+  if (rc == JF_OK) rc = device_alloc(&s->saved, saved, "distillation records");
+  if (rc != JF_OK) {
+    jf_scorer_destroy(s);
+    return rc;
+  }
+  s->workspace_bytes = max_rows * sizeof(jf::ProcessRow) +
+                       parts * (sizeof(float2) + sizeof(uint32_t)) +
+                       (maxima + saved) * sizeof(float);
+  *out = s;
+  return JF_OK;
+}
+
+uint64_t jf_scorer_workspace_bytes(const jf_scorer *s) { return s ? s->workspace_bytes : 0; }
+
+// What every call checks of its rows of logits.
+static int check_rows(const jf_scorer *s, uint32_t rows, uint32_t dtype, const void *logits,
+                      uint64_t stride, const char *what) {
+  if (!rows || rows > s->max_rows)
+    return fail(JF_ERR_INVALID_ARGUMENT, "invalid scoring batch width");
+  if (dtype != JF_DTYPE_F32 && dtype != JF_DTYPE_BF16)
+    return fail(JF_ERR_INVALID_ARGUMENT, std::string("unsupported ") + what + " dtype");
+  if (!logits) return fail(JF_ERR_INVALID_ARGUMENT, std::string("null ") + what);
+  if (rows > 1 && stride < s->vocabulary)
+    return fail(JF_ERR_INVALID_ARGUMENT,
+                std::string(what) + " row stride is below the vocabulary");
+  if ((uintptr_t)logits % element_size(dtype))
+    return fail(JF_ERR_INVALID_ARGUMENT,
+                std::string(what) + " are not aligned to their element size");
+  return JF_OK;
+}
+
+// ---- processed logits --------------------------------------------------------
+
+static int fill_process_rows(const jf_scorer *s, const jf_process_args *a,
+                             std::vector<jf::ProcessRow> &rows) {
+  bool any_constrained = false;
+  for (uint32_t r = 0; r < a->rows; ++r) {
+    const jf_policy &p = a->policies[r];
+    const int rc = jf_policy_validate(&p);
+    if (rc != JF_OK) return rc;
+    jf::ProcessRow row{};
+    row.penalty_row = row.bias_row = jf::kNoRow;
+    row.mask_row = a->mask_rows ? a->mask_rows[r] : r;
+    if (p.flags & JF_POLICY_CONSTRAINED) {
+      row.flags |= jf::kProcessMasked;
+      any_constrained = true;
+    }
+    if (p.flags & JF_POLICY_EXCLUDE_STOP) row.flags |= jf::kProcessStops;
+    if (p.repetition != 1.0f || p.presence != 0.0f || p.frequency != 0.0f) {
+      if (!a->penalties || !a->penalty_rows || a->penalty_rows[r] >= a->penalties->rows)
+        return fail(JF_ERR_INVALID_ARGUMENT, "penalized lane has no penalty table row");
+      if (a->penalties->vocabulary != s->vocabulary)
+        return fail(JF_ERR_INVALID_ARGUMENT, "penalty table vocabulary differs");
+      if (a->penalties->stale[a->penalty_rows[r]])
+        return fail(JF_ERR_LOGIC, "penalty table row is out of date after a failed update; "
+                                  "rebuild it");
+      row.penalty_row = a->penalty_rows[r];
+      row.repetition = p.repetition;
+      row.repetition_inverse = std::min(1.0f / p.repetition, FLT_MAX);
+      row.presence = p.presence;
+      row.frequency = p.frequency;
+      row.extra_count = a->extra_counts ? a->extra_counts[r] : 0u;
+      if (row.extra_count > (uint32_t)jf::kMaxExtra)
+        return fail(JF_ERR_INVALID_ARGUMENT, "more than 16 extra penalty tokens in a row");
+      if (row.extra_count && !a->extra_tokens)
+        return fail(JF_ERR_INVALID_ARGUMENT, "extra penalty tokens are null");
+      const uint64_t offset = !row.extra_count   ? 0
+                              : a->extra_offsets ? a->extra_offsets[r]
+                                                 : (uint64_t)r * a->extra_stride;
+      if (offset > 0xffffffffull - jf::kMaxExtra)
+        return fail(JF_ERR_INVALID_ARGUMENT, "extra token offset exceeds 32 bits");
+      row.extra_offset = (uint32_t)offset;
+    }
+    if (a->bias_rows && a->bias_rows[r] != JF_NO_TOKEN) {
+      if (!a->biases || a->bias_rows[r] >= a->biases->rows)
+        return fail(JF_ERR_INVALID_ARGUMENT, "biased row has no bias table row");
+      if (a->biases->vocabulary != s->vocabulary)
+        return fail(JF_ERR_INVALID_ARGUMENT, "bias table vocabulary differs");
+      if (a->biases->stale[a->bias_rows[r]])
+        return fail(JF_ERR_LOGIC, "bias table row is out of date after a failed update; set it");
+      row.bias_row = a->bias_rows[r];
+    }
+    rows.push_back(row);
+  }
+  if (any_constrained &&
+      (!a->masks || (a->rows > 1 && a->mask_stride < (s->vocabulary + 31) / 32)))
+    return fail(JF_ERR_INVALID_ARGUMENT, "constraint mask buffer is missing or short");
+  return JF_OK;
+}
+
+int jf_process_logits(jf_scorer *s, const jf_process_args *a, void *stream) {
+  if (!s || !a) return fail(JF_ERR_INVALID_ARGUMENT, "null scorer or arguments");
+  int rc = check_device(s->device);
+  if (rc != JF_OK) return rc;
+  rc = check_rows(s, a->rows, a->dtype, a->logits, a->logits_stride, "logits");
+  if (rc != JF_OK) return rc;
+  rc = check_rows(s, a->rows, a->out_dtype, a->out, a->out_stride, "processed logits");
+  if (rc != JF_OK) return rc;
+  if (!a->policies) return fail(JF_ERR_INVALID_ARGUMENT, "null policies");
+  const bool in_place = a->out == a->logits;
+  if (in_place &&
+      (a->out_dtype != a->dtype || (a->rows > 1 && a->out_stride != a->logits_stride)))
+    return fail(JF_ERR_INVALID_ARGUMENT,
+                "logits processed in place keep their dtype and row stride");
+  try {
+    s->host_rows.clear();
+    rc = fill_process_rows(s, a, s->host_rows);
+    if (rc != JF_OK) return rc;
+    // Uploaded only when they change (stream order keeps earlier launches on
+    // the records they were enqueued with).
+    const size_t bytes = s->host_rows.size() * sizeof(jf::ProcessRow);
+    if (s->last_rows.size() < s->host_rows.size() ||
+        std::memcmp(s->last_rows.data(), s->host_rows.data(), bytes) != 0) {
+      s->last_rows.clear();
+      rc = s->staging.upload(s->rows, s->host_rows.data(), bytes, (hipStream_t)stream);
+      if (rc != JF_OK) return rc;
+      s->last_rows = s->host_rows;
+    }
+  } catch (const std::bad_alloc &) {
+    s->last_rows.clear();
+    return fail(JF_ERR_NO_MEMORY, "row record allocation failed");
+  }
+  const uint64_t stride = a->rows > 1 ? a->logits_stride : s->vocabulary;
+  const uint64_t out_stride = a->rows > 1 ? a->out_stride : s->vocabulary;
+  const uint32_t most = kMaxBlocks / s->chunks;
+  for (uint32_t r = 0; r < a->rows; r += most) {
+    jf::ProcessLaunch L{};
+    L.logits = rows_at(a->logits, r, stride, a->dtype);
+    L.out = (void *)rows_at(a->out, r, out_stride, a->out_dtype);
+    L.stride = stride;
+    L.out_stride = out_stride;
+    L.rows = s->rows + r;
+    L.row_count = std::min(most, a->rows - r);
+    L.vocabulary = s->vocabulary;
+    L.chunks = s->chunks;
+    L.in_place = in_place ? 1u : 0u;
+    L.masks = a->masks;
+    L.mask_stride = a->mask_stride;
+    L.stop0 = a->stop_token_0;
+    L.stop1 = a->stop_token_1;
+    if (a->penalties) {
+      L.pen_entries = (const jf::PenaltyEntry *)a->penalties->entries;
+      L.pen_offsets = a->penalties->offsets;
+      L.pen_max_entries = a->penalties->max_entries;
+    }
+    if (a->biases) {
+      L.bias_entries = a->biases->entries;
+      L.bias_offsets = a->biases->offsets;
+      L.bias_max_entries = a->biases->max_entries;
+    }
+    L.buckets = (s->vocabulary + jf::kPenaltyBucket - 1) / jf::kPenaltyBucket;
+    L.extra = a->extra_tokens;
+    const int e = jf::launch_process(L, a->dtype, a->out_dtype, stream);
+    if (e != hipSuccess) return hip_fail((hipError_t)e, "processed logits launch");
+  }
+  return JF_OK;
+}
+
+// ---- the pass over a row -----------------------------------------------------
+
+// Blocks a row: one a chunk, and for many rows several chunks a block.
+static void split_rows(const jf_scorer *s, uint32_t rows, jf::ScoreLaunch *L) {
+  (void)rows;
+  L->segment_chunks = 1;
+  L->segments = s->chunks;
+}
+
+static jf::ScoreLaunch score_rows(const jf_scorer *s, const void *logits, uint64_t stride,
+                                  uint32_t dtype, uint32_t first, uint32_t rows) {
+  jf::ScoreLaunch L{};
+  L.logits = rows_at(logits, first, stride, dtype);
+  L.stride = stride;
+  L.row_count = rows;
+  L.vocabulary = s->vocabulary;
+  L.groups = s->chunks * jf::kScoreChunkGroups;
+  split_rows(s, rows, &L);
+  L.temperature = 1.0f;
+  // Launches of one call follow one another on its stream: each takes the
+  // scratch of the first rows again.
+  L.partials = s->partials;
+  L.aheads = s->aheads;
+  L.maxima = s->maxima;
+  return L;
+}
+
+// ---- log-probabilities -------------------------------------------------------
+
+int jf_logprobs(jf_scorer *s, const jf_logprobs_args *a, void *stream) {
+  if (!s || !a) return fail(JF_ERR_INVALID_ARGUMENT, "null scorer or arguments");
+  int rc = check_device(s->device);
+  if (rc != JF_OK) return rc;
+  rc = check_rows(s, a->rows, a->dtype, a->logits, a->logits_stride, "logits");
+  if (rc != JF_OK) return rc;
+  if (a->top > jf::kTopLogprobs)
+    return fail(JF_ERR_INVALID_ARGUMENT, "more than 128 alternatives in a row");
+  if (a->top && (!a->out_top_ids || !a->out_top_logprobs))
+    return fail(JF_ERR_INVALID_ARGUMENT, "alternatives need ids and log-probabilities");
+  if (a->token_count && (!a->tokens || !a->out_logprobs))
+    return fail(JF_ERR_INVALID_ARGUMENT, "scored tokens need ids and log-probabilities");
+  if (a->token_count && a->rows > 1 && a->token_stride < a->token_count)
+    return fail(JF_ERR_INVALID_ARGUMENT, "token row stride is below the token count");
+  if (a->out_ranks && !a->token_count)
+    return fail(JF_ERR_INVALID_ARGUMENT, "ranks need scored tokens");
+  if (!a->top && !a->token_count && !a->out_lse)
+    return fail(JF_ERR_INVALID_ARGUMENT, "nothing to score");
+  const uint64_t stride = a->rows > 1 ? a->logits_stride : s->vocabulary;
+  const uint32_t most = a->top ? jf::kTopRows : kMaxBlocks / s->chunks;
+  for (uint32_t r = 0; r < a->rows; r += most) {
+    jf::ScoreLaunch L = score_rows(s, a->logits, stride, a->dtype, r, std::min(most, a->rows - r));
+    L.temperatures = at(a->temperatures, r);
+    L.tokens = at(a->tokens, r * a->token_stride);
+    L.token_count = a->token_count;
+    L.token_stride = a->rows > 1 ? a->token_stride : 0;
+    L.out_lse = at(a->out_lse, r);
+    L.out_logprobs = at(a->out_logprobs, (uint64_t)r * a->token_count);
+    L.out_ranks = at(a->out_ranks, r);
+    L.top = a->top;
+    L.out_top_ids = at(a->out_top_ids, (uint64_t)r * a->top);
+    L.out_top_logprobs = at(a->out_top_logprobs, (uint64_t)r * a->top);
+    const int e = jf::launch_score(L, a->dtype, stream);
+    if (e != hipSuccess) return hip_fail((hipError_t)e, "log-probabilities launch");
+  }
+  return JF_OK;
+}
+
+// ---- distillation ------------------------------------------------------------
+
+// `forward`, `backward`: the passes the call makes.
+static int check_distill(const jf_scorer *s, const jf_distill_args *a, bool forward,
+                         bool backward) {
+  int rc = check_device(s->device);
+  if (rc != JF_OK) return rc;
+  rc = check_rows(s, a->rows, a->dtype, a->logits, a->logits_stride, "logits");
+  if (rc != JF_OK) return rc;
+  if (!a->teacher_count || a->teacher_count > jf::kTeacherTokens)
+    return fail(JF_ERR_INVALID_ARGUMENT, "a teacher's list holds 1..256 tokens");
+  if (!a->teacher_ids || (forward && !a->teacher_values))
+    return fail(JF_ERR_INVALID_ARGUMENT, "a teacher's list needs ids and values");
+  if (a->rows > 1 && a->teacher_stride < a->teacher_count)
+    return fail(JF_ERR_INVALID_ARGUMENT, "teacher row stride is below the teacher count");
+  if (!std::isfinite(a->temperature) || a->temperature < FLT_MIN)
+    return fail(JF_ERR_INVALID_ARGUMENT,
+                "distillation requires a finite temperature of at least FLT_MIN");
+  if (forward && !a->out_loss) return fail(JF_ERR_INVALID_ARGUMENT, "null losses");
+  if (!backward) return JF_OK;
+  if (!a->grad_loss) return fail(JF_ERR_INVALID_ARGUMENT, "null loss gradients");
+  if (!forward && !a->saved)
+    return fail(JF_ERR_INVALID_ARGUMENT, "the backward pass needs what the forward pass saved");
+  rc = check_rows(s, a->rows, a->dtype, a->grad, a->grad_stride, "gradients");
+  if (rc != JF_OK) return rc;
+  if (a->grad == a->logits && a->rows > 1 && a->grad_stride != a->logits_stride)
+    return fail(JF_ERR_INVALID_ARGUMENT, "gradients in place of the logits keep their row stride");
+  return JF_OK;
+}
+
+static int distill(jf_scorer *s, const jf_distill_args *a, bool forward, bool backward,
+                   void *stream) {
+  if (!s || !a) return fail(JF_ERR_INVALID_ARGUMENT, "null scorer or arguments");
+  const int rc = check_distill(s, a, forward, backward);
+  if (rc != JF_OK) return rc;
+  const uint64_t stride = a->rows > 1 ? a->logits_stride : s->vocabulary;
+  const uint64_t grad_stride = a->rows > 1 ? a->grad_stride : s->vocabulary;
+  const uint32_t most = kMaxBlocks / s->chunks, K = a->teacher_count;
+  for (uint32_t r = 0; r < a->rows; r += most) {
+    const uint32_t n = std::min(most, a->rows - r);
+    float *saved = a->saved ? a->saved + (uint64_t)r * (2 + K) : backward ? s->saved : nullptr;
+    if (forward) {
+      jf::ScoreLaunch L = score_rows(s, a->logits, stride, a->dtype, r, n);
+      L.temperature = a->temperature;
+      L.out_lse = at(a->out_lse, r);
+      L.teacher_ids = a->teacher_ids + r * a->teacher_stride;
+      L.teacher_values = a->teacher_values + r * a->teacher_stride;
+      L.teacher_stride = a->teacher_stride;
+      L.teacher_count = K;
+      L.normalize = a->normalize ? 1u : 0u;
+      L.out_loss = a->out_loss + r;
+      L.saved = saved;
+      const int e = jf::launch_score(L, a->dtype, stream);
+      if (e != hipSuccess) return hip_fail((hipError_t)e, "distillation launch");
+    }
+    if (backward) {
+      jf::DistillGradLaunch L{};
+      L.logits = rows_at(a->logits, r, stride, a->dtype);
+      L.stride = stride;
+      L.grad = (void *)rows_at(a->grad, r, grad_stride, a->dtype);
+      L.grad_stride = grad_stride;
+      L.row_count = n;
+      L.vocabulary = s->vocabulary;
+      L.chunks = s->chunks;
+      L.temperature = a->temperature;
+      L.teacher_ids = a->teacher_ids + r * a->teacher_stride;
+      L.teacher_stride = a->teacher_stride;
+      L.teacher_count = K;
+      L.saved = saved;
+      L.grad_loss = a->grad_loss + r * a->grad_loss_stride;
+      L.grad_loss_stride = a->grad_loss_stride;
+      const int e = jf::launch_distill_grad(L, a->dtype, stream);
+      if (e != hipSuccess) return hip_fail((hipError_t)e, "distillation gradient launch");
+    }
+  }
+  return JF_OK;
+}
+
+int jf_distill(jf_scorer *s, const jf_distill_args *a, void *stream) {
+  return distill(s, a, true, false, stream);
+}
+int jf_distill_backward(jf_scorer *s, const jf_distill_args *a, void *stream) {
+  return distill(s, a, false, true, stream);
+}
+int jf_distill_step(jf_scorer *s, const jf_distill_args *a, void *stream) {
+  return distill(s, a, true, true, stream);
+}
+
+}  // extern "C"

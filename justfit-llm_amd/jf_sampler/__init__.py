@@ -25,6 +25,8 @@ JF_DRAFT_CANDIDATES = 16
 JF_UNIFORM_ACCEPTANCE = 8
 JF_UNIFORM_CORRECTION = 15
 JF_UNIFORM_TREE_DRAWS = 24
+JF_TOP_LOGPROBS = 128
+JF_TEACHER_TOKENS = 256
 
 # Every symbol include/jf_sampler.h declares.
 EXPORTS = [
@@ -39,6 +41,9 @@ EXPORTS = [
     "jf_draft_selector_create", "jf_draft_selector_destroy", "jf_draft_select",
     "jf_tree_gather", "jf_build_draft_tree", "jf_mask_request_encode",
     "jf_mask_response_decode", "jf_mask_rows_check", "jf_mask_chain_fill", "jf_mask_tree_fill",
+    "jf_scorer_create", "jf_scorer_destroy", "jf_scorer_workspace_bytes",
+    "jf_bias_table_create", "jf_bias_table_destroy", "jf_bias_table_set",
+    "jf_process_logits", "jf_logprobs", "jf_distill", "jf_distill_backward", "jf_distill_step",
 ]
 
 c_u32 = ctypes.c_uint32
@@ -126,6 +131,38 @@ class JfTreeGatherArgs(ctypes.Structure):
         ("start_event", c_vp), ("done_event", c_vp)]
 
 
+class JfProcessArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_u32), ("dtype", c_u32), ("logits", c_vp), ("logits_stride", c_u64),
+        ("out", c_vp), ("out_dtype", c_u32), ("out_stride", c_u64), ("masks", c_vp),
+        ("mask_stride", c_u64), ("mask_rows", ctypes.POINTER(c_u32)),
+        ("policies", ctypes.POINTER(JfPolicy)), ("stop_token_0", c_u32), ("stop_token_1", c_u32),
+        ("penalties", c_vp), ("penalty_rows", ctypes.POINTER(c_u32)), ("extra_tokens", c_vp),
+        ("extra_counts", ctypes.POINTER(c_u32)), ("extra_stride", c_u64),
+        ("extra_offsets", ctypes.POINTER(c_u64)), ("biases", c_vp),
+        ("bias_rows", ctypes.POINTER(c_u32)),
+    ]
+
+
+class JfLogprobsArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_u32), ("dtype", c_u32), ("logits", c_vp), ("logits_stride", c_u64),
+        ("temperatures", c_vp), ("tokens", c_vp), ("token_count", c_u32),
+        ("token_stride", c_u64), ("out_lse", c_vp), ("out_logprobs", c_vp), ("out_ranks", c_vp),
+        ("top", c_u32), ("out_top_ids", c_vp), ("out_top_logprobs", c_vp),
+    ]
+
+
+class JfDistillArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_u32), ("dtype", c_u32), ("logits", c_vp), ("logits_stride", c_u64),
+        ("temperature", c_f32), ("normalize", c_u32), ("teacher_ids", c_vp),
+        ("teacher_values", c_vp), ("teacher_stride", c_u64), ("teacher_count", c_u32),
+        ("out_loss", c_vp), ("out_lse", c_vp), ("saved", c_vp), ("grad_loss", c_vp),
+        ("grad_loss_stride", c_u64), ("grad", c_vp), ("grad_stride", c_u64),
+    ]
+
+
 class JfDraftTree(ctypes.Structure):
     _fields_ = [("rows", c_u32), ("copies", c_u32), ("parent", c_u32 * 16), ("depth", c_u32 * 16),
                 ("copy", c_u32 * 16), ("token", c_u32 * 16), ("path_length", c_u32 * 16),
@@ -205,6 +242,18 @@ def lib():
         L.jf_mask_rows_check.argtypes = [c_vp, c_u32, c_u32, c_u32]
         L.jf_mask_chain_fill.argtypes = [c_vp, c_u32, c_u32, c_u32]
         L.jf_mask_tree_fill.argtypes = [c_vp, c_u32, c_vp, c_vp, c_u32]
+        L.jf_scorer_create.argtypes = [c_u32, c_u32, ctypes.POINTER(c_vp)]
+        L.jf_scorer_destroy.argtypes = [c_vp]
+        L.jf_scorer_workspace_bytes.argtypes = [c_vp]
+        L.jf_scorer_workspace_bytes.restype = c_u64
+        L.jf_bias_table_create.argtypes = [c_u32, c_u32, c_u32, ctypes.POINTER(c_vp)]
+        L.jf_bias_table_destroy.argtypes = [c_vp]
+        L.jf_bias_table_set.argtypes = [c_vp, c_u32, c_vp, c_vp, c_u64, c_vp]
+        L.jf_process_logits.argtypes = [c_vp, ctypes.POINTER(JfProcessArgs), c_vp]
+        L.jf_logprobs.argtypes = [c_vp, ctypes.POINTER(JfLogprobsArgs), c_vp]
+        L.jf_distill.argtypes = [c_vp, ctypes.POINTER(JfDistillArgs), c_vp]
+        L.jf_distill_backward.argtypes = [c_vp, ctypes.POINTER(JfDistillArgs), c_vp]
+        L.jf_distill_step.argtypes = [c_vp, ctypes.POINTER(JfDistillArgs), c_vp]
         _lib = L
     return _lib
 
@@ -552,6 +601,219 @@ class DraftSelector:
     def close(self):
         if self.handle:
             lib().jf_draft_selector_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class BiasTable:
+    """jf_bias_table: device logit biases, one row a request."""
+
+    def __init__(self, vocabulary, rows, max_entries):
+        h = c_vp()
+        check(lib().jf_bias_table_create(vocabulary, rows, max_entries, ctypes.byref(h)))
+        self.handle = h
+        self.vocabulary = vocabulary
+        self.rows = rows
+
+    def set(self, row, tokens, biases):
+        """Replaces a row's biases (host sequences; float("-inf") bans)."""
+        import numpy as np
+        t = np.ascontiguousarray(tokens, dtype=np.uint32)
+        b = np.ascontiguousarray(biases, dtype=np.float32)
+        if t.size != b.size:
+            raise ValueError("tokens and biases differ in length")
+        check(lib().jf_bias_table_set(self.handle, row, t.ctypes.data_as(c_vp),
+                                      b.ctypes.data_as(c_vp), t.size, _stream()))
+
+    def close(self):
+        if self.handle:
+            lib().jf_bias_table_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _dtype(t, what):
+    import torch
+    if t.dtype == torch.float32:
+        return JF_DTYPE_F32
+    if t.dtype == torch.bfloat16:
+        return JF_DTYPE_BF16
+    raise ValueError(f"{what} are f32 or bf16, not {t.dtype}")
+
+
+def _rows(t, vocabulary, rows, what):
+    """Checks a [rows, vocabulary] tensor of contiguous rows."""
+    if t.dim() != 2 or t.shape[1] != vocabulary or (rows is not None and t.shape[0] != rows):
+        raise ValueError(f"{what} have shape {tuple(t.shape)}")
+    if vocabulary > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what} have no contiguous rows")
+
+
+def _plain(t, shape, what, floating):
+    """The address of an optional contiguous f32 (or 32-bit id) tensor."""
+    import torch
+    if t is None:
+        return None
+    if tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{what} is no contiguous tensor of shape {shape}")
+    if t.dtype not in ((torch.float32,) if floating else (torch.int32, torch.uint32)):
+        raise ValueError(f"{what} holds {t.dtype}")
+    return t.data_ptr()
+
+
+class Scorer:
+    """jf_scorer: processed logits, log-probabilities and distillation over
+    one vocabulary, up to max_rows rows a call. The *_args methods check
+    tensors and build the record that launch_* issues; a record names device
+    addresses, so its tensors have to outlive it (host arrays ride along)."""
+
+    def __init__(self, vocabulary, max_rows):
+        h = c_vp()
+        check(lib().jf_scorer_create(vocabulary, max_rows, ctypes.byref(h)))
+        self.handle = h
+        self.vocabulary = vocabulary
+        self.max_rows = max_rows
+
+    def workspace_bytes(self):
+        return lib().jf_scorer_workspace_bytes(self.handle)
+
+    def process_args(self, logits, policies, out, *, masks=None, mask_rows=None,
+                     stop_tokens=(JF_NO_TOKEN, JF_NO_TOKEN), penalties=None, penalty_rows=None,
+                     extra_tokens=None, extra_counts=None, extra_stride=0, extra_offsets=None,
+                     biases=None, bias_rows=None):
+        """Builds a JfProcessArgs (kept-alive host arrays ride along). bias_rows:
+        the bias table's row of each row, None for a row without biases."""
+        rows = logits.shape[0]
+        _rows(logits, self.vocabulary, None, "logits")
+        _rows(out, self.vocabulary, rows, "processed logits")
+        a = JfProcessArgs()
+        a.rows = rows
+        a.dtype, a.out_dtype = _dtype(logits, "logits"), _dtype(out, "processed logits")
+        a.logits, a.logits_stride = logits.data_ptr(), logits.stride(0)
+        a.out, a.out_stride = out.data_ptr(), out.stride(0)
+        if masks is not None:
+            a.masks = masks.data_ptr()
+            a.mask_stride = masks.stride(0)
+        pol = (JfPolicy * rows)(*policies)
+        a.policies = pol
+        a.stop_token_0, a.stop_token_1 = stop_tokens
+        keep = [pol]
+        if penalties is not None:
+            a.penalties = penalties.handle
+        if extra_tokens is not None:
+            a.extra_tokens = extra_tokens.data_ptr()
+            a.extra_stride = extra_stride
+        if biases is not None:
+            a.biases = biases.handle
+        if bias_rows is not None:
+            bias_rows = [JF_NO_TOKEN if b is None else b for b in bias_rows]
+        for name, values, ctype in (("mask_rows", mask_rows, c_u32),
+                                    ("penalty_rows", penalty_rows, c_u32),
+                                    ("extra_counts", extra_counts, c_u32),
+                                    ("extra_offsets", extra_offsets, c_u64),
+                                    ("bias_rows", bias_rows, c_u32)):
+            if values is not None:
+                if len(values) != rows:
+                    raise ValueError(f"{name} has {len(values)} entries for {rows} rows")
+                arr = (ctype * rows)(*[int(v) for v in values])
+                setattr(a, name, arr)
+                keep.append(arr)
+        return a, keep
+
+    def launch_process(self, a, stream=None):
+        check(lib().jf_process_logits(self.handle, ctypes.byref(a),
+                                      _stream() if stream is None else stream))
+
+    def process(self, *args, **kwargs):
+        a, _ = self.process_args(*args, **kwargs)
+        self.launch_process(a)
+
+    def logprobs_args(self, logits, *, tokens=None, temperatures=None, lse=None, logprobs=None,
+                      ranks=None, top_ids=None, top_logprobs=None):
+        """Builds a JfLogprobsArgs over torch device tensors: tokens and
+        logprobs [rows, n], lse, ranks and temperatures [rows], top_ids and
+        top_logprobs [rows, k]."""
+        rows = logits.shape[0]
+        _rows(logits, self.vocabulary, None, "logits")
+        a = JfLogprobsArgs()
+        a.rows, a.dtype = rows, _dtype(logits, "logits")
+        a.logits, a.logits_stride = logits.data_ptr(), logits.stride(0)
+        a.temperatures = _plain(temperatures, (rows,), "temperatures", True)
+        if tokens is not None:
+            a.token_count = tokens.shape[1]
+            a.tokens = _plain(tokens, (rows, a.token_count), "tokens", False)
+            a.token_stride = a.token_count
+        a.out_logprobs = _plain(logprobs, (rows, a.token_count), "logprobs", True)
+        a.out_lse = _plain(lse, (rows,), "lse", True)
+        a.out_ranks = _plain(ranks, (rows,), "ranks", False)
+        if top_ids is not None:
+            a.top = top_ids.shape[1]
+            a.out_top_ids = _plain(top_ids, (rows, a.top), "top_ids", False)
+        a.out_top_logprobs = _plain(top_logprobs, (rows, a.top), "top_logprobs", True)
+        return a
+
+    def launch_logprobs(self, a, stream=None):
+        check(lib().jf_logprobs(self.handle, ctypes.byref(a),
+                                _stream() if stream is None else stream))
+
+    def logprobs(self, *args, **kwargs):
+        self.launch_logprobs(self.logprobs_args(*args, **kwargs))
+
+    def distill_args(self, logits, teacher_ids, teacher_values, *, temperature=1.0,
+                     normalize=True, loss=None, lse=None, saved=None, grad_loss=None, grad=None):
+        """Builds a JfDistillArgs over torch device tensors: teacher_ids (-1:
+        an absent slot) and teacher_values [rows, k] with contiguous rows,
+        loss and lse [rows], saved [rows, 2 + k], grad_loss [rows] (also
+        expanded from one value), grad as the logits."""
+        rows, k = teacher_ids.shape
+        _rows(logits, self.vocabulary, rows, "logits")
+        a = JfDistillArgs()
+        a.rows, a.dtype = rows, _dtype(logits, "logits")
+        a.logits, a.logits_stride = logits.data_ptr(), logits.stride(0)
+        a.temperature, a.normalize = temperature, 1 if normalize else 0
+        a.teacher_ids = _plain(teacher_ids, (rows, k), "teacher_ids", False)
+        a.teacher_values = _plain(teacher_values, (rows, k), "teacher_values", True)
+        a.teacher_stride = a.teacher_count = k
+        a.out_loss = _plain(loss, (rows,), "loss", True)
+        a.out_lse = _plain(lse, (rows,), "lse", True)
+        a.saved = _plain(saved, (rows, 2 + k), "saved", True)
+        if grad_loss is not None:
+            import torch
+            if tuple(grad_loss.shape) != (rows,) or grad_loss.dtype != torch.float32:
+                raise ValueError(f"grad_loss is no f32 tensor of {rows} rows")
+            a.grad_loss, a.grad_loss_stride = grad_loss.data_ptr(), grad_loss.stride(0)
+        if grad is not None:
+            _rows(grad, self.vocabulary, rows, "gradients")
+            if grad.dtype != logits.dtype:
+                raise ValueError("gradients have the logits' dtype")
+            a.grad, a.grad_stride = grad.data_ptr(), grad.stride(0)
+        return a
+
+    def launch_distill(self, a, stream=None):
+        check(lib().jf_distill(self.handle, ctypes.byref(a),
+                               _stream() if stream is None else stream))
+
+    def launch_distill_backward(self, a, stream=None):
+        check(lib().jf_distill_backward(self.handle, ctypes.byref(a),
+                                        _stream() if stream is None else stream))
+
+    def launch_distill_step(self, a, stream=None):
+        check(lib().jf_distill_step(self.handle, ctypes.byref(a),
+                                    _stream() if stream is None else stream))
+
+    def close(self):
+        if self.handle:
+            lib().jf_scorer_destroy(self.handle)
             self.handle = None
 
     def __del__(self):

@@ -1,0 +1,40 @@
+"""Distillation of a draft model as a torch loss: the losses and gradients are
+jf_distill's and jf_distill_backward's (no fallback)."""
+import torch
+
+from . import JF_TEACHER_TOKENS
+
+
+class _DistillLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, scorer, teacher_ids, teacher_values, temperature, normalize):
+        rows, k = teacher_ids.shape
+        loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        saved = torch.empty((rows, 2 + k), dtype=torch.float32, device=logits.device)
+        scorer.launch_distill(scorer.distill_args(
+            logits, teacher_ids, teacher_values, temperature=temperature, normalize=normalize,
+            loss=loss, saved=saved))
+        ctx.save_for_backward(logits, teacher_ids, teacher_values, saved)
+        ctx.scorer, ctx.temperature, ctx.normalize = scorer, temperature, normalize
+        return loss
+
+    @staticmethod
+    def backward(ctx, grad_loss):
+        logits, teacher_ids, teacher_values, saved = ctx.saved_tensors
+        grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        ctx.scorer.launch_distill_backward(ctx.scorer.distill_args(
+            logits, teacher_ids, teacher_values, temperature=ctx.temperature,
+            normalize=ctx.normalize, saved=saved, grad_loss=grad_loss, grad=grad))
+        return grad, None, None, None, None, None
+
+
+def distill_loss(scorer, logits, teacher_ids, teacher_values, temperature=1.0, normalize=True):
+    """Each row's loss against a teacher's list (jf_distill) on torch's
+    current stream, with gradients for `logits` ([rows, vocabulary], f32 or
+    bf16, contiguous rows). teacher_ids: int32 [rows, k], -1 for absent slots;
+    teacher_values: f32 [rows, k], logits with `normalize`, otherwise
+    log-probabilities at the temperature."""
+    if not 1 <= teacher_ids.shape[1] <= JF_TEACHER_TOKENS:
+        raise ValueError(f"a teacher's list holds 1..{JF_TEACHER_TOKENS} tokens")
+    return _DistillLoss.apply(logits, scorer, teacher_ids, teacher_values, float(temperature),
+                              bool(normalize))
