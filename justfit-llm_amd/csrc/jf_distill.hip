@@ -34,11 +34,7 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillGradLaunch a) 
   // A row with no list, or whose loss nothing follows from, is not read.
   const bool read = weight != 0.0f && scale != 0.0f;
   LogitWords w[LOADS];
-#pragma unroll
-  for (uint32_t j = 0; j < LOADS; ++j) {
-    const uint32_t token = base + j * SLAB + tid * VEC;
-    if (read && token < V) w[j] = load_words<DT>(z, token, V, 0);
-  }
+  if (read) load_chunk<DT>(z, base, V, 0, w);
   listed[tid] = 0;
   __syncthreads();
   if (tid < K && scale != 0.0f) {

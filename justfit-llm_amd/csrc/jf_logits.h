@@ -46,18 +46,19 @@ __device__ __forceinline__ typename Logits<DT>::Element *row_of(void *logits, ui
 __device__ __forceinline__ float logit_value(float x) { return x; }
 __device__ __forceinline__ float logit_value(uint16_t x) { return bf16_to_float(x); }
 
-// Rounds to nearest, ties to even; a NaN stays one (its top mantissa bit set).
-__device__ __forceinline__ uint32_t float_to_bf16(float x) {
-  const uint32_t u = f2u(x);
-  const uint32_t r = (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
-  return x == x ? r : (u >> 16) | 0x40u;
+// Two values rounded to bf16 (to nearest, ties to even; a NaN stays one), the
+// first in the low half: one conversion instruction.
+__device__ __forceinline__ uint32_t floats_to_bf16(float lo, float hi) {
+  typedef float Floats __attribute__((ext_vector_type(2)));
+  typedef __bf16 Halves __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((Floats{lo, hi}), Halves));
 }
 template <int DT>
 __device__ __forceinline__ typename Logits<DT>::Element logit_of(float x) {
   if constexpr (DT == 0)
     return x;
   else
-    return (uint16_t)float_to_bf16(x);
+    return (uint16_t)floats_to_bf16(x, x);
 }
 
 // The VEC values of one vector.
@@ -82,7 +83,7 @@ __device__ __forceinline__ LogitWords pack(const float (&v)[Logits<DT>::VEC]) {
     for (int e = 0; e < 4; ++e) w[e] = f2u(v[e]);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = float_to_bf16(v[2 * e]) | float_to_bf16(v[2 * e + 1]) << 16;
+    for (int e = 0; e < 4; ++e) w[e] = floats_to_bf16(v[2 * e], v[2 * e + 1]);
   }
   return w;
 }
@@ -106,6 +107,23 @@ __device__ __forceinline__ LogitWords load_words(const typename Logits<DT>::Elem
     }
   }
   return w;
+}
+// A thread's vectors of the chunk at `base`. One branch for the chunk: with one
+// a vector the compiler keeps every vector's ways apart in registers.
+template <int DT>
+__device__ __forceinline__ void load_chunk(const typename Logits<DT>::Element *row, uint32_t base,
+                                           uint32_t vocabulary, uint32_t past,
+                                           LogitWords (&w)[kLoads<DT>]) {
+  const uint32_t token = base + threadIdx.x * Logits<DT>::VEC;
+  if (base + kScoreChunk <= vocabulary) {
+#pragma unroll
+    for (uint32_t j = 0; j < kLoads<DT>; ++j)
+      w[j] = *(const typename Logits<DT>::Words *)(row + token + j * kSlab<DT>);
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < kLoads<DT>; ++j)
+      w[j] = load_words<DT>(row, token + j * kSlab<DT>, vocabulary, past);
+  }
 }
 // The bits of -infinity for `past`.
 template <int DT>

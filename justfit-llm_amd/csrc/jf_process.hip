@@ -53,13 +53,7 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
   // An unmasked row that is written elsewhere needs every vector: ask first.
   const bool whole = !masked && !a.in_place;
   LogitWords w[LOADS];
-  if (whole) {
-#pragma unroll
-    for (uint32_t j = 0; j < LOADS; ++j) {
-      const uint32_t token = base + j * SLAB + tid * VEC;
-      if (token < V) w[j] = load_words<DI>(x, token, V, 0);
-    }
-  }
+  if (whole) load_chunk<DI>(x, base, V, 0, w);
 
   uint32_t pen0 = 0, pen1 = 0, bias0 = 0, bias1 = 0;
   const uint32_t b0 = chunk * (kScoreChunk / kPenaltyBucket);
@@ -90,13 +84,18 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
   if (tid < p.extra_count) s.extras[tid] = a.extra[p.extra_offset + tid];
   const bool edits = pen1 > pen0 || bias1 > bias0 || p.extra_count;
   if (edits || masked) __syncthreads();
+  // A dropped token's edits are not worked out, nor its logit read.
+  const auto dropped = [&](uint32_t at) {
+    return masked && !(s.admitted[at >> 5] >> (at & 31u) & 1u);
+  };
   if (pen1 > pen0) {
     const PenaltyEntry *list = a.pen_entries + (uint64_t)p.penalty_row * a.pen_max_entries;
     for (uint32_t i = pen0 + tid; i < pen1; i += 256) {
       const PenaltyEntry e = list[i];
+      const uint32_t at = e.token - base;
+      if (dropped(at)) continue;
       uint32_t count = e.word & kCountMask;
       for (uint32_t k = 0; k < p.extra_count; ++k) count += s.extras[k] == e.token;
-      const uint32_t at = e.token - base;
       s.value[at] = penalize(logit_value(x[e.token]), count, p.repetition, p.repetition_inverse,
                              p.presence, p.frequency);
       atomicOr(&s.edited[at >> 5], 1u << (at & 31u));
@@ -107,7 +106,8 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
     __syncthreads();
     if (tid < p.extra_count) {
       const uint32_t token = s.extras[tid], at = token - base;
-      bool take = token < V && at < kScoreChunk && !(s.edited[at >> 5] >> (at & 31u) & 1u);
+      bool take = token < V && at < kScoreChunk && !dropped(at) &&
+                  !(s.edited[at >> 5] >> (at & 31u) & 1u);
       uint32_t count = 0;
       for (uint32_t k = 0; k < p.extra_count; ++k) {
         count += s.extras[k] == token;
@@ -127,6 +127,7 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
     for (uint32_t i = bias0 + tid; i < bias1; i += 256) {
       const PenaltyEntry e = list[i];
       const uint32_t at = e.token - base;
+      if (dropped(at)) continue;
       const float bias = u2f(e.word);
       // Only this token's own bias can set its bit meanwhile.
       const float v = s.edited[at >> 5] >> (at & 31u) & 1u ? s.value[at] : logit_value(x[e.token]);
@@ -180,8 +181,7 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
     } else if (token + VEC <= V) {
       typedef uint32_t Pair __attribute__((ext_vector_type(2)));
       typedef Pair PairAt2 __attribute__((aligned(2)));
-      *(PairAt2 *)(y + token) = Pair{float_to_bf16(v[0]) | float_to_bf16(v[1]) << 16,
-                                     float_to_bf16(v[2]) | float_to_bf16(v[3]) << 16};
+      *(PairAt2 *)(y + token) = Pair{floats_to_bf16(v[0], v[1]), floats_to_bf16(v[2], v[3])};
     } else {
 #pragma unroll
       for (uint32_t e = 0; e < VEC; ++e)

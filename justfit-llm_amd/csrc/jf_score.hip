@@ -103,15 +103,7 @@ __global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
   for (uint32_t chunk = first; chunk < last; ++chunk) {
     const uint32_t base = chunk * kScoreChunk;
     LogitWords w[LOADS];
-    if (base + kScoreChunk <= V) {
-#pragma unroll
-      for (uint32_t j = 0; j < LOADS; ++j)
-        w[j] = *(const typename Logits<DT>::Words *)(x + base + j * SLAB + tid * VEC);
-    } else {
-#pragma unroll
-      for (uint32_t j = 0; j < LOADS; ++j)
-        w[j] = load_words<DT>(x, base + j * SLAB + tid * VEC, V, kPastMinusInfinity<DT>);
-    }
+    load_chunk<DT>(x, base, V, kPastMinusInfinity<DT>, w);
     float part[LOADS], m = -__builtin_inff();
 #pragma unroll
     for (uint32_t j = 0; j < LOADS; ++j) {
@@ -211,145 +203,201 @@ struct RowScore {
 };
 
 constexpr uint32_t kMostItems = 32;  // groups, and then tokens, a thread holds at most
+// Lists of up to this many alternatives are cut by the best items of 64 quads
+// of lanes, longer ones by those of the 256 threads: a cut by fewer units is
+// quicker to find and lists more items.
+constexpr uint32_t kQuadTop = 32;
+constexpr uint32_t kListItems = kMostItems * (kTopLogprobs - 1) + 1;
+static_assert(4 * kMostItems * (kQuadTop - 1) + 1 <= kListItems);
+constexpr uint32_t kIdBits = 20;  // tokens and groups are below 2^20
 
-struct TopLds {
-  uint4 key[64];  // the threads' best keys
-  uint32_t list_key[kMostItems * (kTopLogprobs - 1) + 1];
-  uint32_t list_id[kMostItems * (kTopLogprobs - 1) + 1];
-  uint32_t best[kTopLogprobs];
-  uint32_t bound_key, bound_id, ahead, ties, count;
+struct TopList {
+  uint32_t unit_key[256], unit_id[256];
+  uint2 item[kListItems];  // key, id
+  uint32_t count;
 };
 
+// The k-th largest (from 1) of the wave's 64 * U values below 2^BITS, found
+// bit by bit: the largest t that k values reach.
+template <uint32_t U, int BITS>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[U], uint32_t k) {
+  uint32_t t = 0;
+#pragma unroll 4
+  for (int b = BITS - 1; b >= 0; --b) {
+    const uint32_t trial = t | 1u << b;
+    uint32_t reach = 0;
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) reach += (uint32_t)__popcll(ballot(v[u] >= trial));
+    if (reach >= k) t = trial;
+  }
+  return t;
+}
+
 // Lists in LDS, in no order, the block's items at or ahead of the k-th of its
-// threads' best items, in the order (key down, id up); key 0 is no item, and
-// with fewer than k threads that have an item every one is listed. So the list
-// holds the block's k best items. An item on it belongs to one of those k
-// threads, the k-th of which has no other one there: at most
-// (k - 1) * kMostItems + 1 items. Returns their number.
-template <uint32_t N>
-__device__ __forceinline__ uint32_t list_best(TopLds &s, uint32_t k, const uint32_t (&key)[N],
+// units' best items (a unit: four lanes, or with U = 4 one thread), in the
+// order (key down, id up); key 0 is no item, and with fewer than k units that
+// have an item every one is listed. So the list holds the block's k best items.
+// An item on it belongs to one of those k units, the k-th of which has no other
+// one there: at most (k - 1) * 4 / U * N + 1 items. Returns their number.
+// s.count is 0 on entry, ordered by a barrier.
+template <uint32_t N, uint32_t U>
+__device__ __forceinline__ uint32_t list_best(TopList &s, uint32_t k, const uint32_t (&key)[N],
                                               const uint32_t (&id)[N]) {
-  static_assert(N <= kMostItems);
-  const uint32_t tid = threadIdx.x;
+  static_assert(N <= kMostItems && (U == 1 || U == 4));
+  const uint32_t tid = threadIdx.x, lane = tid & 63u;
   uint32_t best = 0, best_id = 0;
+  const auto take = [&](uint32_t other, uint32_t other_id) {
+    if (other > best || (other == best && other_id < best_id)) {
+      best = other;
+      best_id = other_id;
+    }
+  };
 #pragma unroll
-  for (uint32_t i = 0; i < N; ++i)
-    if (key[i] > best || (key[i] == best && key[i] && id[i] < best_id)) {
-      best = key[i];
-      best_id = id[i];
+  for (uint32_t i = 0; i < N; ++i) take(key[i], id[i]);
+  const uint32_t own = best, own_id = best_id;
+  if constexpr (U == 1) {
+    take(xor_u32<1>(best), xor_u32<1>(best_id));
+    take(xor_u32<2>(best), xor_u32<2>(best_id));
+    if (tid % 4 == 0) {
+      s.unit_key[tid / 4] = best;
+      s.unit_id[tid / 4] = best_id;
     }
-  __syncthreads();  // what an earlier call left has been read
-  ((uint32_t *)s.key)[tid] = best;
-  if (tid == 0) {
-    s.bound_key = 0xffffffffu;
-    s.bound_id = 0;
-    s.ties = s.count = 0;
+  } else {
+    s.unit_key[tid] = best;
+    s.unit_id[tid] = best_id;
   }
-  const uint32_t threads = (uint32_t)__syncthreads_count(best != 0);
-  uint32_t bound_key = 1, bound_id = 0xffffffffu;  // everything
-  if (threads >= k) {
-    uint32_t ahead = 0;
-    for (uint32_t t = 0; t < 64; ++t) {
-      const uint4 other = s.key[t];
-      ahead += other.x > best;
-      ahead += other.y > best;
-      ahead += other.z > best;
-      ahead += other.w > best;
-    }
-    // The k-th best key is the least with fewer than k ahead of it.
-    if (ahead < k) atomicMin(&s.bound_key, best);
-    __syncthreads();
-    bound_key = s.bound_key;
-    const bool tie = best == bound_key;
-    if (tie) {
-      s.list_id[atomicAdd(&s.ties, 1u)] = best_id;
-      s.ahead = ahead;  // the same for every tie
-    }
-    __syncthreads();
-    // Of the threads at that key, the one whose id is k - ahead in order.
-    const uint32_t ties = s.ties, place = k - 1 - s.ahead;
-    if (tie) {
-      uint32_t lower = 0;
-      for (uint32_t t = 0; t < ties; ++t) lower += s.list_id[t] < best_id;
-      if (lower == place) s.bound_id = best_id;
-    }
-    __syncthreads();
-    bound_id = s.bound_id;
-  }
+  __syncthreads();
+  // Every wave finds the cut by itself.
+  uint32_t unit[U], unit_id[U], present = 0;
 #pragma unroll
-  for (uint32_t i = 0; i < N; ++i)
-    if (key[i] > bound_key || (key[i] == bound_key && id[i] <= bound_id)) {
-      const uint32_t at = atomicAdd(&s.count, 1u);
-      s.list_key[at] = key[i];
-      s.list_id[at] = id[i];
+  for (uint32_t u = 0; u < U; ++u) {
+    unit[u] = s.unit_key[lane * U + u];
+    unit_id[u] = s.unit_id[lane * U + u];
+    present += (uint32_t)__popcll(ballot(unit[u] != 0));
+  }
+  uint32_t cut = 1, cut_id = 0xffffffffu;  // everything
+  if (present >= k) {
+    cut = kth_largest<U, 32>(unit, k);
+    uint32_t ahead = 0, ties = 0, tie_id[U], last = 0;
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      ahead += (uint32_t)__popcll(ballot(unit[u] > cut));
+      ties += (uint32_t)__popcll(ballot(unit[u] == cut));
+      // Ids from the top down, so that the lowest is the largest.
+      tie_id[u] = unit[u] == cut ? (1u << kIdBits) - 1u - unit_id[u] : 0u;
+      last = max(last, unit[u] == cut ? unit_id[u] : 0u);
     }
+    if (ahead + ties == k)
+      cut_id = wave_max_u32(last);
+    else
+      cut_id = (1u << kIdBits) - 1u - kth_largest<U, kIdBits>(tie_id, k - ahead);
+  }
+  if (own > cut || (own == cut && own_id <= cut_id)) {
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i)
+      if (key[i] > cut || (key[i] == cut && id[i] <= cut_id))
+        s.item[atomicAdd(&s.count, 1u)] = make_uint2(key[i], id[i]);
+  }
   __syncthreads();
   return s.count;
 }
 
-// The place of list item i among the n listed ones.
-__device__ __forceinline__ uint32_t place_of(const TopLds &s, uint32_t n, uint32_t key,
-                                             uint32_t id) {
+// The place of an item among the n listed ones.
+__device__ __forceinline__ uint32_t place_of(const TopList &s, uint32_t n, uint2 item) {
   uint32_t place = 0;
+#pragma unroll 8
   for (uint32_t j = 0; j < n; ++j) {
-    const uint32_t other = s.list_key[j];
-    place += other > key || (other == key && s.list_id[j] < id) ? 1u : 0u;
+    const uint2 other = s.item[j];
+    place += other.x > item.x || (other.x == item.x && other.y < item.y) ? 1u : 0u;
   }
   return place;
 }
 
-// The row's best groups into s.best; returns their number, at most
-// kTopLogprobs and at least the k best.
-template <uint32_t N>
-__device__ __forceinline__ uint32_t best_groups(TopLds &s, const float *maxima, uint32_t groups,
-                                                uint32_t k) {
+// The row's best groups; `best` receives them. Returns their number, at most
+// kTopLogprobs, the k best among them.
+template <uint32_t N, uint32_t U>
+__device__ __forceinline__ uint32_t best_groups(TopList &s, uint32_t *best, const float *maxima,
+                                                uint32_t groups, uint32_t k) {
   const uint32_t tid = threadIdx.x;
+  float m[N];
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i)
+    m[i] = maxima[min(i * 256 + tid, groups - 1)];
   uint32_t key[N], id[N];
 #pragma unroll
   for (uint32_t i = 0; i < N; ++i) {
     id[i] = i * 256 + tid;
-    key[i] = id[i] < groups ? listed_key(maxima[id[i]]) : 0u;
+    key[i] = id[i] < groups ? listed_key(m[i]) : 0u;
   }
-  const uint32_t n = list_best(s, k, key, id);
+  const uint32_t n = list_best<N, U>(s, k, key, id);
   if (n <= kTopLogprobs) {
-    if (tid < n) s.best[tid] = s.list_id[tid];
+    if (tid < n) best[tid] = s.item[tid].y;
   } else {
     for (uint32_t i = tid; i < n; i += 256) {
-      const uint32_t place = place_of(s, n, s.list_key[i], s.list_id[i]);
-      if (place < k) s.best[place] = s.list_id[i];
+      const uint32_t place = place_of(s, n, s.item[i]);
+      if (place < k) best[place] = s.item[i].y;
     }
   }
   __syncthreads();
+  if (tid == 0) s.count = 0;  // ordered by the next list's barrier before its items
   return n <= kTopLogprobs ? n : k;
 }
 
-// The row's k best tokens from its best groups: a wave reads a group a load.
-template <int DT, uint32_t N>
-__device__ __forceinline__ void best_tokens(TopLds &s, const ScoreLaunch &a, uint32_t row,
-                                            const typename Logits<DT>::Element *x, uint32_t n,
-                                            const RowScore &score) {
+// The row's k best tokens from its n best groups: a wave reads a group a load.
+template <int DT, uint32_t N, uint32_t U>
+__device__ __forceinline__ void best_tokens(TopList &s, const uint32_t *best, const ScoreLaunch &a,
+                                            uint32_t row, const typename Logits<DT>::Element *x,
+                                            uint32_t n, const RowScore &score) {
   const uint32_t tid = threadIdx.x, k = a.top;
+  float v[N];
   uint32_t key[N], id[N];
 #pragma unroll
   for (uint32_t i = 0; i < N; ++i) {
     const uint32_t slot = i * 4 + (tid >> 6);
-    id[i] = slot < n ? s.best[slot] * kScoreGroup + (tid & 63u) : 0xffffffffu;
-    key[i] = id[i] < a.vocabulary ? listed_key(logit_value(x[id[i]])) : 0u;
+    id[i] = best[min(slot, n - 1)] * kScoreGroup + (tid & 63u);
+    v[i] = logit_value(x[min(id[i], a.vocabulary - 1)]);
   }
-  const uint32_t m = list_best(s, k, key, id);
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i)
+    key[i] = i * 4 + (tid >> 6) < n && id[i] < a.vocabulary ? listed_key(v[i]) : 0u;
+  const uint32_t m = list_best<N, U>(s, k, key, id);
   uint32_t *ids = a.out_top_ids + (uint64_t)row * k;
   float *logprobs = a.out_top_logprobs + (uint64_t)row * k;
   for (uint32_t i = tid; i < m; i += 256) {
-    const uint32_t item = s.list_key[i], token = s.list_id[i];
-    const uint32_t place = place_of(s, m, item, token);
+    const uint2 item = s.item[i];
+    const uint32_t place = place_of(s, m, item);
     if (place < k) {
-      ids[place] = token;
-      logprobs[place] = score.logprob(key_logit(item));
+      ids[place] = item.y;
+      logprobs[place] = score.logprob(key_logit(item.x));
     }
   }
   for (uint32_t i = m + tid; i < k; i += 256) {
     ids[i] = kNoToken;
     logprobs[i] = -__builtin_inff();
+  }
+}
+
+template <int DT, uint32_t U>
+__device__ __forceinline__ void row_best(TopList &s, uint32_t *best, const ScoreLaunch &a,
+                                         uint32_t row, const typename Logits<DT>::Element *x,
+                                         const RowScore &score) {
+  const float *maxima = a.maxima + (uint64_t)row * a.groups;
+  uint32_t n;
+  if (a.groups <= 10 * 256)
+    n = best_groups<10, U>(s, best, maxima, a.groups, a.top);
+  else if (a.groups <= 16 * 256)
+    n = best_groups<16, U>(s, best, maxima, a.groups, a.top);
+  else
+    n = best_groups<kMostItems, U>(s, best, maxima, a.groups, a.top);
+  if (n == 0) {  // nothing to list
+    for (uint32_t i = threadIdx.x; i < a.top; i += 256) {
+      a.out_top_ids[(uint64_t)row * a.top + i] = kNoToken;
+      a.out_top_logprobs[(uint64_t)row * a.top + i] = -__builtin_inff();
+    }
+  } else if (U == 1 && n <= 8 * 4) {
+    best_tokens<DT, 8, U>(s, best, a, row, x, n, score);
+  } else {
+    best_tokens<DT, kMostItems, U>(s, best, a, row, x, n, score);
   }
 }
 
@@ -365,30 +413,25 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void logprobs_kernel(ScoreLaunch a)
   if (tid == 0 && a.out_lse) a.out_lse[row] = score.lse();
   for (uint32_t i = tid; i < a.token_count; i += THREADS) {
     const uint32_t token = a.tokens[(uint64_t)row * a.token_stride + i];
-    const bool known = token < a.vocabulary;
-    if (a.out_logprobs)
-      a.out_logprobs[(uint64_t)row * a.token_count + i] =
-          known ? score.logprob(logit_value(x[token])) : -__builtin_inff();
-    if (i == 0 && a.out_ranks) {
-      uint32_t rank = 1;
-      for (uint32_t g = 0; g < a.segments; ++g) rank += a.aheads[(uint64_t)row * a.segments + g];
-      a.out_ranks[row] = known ? rank : 0u;
-    }
+    a.out_logprobs[(uint64_t)row * a.token_count + i] =
+        token < a.vocabulary ? score.logprob(logit_value(x[token])) : -__builtin_inff();
+  }
+  if (a.out_ranks && tid < 64) {
+    const uint32_t ahead =
+        wave_sum_u32(tid < a.segments ? a.aheads[(uint64_t)row * a.segments + tid] : 0u);
+    if (tid == 0)
+      a.out_ranks[row] =
+          a.tokens[(uint64_t)row * a.token_stride] < a.vocabulary ? ahead + 1u : 0u;
   }
   if constexpr (TOP) {
-    __shared__ TopLds s;
-    const float *maxima = a.maxima + (uint64_t)row * a.groups;
-    uint32_t n;
-    if (a.groups <= 8 * 256)
-      n = best_groups<8>(s, maxima, a.groups, a.top);
-    else if (a.groups <= 16 * 256)
-      n = best_groups<16>(s, maxima, a.groups, a.top);
+    __shared__ TopList s;
+    __shared__ uint32_t best[kTopLogprobs];
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    if (a.top <= kQuadTop)
+      row_best<DT, 1>(s, best, a, row, x, score);
     else
-      n = best_groups<kMostItems>(s, maxima, a.groups, a.top);
-    if (n <= 8 * 4)
-      best_tokens<DT, 8>(s, a, row, x, n, score);
-    else
-      best_tokens<DT, kMostItems>(s, a, row, x, n, score);
+      row_best<DT, 4>(s, best, a, row, x, score);
   }
 }
 
