@@ -4,37 +4,66 @@
 // with the same policy draws from.
 //
 // Only a few tokens of a row are edited: the row's penalty entries, its extra
-// tokens and its biases, sorted lists in buckets of 2048 tokens. A block takes
-// one chunk of a row. It works the chunk's edited values out first, in fp32,
-// in three steps with a barrier between them (penalties, extra tokens that the
-// table does not hold, biases on what the first two left), into an LDS tile
-// that is written only at those tokens, with a bitmap of them; then the
-// chunk's vectors go from registers to the output, each lane replacing what
-// the bitmap and the mask words say.
+// tokens and its biases, lists sorted by token. A block takes one chunk of a
+// row. Each list's entries of the chunk go to LDS in their order, a thread an
+// entry: a penalty entry as its finished value (it reads its own logit), a bias
+// as it is, with a bitmap of the list's tokens and, for each of its words, the
+// place of the word's first entry. Then the chunk's vectors go from registers
+// to the output; the lane that holds an edited token finds its entry by the
+// word's first place and the bits before it. That keeps a block at 13 KB of
+// LDS, eight blocks on a CU: what bounds the kernel is the chain of dependent
+// loads (row record, list bounds and mask, entries and vectors, entries'
+// logits), and the chunks in flight hide it. (A tile of 8192 values in LDS held
+// four blocks: 256 masked rows x 248,320 bf16 took 73 us.)
 //
-// A vector is loaded only if one of its tokens is admitted and not edited, and
-// in place written only if one of them changes: a grammar's row, which drops
-// nearly all of its tokens, is written without being read, and an unmasked row
-// in place touches nothing but its edits.
+// A vector is loaded only if one of its tokens is admitted, and in place
+// written only if one of them changes: a grammar's row, which drops nearly all
+// of its tokens, is written without being read, and an unmasked row in place
+// touches nothing but the vectors of its edits.
 #include <hip/hip_runtime.h>
 
+#include "jf_kernels.h"
 #include "jf_logits.h"
 
 namespace jf {
 
 namespace {
 
+constexpr uint32_t kMapWords = kScoreChunk / 32;
+constexpr uint32_t kStaged = 1024;  // a list's entries in LDS; later ones stay in memory
+
+// A list's entries of the chunk.
+struct ListLds {
+  uint32_t bits[kMapWords];
+  uint16_t first[kMapWords];  // of a word with any bit
+  float value[kStaged];
+};
 struct ProcessLds {
-  float value[kScoreChunk];              // written and read at edited tokens only
-  uint32_t edited[kScoreChunk / 32];
-  uint32_t admitted[kScoreChunk / 32];
-  uint32_t extras[16];
+  ListLds penalty, bias;
+  uint32_t admitted[kMapWords];
+  uint32_t extra_bits[kMapWords];  // extra tokens that the table does not hold
+  uint32_t extras[kMaxExtra];
+  float extra_value[kMaxExtra];
 };
 
 // VEC bits of a bitmap from token `at` of the chunk (a multiple of VEC).
 template <uint32_t VEC>
 __device__ __forceinline__ uint32_t bits_at(const uint32_t *map, uint32_t at) {
   return (map[at >> 5] >> (at & 31u)) & ((1u << VEC) - 1u);
+}
+__device__ __forceinline__ bool bit_at(const uint32_t *map, uint32_t at) {
+  return map[at >> 5] >> (at & 31u) & 1u;
+}
+// The place in its list's chunk of the entry of token `at`, which it holds.
+__device__ __forceinline__ uint32_t place_at(const ListLds &l, uint32_t at) {
+  return l.first[at >> 5] + __popc(l.bits[at >> 5] & ((1u << (at & 31u)) - 1u));
+}
+// Entry i of a list's chunk: its bit, and its place if it begins a word.
+__device__ __forceinline__ void mark(ListLds &l, const PenaltyEntry *list, uint32_t i,
+                                     uint32_t token, uint32_t base) {
+  const uint32_t at = token - base;
+  atomicOr(&l.bits[at >> 5], 1u << (at & 31u));
+  if (i == 0 || (list[i - 1].token - base) >> 5 != at >> 5) l.first[at >> 5] = (uint16_t)i;
 }
 
 template <int DI, int DO>
@@ -55,20 +84,20 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
   LogitWords w[LOADS];
   if (whole) load_chunk<DI>(x, base, V, 0, w);
 
-  uint32_t pen0 = 0, pen1 = 0, bias0 = 0, bias1 = 0;
+  uint32_t pen0 = 0, pens = 0, bias0 = 0, biases = 0;
   const uint32_t b0 = chunk * (kScoreChunk / kPenaltyBucket);
   const uint32_t b1 = min(b0 + kScoreChunk / kPenaltyBucket, a.buckets);
   if (p.penalty_row != kNoRow) {
     const uint32_t *off = a.pen_offsets + (uint64_t)p.penalty_row * (a.buckets + 1);
     pen0 = off[b0];
-    pen1 = off[b1];
+    pens = off[b1] - pen0;
   }
   if (p.bias_row != kNoRow) {
     const uint32_t *off = a.bias_offsets + (uint64_t)p.bias_row * (a.buckets + 1);
     bias0 = off[b0];
-    bias1 = off[b1];
+    biases = off[b1] - bias0;
   }
-  s.edited[tid] = 0;
+  s.penalty.bits[tid] = s.bias.bits[tid] = s.extra_bits[tid] = 0;
   if (masked) {
     // Tokens past the vocabulary are never stored; words past it not read.
     const uint32_t word = base / 32 + tid;
@@ -82,80 +111,76 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
     s.admitted[tid] = bits;
   }
   if (tid < p.extra_count) s.extras[tid] = a.extra[p.extra_offset + tid];
-  const bool edits = pen1 > pen0 || bias1 > bias0 || p.extra_count;
+  const bool edits = pens || biases || p.extra_count;
   if (edits || masked) __syncthreads();
-  // A dropped token's edits are not worked out, nor its logit read.
-  const auto dropped = [&](uint32_t at) {
-    return masked && !(s.admitted[at >> 5] >> (at & 31u) & 1u);
-  };
-  if (pen1 > pen0) {
-    const PenaltyEntry *list = a.pen_entries + (uint64_t)p.penalty_row * a.pen_max_entries;
-    for (uint32_t i = pen0 + tid; i < pen1; i += 256) {
-      const PenaltyEntry e = list[i];
-      const uint32_t at = e.token - base;
-      if (dropped(at)) continue;
-      uint32_t count = e.word & kCountMask;
-      for (uint32_t k = 0; k < p.extra_count; ++k) count += s.extras[k] == e.token;
-      s.value[at] = penalize(logit_value(x[e.token]), count, p.repetition, p.repetition_inverse,
-                             p.presence, p.frequency);
-      atomicOr(&s.edited[at >> 5], 1u << (at & 31u));
+  if (!whole && !a.in_place) {
+#pragma unroll
+    for (uint32_t j = 0; j < LOADS; ++j) {
+      const uint32_t at = j * SLAB + tid * VEC;
+      w[j] = LogitWords{};
+      if (base + at < V && bits_at<VEC>(s.admitted, at)) w[j] = load_words<DI>(x, base + at, V, 0);
     }
+  }
+  const PenaltyEntry *pen_list =
+      a.pen_entries + (uint64_t)p.penalty_row * a.pen_max_entries + pen0;
+  const PenaltyEntry *bias_list =
+      a.bias_entries + (uint64_t)p.bias_row * a.bias_max_entries + bias0;
+  const auto penalized = [&](const PenaltyEntry &e, float logit) {
+    uint32_t count = e.word & kCountMask;
+    for (uint32_t k = 0; k < p.extra_count; ++k) count += s.extras[k] == e.token;
+    return penalize(logit, count, p.repetition, p.repetition_inverse, p.presence, p.frequency);
+  };
+  for (uint32_t i = tid; i < biases; i += 256) {
+    const PenaltyEntry e = bias_list[i];
+    mark(s.bias, bias_list, i, e.token, base);
+    if (i < kStaged) s.bias.value[i] = u2f(e.word);
+  }
+  for (uint32_t i = tid; i < pens; i += 256) {
+    const PenaltyEntry e = pen_list[i];
+    mark(s.penalty, pen_list, i, e.token, base);
+    // A dropped token's value is never taken, nor its logit read.
+    if (i < kStaged && !(masked && !bit_at(s.admitted, e.token - base)))
+      s.penalty.value[i] = penalized(e, logit_value(x[e.token]));
   }
   if (p.extra_count) {
-    // Extra tokens outside the table, each at its first place in the list.
     __syncthreads();
     if (tid < p.extra_count) {
-      const uint32_t token = s.extras[tid], at = token - base;
-      bool take = token < V && at < kScoreChunk && !dropped(at) &&
-                  !(s.edited[at >> 5] >> (at & 31u) & 1u);
-      uint32_t count = 0;
-      for (uint32_t k = 0; k < p.extra_count; ++k) {
-        count += s.extras[k] == token;
-        take = take && !(k < tid && s.extras[k] == token);
-      }
-      // One wave holds all of them: its reads of the bitmap come before this.
-      if (take) {
-        s.value[at] = penalize(logit_value(x[token]), count, p.repetition, p.repetition_inverse,
-                               p.presence, p.frequency);
-        atomicOr(&s.edited[at >> 5], 1u << (at & 31u));
-      }
-    }
-  }
-  if (bias1 > bias0) {
-    __syncthreads();
-    const PenaltyEntry *list = a.bias_entries + (uint64_t)p.bias_row * a.bias_max_entries;
-    for (uint32_t i = bias0 + tid; i < bias1; i += 256) {
-      const PenaltyEntry e = list[i];
+      const PenaltyEntry e{s.extras[tid], 0};
       const uint32_t at = e.token - base;
-      if (dropped(at)) continue;
-      const float bias = u2f(e.word);
-      // Only this token's own bias can set its bit meanwhile.
-      const float v = s.edited[at >> 5] >> (at & 31u) & 1u ? s.value[at] : logit_value(x[e.token]);
-      // A ban holds whatever the logit.
-      s.value[at] = bias == -__builtin_inff() ? bias : v + bias;
-      atomicOr(&s.edited[at >> 5], 1u << (at & 31u));
+      if (e.token < V && at < kScoreChunk && !bit_at(s.penalty.bits, at)) {
+        // A token that comes more than once leaves the same value each time.
+        s.extra_value[tid] = penalized(e, logit_value(x[e.token]));
+        atomicOr(&s.extra_bits[at >> 5], 1u << (at & 31u));
+      }
     }
   }
   if (edits) __syncthreads();
 
-  if (!whole) {
+  // The tokens of a vector that some list edits.
+  const auto edited_at = [&](uint32_t at) {
+    return edits ? bits_at<VEC>(s.penalty.bits, at) | bits_at<VEC>(s.bias.bits, at) |
+                       bits_at<VEC>(s.extra_bits, at)
+                 : 0u;
+  };
+  if (a.in_place) {
 #pragma unroll
     for (uint32_t j = 0; j < LOADS; ++j) {
-      const uint32_t at = j * SLAB + tid * VEC, token = base + at;
-      if (token >= V) continue;
-      const uint32_t edited = edits ? bits_at<VEC>(s.edited, at) : 0u;
-      const uint32_t admitted = masked ? bits_at<VEC>(s.admitted, at) : ALL;
-      const bool write = !a.in_place || edited || admitted != ALL;
+      const uint32_t at = j * SLAB + tid * VEC;
       w[j] = LogitWords{};
-      if (write && (admitted & ~edited)) w[j] = load_words<DI>(x, token, V, 0);
+      if (base + at >= V) continue;
+      const uint32_t admitted = masked ? bits_at<VEC>(s.admitted, at) : ALL;
+      if (admitted && (admitted != ALL || edited_at(at)))
+        w[j] = load_words<DI>(x, base + at, V, 0);
     }
+    // A neighbour's edit reads no logit that this block writes: every read of
+    // a list's logit came before the barrier above.
   }
 #pragma unroll
   for (uint32_t j = 0; j < LOADS; ++j) {
     const uint32_t at = j * SLAB + tid * VEC, token = base + at;
     if (token >= V) continue;
-    const uint32_t edited = edits ? bits_at<VEC>(s.edited, at) : 0u;
     const uint32_t admitted = masked ? bits_at<VEC>(s.admitted, at) : ALL;
+    const uint32_t edited = edited_at(at) & admitted;
     if (a.in_place && !edited && admitted == ALL) continue;
     if (DI == DO && !edited && admitted == ALL) {
       store_words<DO>(y, token, V, w[j]);
@@ -163,11 +188,29 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
     }
     float v[VEC];
     unpack<DI>(w[j], v);
+    if (edited) {
 #pragma unroll
-    for (uint32_t e = 0; e < VEC; ++e) {
-      if (edited >> e & 1u) v[e] = s.value[at + e];
-      if (!(admitted >> e & 1u)) v[e] = -__builtin_inff();
+      for (uint32_t e = 0; e < VEC; ++e) {
+        if (!(edited >> e & 1u)) continue;
+        if (bit_at(s.penalty.bits, at + e)) {
+          const uint32_t i = place_at(s.penalty, at + e);
+          v[e] = i < kStaged ? s.penalty.value[i] : penalized(pen_list[i], v[e]);
+        } else if (bit_at(s.extra_bits, at + e)) {
+          uint32_t k = 0;
+          while (s.extras[k] != token + e) ++k;
+          v[e] = s.extra_value[k];
+        }
+        if (bit_at(s.bias.bits, at + e)) {
+          const uint32_t i = place_at(s.bias, at + e);
+          const float bias = i < kStaged ? s.bias.value[i] : u2f(bias_list[i].word);
+          // A ban holds whatever the logit.
+          v[e] = bias == -__builtin_inff() ? bias : v[e] + bias;
+        }
+      }
     }
+#pragma unroll
+    for (uint32_t e = 0; e < VEC; ++e)
+      if (!(admitted >> e & 1u)) v[e] = -__builtin_inff();
     if constexpr (DI == DO) {
       store_words<DO>(y, token, V, pack<DO>(v));
     } else if constexpr (DI == 1) {

@@ -34,7 +34,7 @@ POLICIES = [dict(), dict(repetition=1.3), dict(presence=0.7, frequency=0.2),
 
 
 def _run(V, rows, dtype, out_dtype, pad=0, lead=0, out_pad=0, in_place=False, seed=0, x=None,
-         biases=7, extras=True):
+         biases=7, extras=True, history=900):
     """Every row its own policy; returns nothing, checks every element."""
     import torch
     print(f"process V={V} rows={rows} {dtype}->{out_dtype} pad={pad} lead={lead} "
@@ -46,7 +46,7 @@ def _run(V, rows, dtype, out_dtype, pad=0, lead=0, out_pad=0, in_place=False, se
         x = bf16(x)
     policies = [J.policy(**POLICIES[r % len(POLICIES)]) for r in range(rows)]
     stops = (V // 2, V - 1)
-    n = max(2, min(V, 900))
+    n = max(2, min(2 * V, history))
     table = J.PenaltyTable(V, rows, n + 8)
     words, bias, extra = [], [], np.zeros((rows, 5), np.uint32)
     bias_table = J.BiasTable(V, rows, max(1, biases))
@@ -117,9 +117,13 @@ def test_in_place(V, dtype):
     _run(V, 9, dtype, dtype, pad=3, lead=1, in_place=True)
 
 
-def test_long_lists_fill_a_chunk():
-    """More entries and biases than a block has threads, in one chunk."""
-    _run(3001, 8, "f32", "f32", biases=700, extras=False)
+@pytest.mark.parametrize("biases,history", [(700, 900), (3001, 900), (10, 12000), (2500, 12000)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_long_lists_fill_a_chunk(biases, history, in_place):
+    """More entries and biases than a block has threads, and than its LDS
+    stages, in one chunk."""
+    _run(9001 if history > 9000 else 3001, 8, "f32", "f32", biases=biases, history=history,
+         in_place=in_place)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
