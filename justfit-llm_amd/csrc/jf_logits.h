@@ -108,20 +108,21 @@ __device__ __forceinline__ LogitWords load_words(const typename Logits<DT>::Elem
   }
   return w;
 }
-// A thread's vectors of the chunk at `base`. One branch for the chunk: with one
-// a vector the compiler keeps every vector's ways apart in registers.
-template <int DT>
+// A thread's vectors of the chunk of N slabs at `base`. One branch for the
+// chunk: with one a vector the compiler keeps every vector's ways apart in
+// registers.
+template <int DT, uint32_t N>
 __device__ __forceinline__ void load_chunk(const typename Logits<DT>::Element *row, uint32_t base,
                                            uint32_t vocabulary, uint32_t past,
-                                           LogitWords (&w)[kLoads<DT>]) {
+                                           LogitWords (&w)[N]) {
   const uint32_t token = base + threadIdx.x * Logits<DT>::VEC;
-  if (base + kScoreChunk <= vocabulary) {
+  if (base + N * kSlab<DT> <= vocabulary) {
 #pragma unroll
-    for (uint32_t j = 0; j < kLoads<DT>; ++j)
+    for (uint32_t j = 0; j < N; ++j)
       w[j] = *(const typename Logits<DT>::Words *)(row + token + j * kSlab<DT>);
   } else {
 #pragma unroll
-    for (uint32_t j = 0; j < kLoads<DT>; ++j)
+    for (uint32_t j = 0; j < N; ++j)
       w[j] = load_words<DT>(row, token + j * kSlab<DT>, vocabulary, past);
   }
 }

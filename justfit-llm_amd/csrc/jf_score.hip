@@ -77,118 +77,6 @@ __device__ __forceinline__ uint32_t listed_key(float x) {
   return x > -__builtin_inff() ? logit_key(x) : 0u;
 }
 
-template <int DT, bool TOP, bool RANK>
-__global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
-  constexpr uint32_t VEC = Logits<DT>::VEC, SLAB = kSlab<DT>, LOADS = kLoads<DT>;
-  __shared__ MaxSum wave_part[4];
-  __shared__ uint32_t wave_ahead[4];
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-  const uint32_t row = blockIdx.x / a.segments, segment = blockIdx.x - row * a.segments;
-  const uint32_t V = a.vocabulary;
-  const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
-  const float c = inverse_temperature(a, row) * kLog2e;
-  uint32_t target = 0xffffffffu;
-  float at_target = 0.0f, above_target = 0.0f;
-  uint32_t ahead = 0;
-  if constexpr (RANK) {
-    target = a.tokens[(uint64_t)row * a.token_stride];
-    if (target < V) {
-      at_target = logit_value(x[target]);
-      above_target = next_up(at_target);
-    }
-  }
-  MaxSum run{-__builtin_inff(), 0.0f};
-  const uint32_t first = segment * a.segment_chunks;
-  const uint32_t last = min(first + a.segment_chunks, (V + kScoreChunk - 1) / kScoreChunk);
-  for (uint32_t chunk = first; chunk < last; ++chunk) {
-    const uint32_t base = chunk * kScoreChunk;
-    LogitWords w[LOADS];
-    load_chunk<DT>(x, base, V, kPastMinusInfinity<DT>, w);
-    float part[LOADS], m = -__builtin_inff();
-#pragma unroll
-    for (uint32_t j = 0; j < LOADS; ++j) {
-      float v[VEC];
-      unpack<DT>(w[j], v);
-      part[j] = v[0];
-#pragma unroll
-      for (uint32_t e = 1; e < VEC; ++e) part[j] = __builtin_fmaxf(part[j], v[e]);
-      m = __builtin_fmaxf(m, part[j]);
-    }
-    // A NaN maximum: every value of the thread is NaN.
-    const float grown = __builtin_fmaxf(run.m, m), r = finite_reference(grown);
-    float s = run.s * exp_below(run.m, r, c);
-#pragma unroll
-    for (uint32_t j = 0; j < LOADS; ++j) {
-      float v[VEC];
-      unpack<DT>(w[j], v);
-#pragma unroll
-      for (uint32_t e = 0; e < VEC; ++e) s += exp_below(v[e], r, c);
-    }
-    run = {grown, s};
-    if constexpr (RANK) {
-      if (target < V) {
-        // Ids before the target's are ahead of it at equal logits too.
-        const bool mixed = target - base < kScoreChunk;
-        const float least = base < target ? at_target : above_target;
-#pragma unroll
-        for (uint32_t j = 0; j < LOADS; ++j) {
-          float v[VEC];
-          unpack<DT>(w[j], v);
-#pragma unroll
-          for (uint32_t e = 0; e < VEC; ++e) {
-            const float from =
-                mixed && base + j * SLAB + tid * VEC + e >= target ? above_target : least;
-            ahead += v[e] >= from ? 1u : 0u;
-          }
-        }
-      }
-    }
-    if constexpr (TOP) {
-      // A group's 64 tokens lie in 16 (f32) or 8 (bf16) neighbouring lanes.
-      float *maxima = a.maxima + (uint64_t)row * a.groups + chunk * kScoreChunkGroups;
-#pragma unroll
-      for (uint32_t j = 0; j < LOADS; ++j) {
-        float g = part[j];
-        g = __builtin_fmaxf(g, xor_f32<1>(g));
-        g = __builtin_fmaxf(g, xor_f32<2>(g));
-        g = __builtin_fmaxf(g, xor_f32<4>(g));
-        if constexpr (DT == 0) g = __builtin_fmaxf(g, xor_f32<8>(g));
-        if (tid % (kScoreGroup / VEC) == 0)
-          maxima[(j * SLAB + tid * VEC) / kScoreGroup] = g;
-      }
-    }
-  }
-  run = wave_join(run, c);
-  if constexpr (RANK) ahead = wave_sum_u32(ahead);
-  if (lane == 0) {
-    wave_part[wave] = run;
-    wave_ahead[wave] = ahead;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    const MaxSum all = join(join(wave_part[0], wave_part[1], c),
-                            join(wave_part[2], wave_part[3], c), c);
-    const uint64_t at = (uint64_t)row * a.segments + segment;
-    a.partials[at] = make_float2(all.m, all.s);
-    if constexpr (RANK)
-      a.aheads[at] = wave_ahead[0] + wave_ahead[1] + wave_ahead[2] + wave_ahead[3];
-  }
-}
-
-// ---- finish -----------------------------------------------------------------
-
-// The row's maximum and sum from its segments' (every lane of the wave gets
-// them). A row has at most 64 segments.
-__device__ __forceinline__ MaxSum row_total(const ScoreLaunch &a, uint32_t row, float c) {
-  MaxSum p{-__builtin_inff(), 0.0f};
-  const uint32_t lane = threadIdx.x & 63u;
-  if (lane < a.segments) {
-    const float2 v = a.partials[(uint64_t)row * a.segments + lane];
-    p = {v.x, v.y};
-  }
-  return wave_join(p, c);
-}
-
 // A row's totals as its outputs take them.
 struct RowScore {
   float m, inv_t, log_sum;
@@ -202,50 +90,111 @@ struct RowScore {
   }
 };
 
+// ---- the best tokens ----------------------------------------------------------
+
+// Element i of a row at a uniform address, by a 32-bit offset (a row's bytes
+// stay below 2^22): one address register a load.
+template <class T>
+__device__ __forceinline__ const T *element(const T *row, uint32_t i) {
+  return (const T *)((const char *)row + (uint32_t)(i * sizeof(T)));
+}
+
 constexpr uint32_t kMostItems = 32;  // groups, and then tokens, a thread holds at most
-// Lists of up to this many alternatives are cut by the best items of 64 quads
+constexpr uint32_t kListItems = 512;
+// Lists of up to this many alternatives are cut by the best groups of 64 quads
 // of lanes, longer ones by those of the 256 threads: a cut by fewer units is
-// quicker to find and lists more items.
+// quicker to find and lists more groups.
 constexpr uint32_t kQuadTop = 32;
-constexpr uint32_t kListItems = kMostItems * (kTopLogprobs - 1) + 1;
-static_assert(4 * kMostItems * (kQuadTop - 1) + 1 <= kListItems);
 constexpr uint32_t kIdBits = 20;  // tokens and groups are below 2^20
 
-struct TopList {
+struct TopLds {
   uint32_t unit_key[256], unit_id[256];
   uint2 item[kListItems];  // key, id
-  uint32_t count;
+  uint32_t best[kTopLogprobs];
+  uint64_t wave[2][4];
+  uint32_t count[2];
 };
 
-// The k-th largest (from 1) of the wave's 64 * U values below 2^BITS, found
-// bit by bit: the largest t that k values reach.
+// The k-th largest (from 1) of the wave's 64 * U values below 2^BITS, two bits
+// a step: the largest t that k values reach.
 template <uint32_t U, int BITS>
 __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[U], uint32_t k) {
+  static_assert(BITS % 2 == 0);
   uint32_t t = 0;
-#pragma unroll 4
-  for (int b = BITS - 1; b >= 0; --b) {
-    const uint32_t trial = t | 1u << b;
-    uint32_t reach = 0;
+#pragma unroll 2
+  for (int b = BITS - 2; b >= 0; b -= 2) {
+    uint32_t reach[3] = {};
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) reach += (uint32_t)__popcll(ballot(v[u] >= trial));
-    if (reach >= k) t = trial;
+    for (uint32_t u = 0; u < U; ++u) {
+#pragma unroll
+      for (uint32_t q = 0; q < 3; ++q)
+        reach[q] += (uint32_t)__popcll(ballot(v[u] >= (t | (q + 1) << b)));
+    }
+    t |= (reach[2] >= k ? 3u : reach[1] >= k ? 2u : reach[0] >= k ? 1u : 0u) << b;
   }
   return t;
 }
 
-// Lists in LDS, in no order, the block's items at or ahead of the k-th of its
-// units' best items (a unit: four lanes, or with U = 4 one thread), in the
-// order (key down, id up); key 0 is no item, and with fewer than k units that
-// have an item every one is listed. So the list holds the block's k best items.
-// An item on it belongs to one of those k units, the k-th of which has no other
-// one there: at most (k - 1) * 4 / U * N + 1 items. Returns their number.
-// s.count is 0 on entry, ordered by a barrier.
+// The block's `k` best items one by one, in the order (key down, id up), to
+// put(place, key, id) of every thread; key 0 is no item. each(take) gives a
+// thread's items to take(key, id). Returns how many there are. Any order of
+// items takes k rounds: for those that crowd the list.
+template <class Each, class Put>
+__device__ __forceinline__ uint32_t pick_best(TopLds &s, uint32_t k, const Each &each,
+                                              const Put &put) {
+  uint64_t last = ~0ull;
+  for (uint32_t place = 0; place < k; ++place) {
+    uint64_t best = 0;
+    each([&](uint32_t key, uint32_t id) {
+      const uint64_t item = (uint64_t)key << 32 | (0xffffffffu - id);
+      if (key && item < last && item > best) best = item;
+    });
+    const auto larger = [](uint64_t p, uint64_t q) { return p > q ? p : q; };
+    best = larger(best, xor_u64<1>(best));
+    best = larger(best, xor_u64<2>(best));
+    best = larger(best, xor_u64<4>(best));
+    best = larger(best, xor_u64<8>(best));
+    best = larger(best, xor_u64<16>(best));
+    best = larger(best, xor_u64<32>(best));
+    uint64_t *slot = s.wave[place & 1u];
+    if ((threadIdx.x & 63u) == 0) slot[threadIdx.x >> 6] = best;
+    __syncthreads();
+    last = larger(larger(slot[0], slot[1]), larger(slot[2], slot[3]));
+    if (last == 0) return place;
+    put(place, (uint32_t)(last >> 32), 0xffffffffu - (uint32_t)last);
+  }
+  return k;
+}
+
+// The place of an item among the n listed ones.
+__device__ __forceinline__ uint32_t place_of(const TopLds &s, uint32_t n, uint2 item) {
+  uint32_t place = 0;
+#pragma unroll 8
+  for (uint32_t j = 0; j < n; ++j) {
+    const uint2 other = s.item[j];
+    place += other.x > item.x || (other.x == item.x && other.y < item.y) ? 1u : 0u;
+  }
+  return place;
+}
+
+// The row's best groups by (maximum down, group up) into s.best: the k best
+// and, up to kTopLogprobs in all, perhaps more. Returns their number; `cut` is
+// a key that the k best groups' maxima reach (1 where there are fewer).
+//
+// A unit is four lanes (U = 1: 64 units) or one thread (U = 4: 256 of them).
+// The k-th of the units' best groups is not ahead of the row's k-th best one,
+// so the groups at or ahead of it hold the k best, with few others where the
+// best groups lie in different units.
 template <uint32_t N, uint32_t U>
-__device__ __forceinline__ uint32_t list_best(TopList &s, uint32_t k, const uint32_t (&key)[N],
-                                              const uint32_t (&id)[N]) {
+__device__ __forceinline__ uint32_t best_groups(TopLds &s, const float *maxima, uint32_t groups,
+                                                uint32_t k, uint32_t *cut_out) {
   static_assert(N <= kMostItems && (U == 1 || U == 4));
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
-  uint32_t best = 0, best_id = 0;
+  float m[N];
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i) m[i] = *element(maxima, min(i * 256 + tid, groups - 1));
+  uint32_t key[N], best = 0, best_id = 0;
+  const auto id_of = [&](uint32_t i) { return i * 256 + tid; };
   const auto take = [&](uint32_t other, uint32_t other_id) {
     if (other > best || (other == best && other_id < best_id)) {
       best = other;
@@ -253,8 +202,11 @@ __device__ __forceinline__ uint32_t list_best(TopList &s, uint32_t k, const uint
     }
   };
 #pragma unroll
-  for (uint32_t i = 0; i < N; ++i) take(key[i], id[i]);
-  const uint32_t own = best, own_id = best_id;
+  for (uint32_t i = 0; i < N; ++i) {
+    key[i] = id_of(i) < groups ? listed_key(m[i]) : 0u;
+    take(key[i], id_of(i));
+  }
+  const uint32_t own = best;
   if constexpr (U == 1) {
     take(xor_u32<1>(best), xor_u32<1>(best_id));
     take(xor_u32<2>(best), xor_u32<2>(best_id));
@@ -292,84 +244,91 @@ __device__ __forceinline__ uint32_t list_best(TopList &s, uint32_t k, const uint
     else
       cut_id = (1u << kIdBits) - 1u - kth_largest<U, kIdBits>(tie_id, k - ahead);
   }
-  if (own > cut || (own == cut && own_id <= cut_id)) {
+  *cut_out = cut;
+  if (own >= cut) {
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i)
-      if (key[i] > cut || (key[i] == cut && id[i] <= cut_id))
-        s.item[atomicAdd(&s.count, 1u)] = make_uint2(key[i], id[i]);
+      if (key[i] > cut || (key[i] == cut && id_of(i) <= cut_id)) {
+        const uint32_t at = atomicAdd(&s.count[0], 1u);
+        if (at < kListItems) s.item[at] = make_uint2(key[i], id_of(i));
+      }
   }
   __syncthreads();
-  return s.count;
-}
-
-// The place of an item among the n listed ones.
-__device__ __forceinline__ uint32_t place_of(const TopList &s, uint32_t n, uint2 item) {
-  uint32_t place = 0;
-#pragma unroll 8
-  for (uint32_t j = 0; j < n; ++j) {
-    const uint2 other = s.item[j];
-    place += other.x > item.x || (other.x == item.x && other.y < item.y) ? 1u : 0u;
-  }
-  return place;
-}
-
-// The row's best groups; `best` receives them. Returns their number, at most
-// kTopLogprobs, the k best among them.
-template <uint32_t N, uint32_t U>
-__device__ __forceinline__ uint32_t best_groups(TopList &s, uint32_t *best, const float *maxima,
-                                                uint32_t groups, uint32_t k) {
-  const uint32_t tid = threadIdx.x;
-  float m[N];
-#pragma unroll
-  for (uint32_t i = 0; i < N; ++i)
-    m[i] = maxima[min(i * 256 + tid, groups - 1)];
-  uint32_t key[N], id[N];
-#pragma unroll
-  for (uint32_t i = 0; i < N; ++i) {
-    id[i] = i * 256 + tid;
-    key[i] = id[i] < groups ? listed_key(m[i]) : 0u;
-  }
-  const uint32_t n = list_best<N, U>(s, k, key, id);
+  const uint32_t n = s.count[0];
   if (n <= kTopLogprobs) {
-    if (tid < n) best[tid] = s.item[tid].y;
-  } else {
+    if (tid < n) s.best[tid] = s.item[tid].y;
+  } else if (n <= kListItems) {
     for (uint32_t i = tid; i < n; i += 256) {
       const uint32_t place = place_of(s, n, s.item[i]);
-      if (place < k) best[place] = s.item[i].y;
+      if (place < k) s.best[place] = s.item[i].y;
     }
+  } else {
+    pick_best(
+        s, k,
+        [&](const auto &take_item) {
+          // Read again: held over the rounds they cost 150 registers.
+#pragma unroll 4
+          for (uint32_t id = tid; id < groups; id += 256)
+            take_item(listed_key(*element(maxima, id)), id);
+        },
+        [&](uint32_t place, uint32_t, uint32_t group) {
+          if (tid == 0) s.best[place] = group;
+        });
   }
   __syncthreads();
-  if (tid == 0) s.count = 0;  // ordered by the next list's barrier before its items
   return n <= kTopLogprobs ? n : k;
 }
 
-// The row's k best tokens from its n best groups: a wave reads a group a load.
-template <int DT, uint32_t N, uint32_t U>
-__device__ __forceinline__ void best_tokens(TopList &s, const uint32_t *best, const ScoreLaunch &a,
-                                            uint32_t row, const typename Logits<DT>::Element *x,
-                                            uint32_t n, const RowScore &score) {
+// The row's k best tokens from its n best groups: a wave reads a group a load,
+// eight in flight. The k best reach the groups' cut.
+template <int DT>
+__device__ __forceinline__ void best_tokens(TopLds &s, const ScoreLaunch &a, uint32_t row,
+                                            const typename Logits<DT>::Element *x, uint32_t n,
+                                            uint32_t cut, const RowScore &score) {
   const uint32_t tid = threadIdx.x, k = a.top;
-  float v[N];
-  uint32_t key[N], id[N];
-#pragma unroll
-  for (uint32_t i = 0; i < N; ++i) {
-    const uint32_t slot = i * 4 + (tid >> 6);
-    id[i] = best[min(slot, n - 1)] * kScoreGroup + (tid & 63u);
-    v[i] = logit_value(x[min(id[i], a.vocabulary - 1)]);
-  }
-#pragma unroll
-  for (uint32_t i = 0; i < N; ++i)
-    key[i] = i * 4 + (tid >> 6) < n && id[i] < a.vocabulary ? listed_key(v[i]) : 0u;
-  const uint32_t m = list_best<N, U>(s, k, key, id);
   uint32_t *ids = a.out_top_ids + (uint64_t)row * k;
   float *logprobs = a.out_top_logprobs + (uint64_t)row * k;
-  for (uint32_t i = tid; i < m; i += 256) {
-    const uint2 item = s.item[i];
-    const uint32_t place = place_of(s, m, item);
-    if (place < k) {
-      ids[place] = item.y;
-      logprobs[place] = score.logprob(key_logit(item.x));
+  constexpr uint32_t AHEAD = 8;
+  const auto each_token = [&](const auto &take) {
+    for (uint32_t first = 0; first < n; first += AHEAD * 4) {
+      uint32_t id[AHEAD];
+      float v[AHEAD];
+#pragma unroll
+      for (uint32_t i = 0; i < AHEAD; ++i) {
+        const uint32_t slot = first + i * 4 + (tid >> 6);
+        id[i] = s.best[min(slot, n - 1)] * kScoreGroup + (tid & 63u);
+        if (slot >= n) id[i] = a.vocabulary;
+        v[i] = logit_value(*element(x, min(id[i], a.vocabulary - 1)));
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < AHEAD; ++i)
+        take(id[i] < a.vocabulary ? listed_key(v[i]) : 0u, id[i]);
     }
+  };
+  each_token([&](uint32_t key, uint32_t id) {
+    if (key >= cut) {
+      const uint32_t at = atomicAdd(&s.count[1], 1u);
+      if (at < kListItems) s.item[at] = make_uint2(key, id);
+    }
+  });
+  __syncthreads();
+  uint32_t m = s.count[1];
+  if (m <= kListItems) {
+    for (uint32_t i = tid; i < m; i += 256) {
+      const uint2 item = s.item[i];
+      const uint32_t place = place_of(s, m, item);
+      if (place < k) {
+        ids[place] = item.y;
+        logprobs[place] = score.logprob(key_logit(item.x));
+      }
+    }
+  } else {
+    m = pick_best(s, k, each_token, [&](uint32_t place, uint32_t key, uint32_t id) {
+      if (tid == 0) {
+        ids[place] = id;
+        logprobs[place] = score.logprob(key_logit(key));
+      }
+    });
   }
   for (uint32_t i = m + tid; i < k; i += 256) {
     ids[i] = kNoToken;
@@ -378,119 +337,133 @@ __device__ __forceinline__ void best_tokens(TopList &s, const uint32_t *best, co
 }
 
 template <int DT, uint32_t U>
-__device__ __forceinline__ void row_best(TopList &s, uint32_t *best, const ScoreLaunch &a,
-                                         uint32_t row, const typename Logits<DT>::Element *x,
+__device__ __forceinline__ void row_best(TopLds &s, const ScoreLaunch &a, uint32_t row,
+                                         const typename Logits<DT>::Element *x,
                                          const RowScore &score) {
   const float *maxima = a.maxima + (uint64_t)row * a.groups;
-  uint32_t n;
+  uint32_t n, cut;
   if (a.groups <= 10 * 256)
-    n = best_groups<10, U>(s, best, maxima, a.groups, a.top);
+    n = best_groups<10, U>(s, maxima, a.groups, a.top, &cut);
   else if (a.groups <= 16 * 256)
-    n = best_groups<16, U>(s, best, maxima, a.groups, a.top);
+    n = best_groups<16, U>(s, maxima, a.groups, a.top, &cut);
   else
-    n = best_groups<kMostItems, U>(s, best, maxima, a.groups, a.top);
-  if (n == 0) {  // nothing to list
-    for (uint32_t i = threadIdx.x; i < a.top; i += 256) {
-      a.out_top_ids[(uint64_t)row * a.top + i] = kNoToken;
-      a.out_top_logprobs[(uint64_t)row * a.top + i] = -__builtin_inff();
-    }
-  } else if (U == 1 && n <= 8 * 4) {
-    best_tokens<DT, 8, U>(s, best, a, row, x, n, score);
-  } else {
-    best_tokens<DT, kMostItems, U>(s, best, a, row, x, n, score);
+    n = best_groups<kMostItems, U>(s, maxima, a.groups, a.top, &cut);
+  best_tokens<DT>(s, a, row, x, n, cut, score);
+}
+
+// ---- finish -------------------------------------------------------------------
+
+// The row's maximum and sum from its blocks' (every lane of the wave).
+__device__ __forceinline__ MaxSum row_total(const ScoreLaunch &a, uint32_t row, float c) {
+  MaxSum p{-__builtin_inff(), 0.0f};
+  for (uint32_t g = threadIdx.x & 63u; g < a.segments; g += 64) {
+    const float2 v = a.partials[(uint64_t)row * a.segments + g];
+    p = join(p, MaxSum{v.x, v.y}, c);
   }
+  return wave_join(p, c);
 }
 
 // One row a block: 256 threads with alternatives, otherwise a wave.
 template <int DT, bool TOP>
 __global__ __launch_bounds__(TOP ? 256 : 64) void logprobs_kernel(ScoreLaunch a) {
-  constexpr uint32_t THREADS = TOP ? 256 : 64;
   const uint32_t tid = threadIdx.x, row = blockIdx.x;
   const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
   const float inv_t = inverse_temperature(a, row);
   const MaxSum total = row_total(a, row, inv_t * kLog2e);
   const RowScore score{total.m, inv_t, logf(total.s)};
-  if (tid == 0 && a.out_lse) a.out_lse[row] = score.lse();
-  for (uint32_t i = tid; i < a.token_count; i += THREADS) {
-    const uint32_t token = a.tokens[(uint64_t)row * a.token_stride + i];
-    a.out_logprobs[(uint64_t)row * a.token_count + i] =
-        token < a.vocabulary ? score.logprob(logit_value(x[token])) : -__builtin_inff();
-  }
-  if (a.out_ranks && tid < 64) {
-    const uint32_t ahead =
-        wave_sum_u32(tid < a.segments ? a.aheads[(uint64_t)row * a.segments + tid] : 0u);
-    if (tid == 0)
-      a.out_ranks[row] =
-          a.tokens[(uint64_t)row * a.token_stride] < a.vocabulary ? ahead + 1u : 0u;
+  if (tid < 64) {
+    if (tid == 0 && a.out_lse) a.out_lse[row] = score.lse();
+    uint32_t ahead = 0;
+    if (a.out_ranks) {
+      for (uint32_t g = tid; g < a.segments; g += 64)
+        ahead += a.aheads[(uint64_t)row * a.segments + g];
+      ahead = wave_sum_u32(ahead);
+    }
+    for (uint32_t i = tid; i < a.token_count; i += 64) {
+      const uint32_t token = a.tokens[(uint64_t)row * a.token_stride + i];
+      const bool known = token < a.vocabulary;
+      a.out_logprobs[(uint64_t)row * a.token_count + i] =
+          known ? score.logprob(logit_value(x[token])) : -__builtin_inff();
+      if (i == 0 && a.out_ranks) a.out_ranks[row] = known ? ahead + 1u : 0u;
+    }
   }
   if constexpr (TOP) {
-    __shared__ TopList s;
-    __shared__ uint32_t best[kTopLogprobs];
-    if (tid == 0) s.count = 0;
-    __syncthreads();
+    __shared__ TopLds s;
+    if (tid < 2) s.count[tid] = 0;  // ordered by the units' barrier
     if (a.top <= kQuadTop)
-      row_best<DT, 1>(s, best, a, row, x, score);
+      row_best<DT, 1>(s, a, row, x, score);
     else
-      row_best<DT, 4>(s, best, a, row, x, score);
+      row_best<DT, 4>(s, a, row, x, score);
   }
 }
 
-__device__ __forceinline__ float block_max(float v, float *lds) {
-  v = wave_max_f32(v);
-  __syncthreads();
-  if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return __builtin_fmaxf(__builtin_fmaxf(lds[0], lds[1]), __builtin_fmaxf(lds[2], lds[3]));
-}
-__device__ __forceinline__ float block_sum(float v, float *lds) {
+__device__ __forceinline__ float wave_sum_f32(float v) {
   v += xor_f32<1>(v);
   v += xor_f32<2>(v);
   v += xor_f32<4>(v);
   v += xor_f32<8>(v);
   v += xor_f32<16>(v);
   v += xor_f32<32>(v);
+  return v;
+}
+// Over a block of THREADS (a wave, or four); `lds` is written before one
+// barrier and read after it.
+template <uint32_t THREADS>
+__device__ __forceinline__ float block_max(float v, float (&lds)[4]) {
+  v = wave_max_f32(v);
+  if constexpr (THREADS == 64) return v;
+  if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
+  return __builtin_fmaxf(__builtin_fmaxf(lds[0], lds[1]), __builtin_fmaxf(lds[2], lds[3]));
+}
+template <uint32_t THREADS>
+__device__ __forceinline__ float block_sum(float v, float (&lds)[4]) {
+  v = wave_sum_f32(v);
+  if constexpr (THREADS == 64) return v;
   if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   return (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
-// The distillation's loss of one row a block, one listed token a thread:
+// The distillation's loss of a row a block, one listed token a thread:
 // sum p_k (ln p_k - ln q_k), and what the backward pass takes: the row's
 // maximum, the list's mass over the row's sum, and each slot's probability
-// (-1: no token, or one that an earlier slot lists).
-template <int DT>
-__global__ __launch_bounds__(256) void distill_loss_kernel(ScoreLaunch a) {
-  __shared__ uint32_t listed[kTeacherTokens];
-  __shared__ float lds[4];
+// (-1: no token, or one that an earlier slot lists). Lists of up to 64 take a
+// wave, without a barrier.
+template <int DT, uint32_t THREADS>
+__global__ __launch_bounds__(THREADS) void distill_loss_kernel(ScoreLaunch a) {
+  __shared__ float lds[4][4];
+  __shared__ uint32_t listed[THREADS];
   const uint32_t tid = threadIdx.x, row = blockIdx.x, K = a.teacher_count;
   const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
-  const float inv_t = 1.0f / a.temperature;
   uint32_t id = kNoToken;
   float value = -__builtin_inff(), logit = 0.0f;
   if (tid < K) {
     id = a.teacher_ids[(uint64_t)row * a.teacher_stride + tid];
     value = a.teacher_values[(uint64_t)row * a.teacher_stride + tid];
   }
-  const MaxSum total = row_total(a, row, inv_t * kLog2e);
-  const RowScore score{total.m, inv_t, logf(total.s)};
-  listed[tid] = id;
-  __syncthreads();
   bool valid = id < a.vocabulary;
   if (valid) logit = logit_value(x[id]);
+  listed[tid] = id;
+  const float inv_t = 1.0f / a.temperature;
+  const MaxSum total = row_total(a, row, inv_t * kLog2e);
+  const RowScore score{total.m, inv_t, logf(total.s)};
+  __syncthreads();
+#pragma unroll 8
   for (uint32_t k = 0; k < K; ++k) valid = valid && !(k < tid && listed[k] == id);
   float log_p = valid ? value : -__builtin_inff();
   if (a.normalize) {
     log_p *= inv_t;
-    log_p -= finite_reference(block_max(log_p, lds));
-    const float log_sum = logf(block_sum(expf(log_p), lds));
+    log_p -= finite_reference(block_max<THREADS>(log_p, lds[0]));
+    const float log_sum = logf(block_sum<THREADS>(expf(log_p), lds[1]));
     // -infinity stays: a list of nothing else has no mass.
     if (log_p != -__builtin_inff()) log_p -= log_sum;
   }
   const float p = valid ? expf(log_p) : 0.0f;
   // A token of no teacher probability adds nothing, whatever the student's.
-  const float loss = block_sum(p == 0.0f ? 0.0f : p * (log_p - score.logprob(logit)), lds);
-  const float mass = block_sum(p, lds);
+  const float loss =
+      block_sum<THREADS>(p == 0.0f ? 0.0f : p * (log_p - score.logprob(logit)), lds[2]);
+  const float mass = block_sum<THREADS>(p, lds[3]);
   if (tid == 0) {
     a.out_loss[row] = loss;
     if (a.out_lse) a.out_lse[row] = score.lse();
@@ -506,43 +479,144 @@ __global__ __launch_bounds__(256) void distill_loss_kernel(ScoreLaunch a) {
   }
 }
 
+// ---- the pass -----------------------------------------------------------------
+
+// A block's segment of a row: chunks of N slabs.
+template <int DT, uint32_t N, bool RANK, bool TOP>
+__global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
+  constexpr uint32_t VEC = Logits<DT>::VEC, SLAB = kSlab<DT>, CHUNK = N * SLAB;
+  __shared__ MaxSum wave_part[4];
+  __shared__ uint32_t wave_ahead[4];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  const uint32_t row = blockIdx.x / a.segments, segment = blockIdx.x - row * a.segments;
+  const uint32_t V = a.vocabulary;
+  const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
+  const float c = inverse_temperature(a, row) * kLog2e;
+  uint32_t target = 0xffffffffu;
+  float at_target = 0.0f, above_target = 0.0f;
+  uint32_t ahead = 0;
+  if constexpr (RANK) {
+    target = a.tokens[(uint64_t)row * a.token_stride];
+    if (target < V) {
+      at_target = logit_value(x[target]);
+      above_target = next_up(at_target);
+    }
+  }
+  MaxSum run{-__builtin_inff(), 0.0f};
+  const uint32_t first = segment * a.segment_chunks;
+  const uint32_t last = min(first + a.segment_chunks, (V + CHUNK - 1) / CHUNK);
+  for (uint32_t chunk = first; chunk < last; ++chunk) {
+    const uint32_t base = chunk * CHUNK;
+    LogitWords w[N];
+    load_chunk<DT>(x, base, V, kPastMinusInfinity<DT>, w);
+    float part[N], m = -__builtin_inff();
+#pragma unroll
+    for (uint32_t j = 0; j < N; ++j) {
+      float v[VEC];
+      unpack<DT>(w[j], v);
+      part[j] = v[0];
+#pragma unroll
+      for (uint32_t e = 1; e < VEC; ++e) part[j] = __builtin_fmaxf(part[j], v[e]);
+      m = __builtin_fmaxf(m, part[j]);
+    }
+    // A NaN maximum: every value of the thread is NaN.
+    const float grown = __builtin_fmaxf(run.m, m), r = finite_reference(grown);
+    float s = run.s * exp_below(run.m, r, c);
+#pragma unroll
+    for (uint32_t j = 0; j < N; ++j) {
+      float v[VEC];
+      unpack<DT>(w[j], v);
+#pragma unroll
+      for (uint32_t e = 0; e < VEC; ++e) s += exp_below(v[e], r, c);
+    }
+    run = {grown, s};
+    if constexpr (RANK) {
+      if (target < V) {
+        // Ids before the target's are ahead of it at equal logits too.
+        const bool mixed = target - base < CHUNK;
+        const float least = base < target ? at_target : above_target;
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) {
+          float v[VEC];
+          unpack<DT>(w[j], v);
+#pragma unroll
+          for (uint32_t e = 0; e < VEC; ++e) {
+            const float from =
+                mixed && base + j * SLAB + tid * VEC + e >= target ? above_target : least;
+            ahead += v[e] >= from ? 1u : 0u;
+          }
+        }
+      }
+    }
+    if constexpr (TOP) {
+      // A group's 64 tokens lie in 16 (f32) or 8 (bf16) neighbouring lanes.
+      float *maxima = a.maxima + (uint64_t)row * a.groups + base / kScoreGroup;
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) {
+        float g = part[j];
+        g = __builtin_fmaxf(g, xor_f32<1>(g));
+        g = __builtin_fmaxf(g, xor_f32<2>(g));
+        g = __builtin_fmaxf(g, xor_f32<4>(g));
+        if constexpr (DT == 0) g = __builtin_fmaxf(g, xor_f32<8>(g));
+        if (tid % (kScoreGroup / VEC) == 0)
+          maxima[(j * SLAB + tid * VEC) / kScoreGroup] = g;
+      }
+    }
+  }
+  run = wave_join(run, c);
+  if constexpr (RANK) ahead = wave_sum_u32(ahead);
+  if (lane == 0) {
+    wave_part[wave] = run;
+    wave_ahead[wave] = ahead;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    const MaxSum total = join(join(wave_part[0], wave_part[1], c),
+                              join(wave_part[2], wave_part[3], c), c);
+    const uint64_t at = (uint64_t)row * a.segments + segment;
+    a.partials[at] = make_float2(total.m, total.s);
+    if constexpr (RANK)
+      a.aheads[at] = wave_ahead[0] + wave_ahead[1] + wave_ahead[2] + wave_ahead[3];
+  }
+}
+
 }  // namespace
 
 int launch_score(const ScoreLaunch &a, uint32_t dtype, void *stream) {
   const hipStream_t st = (hipStream_t)stream;
-  const dim3 grid(a.row_count * a.segments), block(256);
+  const dim3 grid(a.row_count * a.segments), rows(a.row_count);
   const bool top = a.top != 0, rank = a.out_ranks != nullptr;
-#define JF_SCORE(DT, TOP, RANK)                                                        \
-  if (dtype == DT && top == TOP && rank == RANK)                                       \
-  hipLaunchKernelGGL((score_kernel<DT, TOP, RANK>), grid, block, 0, st, a)
-  JF_SCORE(0, false, false);
-  JF_SCORE(0, false, true);
-  JF_SCORE(0, true, false);
-  JF_SCORE(0, true, true);
-  JF_SCORE(1, false, false);
-  JF_SCORE(1, false, true);
-  JF_SCORE(1, true, false);
-  JF_SCORE(1, true, true);
+#define JF_SCORE(DT, N, RANK, TOP)                                                       \
+  if (dtype == DT && (a.small != 0) == (N * kSlab<DT> == kSmallChunk) && rank == RANK && \
+      top == TOP)                                                                        \
+  hipLaunchKernelGGL((score_kernel<DT, N, RANK, TOP>), grid, dim3(256), 0, st, a)
+#define JF_SCORE_ALL(DT, N)      \
+  JF_SCORE(DT, N, false, false); \
+  JF_SCORE(DT, N, false, true);  \
+  JF_SCORE(DT, N, true, false);  \
+  JF_SCORE(DT, N, true, true)
+  JF_SCORE_ALL(0, kScoreChunk / kSlab<0>);
+  JF_SCORE_ALL(0, kSmallChunk / kSlab<0>);
+  JF_SCORE_ALL(1, kScoreChunk / kSlab<1>);
+  JF_SCORE_ALL(1, kSmallChunk / kSlab<1>);
+#undef JF_SCORE_ALL
 #undef JF_SCORE
-  hipError_t e = hipGetLastError();
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  const dim3 rows(a.row_count);
-  if (a.teacher_ids) {
-    if (dtype == 0)
-      hipLaunchKernelGGL((distill_loss_kernel<0>), rows, block, 0, st, a);
-    else
-      hipLaunchKernelGGL((distill_loss_kernel<1>), rows, block, 0, st, a);
-  } else if (top) {
-    if (dtype == 0)
-      hipLaunchKernelGGL((logprobs_kernel<0, true>), rows, block, 0, st, a);
-    else
-      hipLaunchKernelGGL((logprobs_kernel<1, true>), rows, block, 0, st, a);
-  } else {
-    if (dtype == 0)
-      hipLaunchKernelGGL((logprobs_kernel<0, false>), rows, dim3(64), 0, st, a);
-    else
-      hipLaunchKernelGGL((logprobs_kernel<1, false>), rows, dim3(64), 0, st, a);
+#define JF_FINISH(DT)                                                                     \
+  if (dtype == DT) {                                                                      \
+    if (a.teacher_ids && a.teacher_count <= 64)                                           \
+      hipLaunchKernelGGL((distill_loss_kernel<DT, 64>), rows, dim3(64), 0, st, a);        \
+    else if (a.teacher_ids)                                                               \
+      hipLaunchKernelGGL((distill_loss_kernel<DT, 256>), rows, dim3(256), 0, st, a);      \
+    else if (top)                                                                         \
+      hipLaunchKernelGGL((logprobs_kernel<DT, true>), rows, dim3(256), 0, st, a);         \
+    else                                                                                  \
+      hipLaunchKernelGGL((logprobs_kernel<DT, false>), rows, dim3(64), 0, st, a);         \
   }
+  JF_FINISH(0)
+  JF_FINISH(1)
+#undef JF_FINISH
   return (int)hipGetLastError();
 }
 

@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 #include <new>
 #include <string>
@@ -61,8 +62,8 @@ struct jf_scorer {
   uint32_t chunks = 0;
   int device = 0;
   jf::ProcessRow *rows = nullptr;  // [max_rows]
-  float2 *partials = nullptr;      // [max_rows][chunks]
-  uint32_t *aheads = nullptr;      // [max_rows][chunks]
+  float2 *partials = nullptr;      // [max_rows][parts]: a row's blocks, most of them small
+  uint32_t *aheads = nullptr;      // [max_rows][parts]
   float *maxima = nullptr;         // [min(max_rows, kTopRows)][chunks * kScoreChunkGroups]
   float *saved = nullptr;          // [max_rows][2 + kTeacherTokens]
   uint64_t workspace_bytes = 0;
@@ -196,7 +197,7 @@ int jf_scorer_create(uint32_t vocabulary, uint32_t max_rows, jf_scorer **out) {
   int rc = JF_OK;
   const hipError_t e = hipGetDevice(&s->device);
   if (e != hipSuccess) rc = hip_fail(e, "hipGetDevice");
-  const uint64_t parts = (uint64_t)max_rows * s->chunks;
+  const uint64_t parts = (uint64_t)max_rows * s->chunks * (jf::kScoreChunk / jf::kSmallChunk);
   const uint64_t maxima = (uint64_t)std::min(max_rows, jf::kTopRows) * s->chunks *
                           jf::kScoreChunkGroups;
   const uint64_t saved = (uint64_t)max_rows * (2 + jf::kTeacherTokens);
@@ -364,11 +365,15 @@ int jf_process_logits(jf_scorer *s, const jf_process_args *a, void *stream) {
 
 // ---- the pass over a row -----------------------------------------------------
 
-// Blocks a row: one a chunk, and for many rows several chunks a block.
+// How a call's rows are split into blocks (JF_SPLIT... see below).
 static void split_rows(const jf_scorer *s, uint32_t rows, jf::ScoreLaunch *L) {
-  (void)rows;
-  L->segment_chunks = 1;
-  L->segments = s->chunks;
+  static const char *e = getenv("JF_SMALL"), *f = getenv("JF_SEG");
+  const uint32_t lim = e ? atoi(e) : 512, seg = f ? atoi(f) : 1;
+  L->small = rows * s->chunks <= lim;
+  const uint32_t chunks = L->small ? (s->vocabulary + jf::kSmallChunk - 1) / jf::kSmallChunk : s->chunks;
+  L->segment_chunks = std::min(L->small ? 1 : seg, chunks);
+  L->segments = (chunks + L->segment_chunks - 1) / L->segment_chunks;
+  L->groups = chunks * ((L->small ? jf::kSmallChunk : jf::kScoreChunk) / jf::kScoreGroup);
 }
 
 static jf::ScoreLaunch score_rows(const jf_scorer *s, const void *logits, uint64_t stride,
@@ -378,7 +383,6 @@ static jf::ScoreLaunch score_rows(const jf_scorer *s, const void *logits, uint64
   L.stride = stride;
   L.row_count = rows;
   L.vocabulary = s->vocabulary;
-  L.groups = s->chunks * jf::kScoreChunkGroups;
   split_rows(s, rows, &L);
   L.temperature = 1.0f;
   // Launches of one call follow one another on its stream: each takes the

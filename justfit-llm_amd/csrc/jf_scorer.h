@@ -13,6 +13,7 @@ namespace jf {
 // A block's tokens at a time, and the tokens whose maximum the score pass
 // keeps (a power of two that divides a chunk).
 constexpr uint32_t kScoreChunk = 8192;
+constexpr uint32_t kSmallChunk = 2048;  // for calls of few rows
 constexpr uint32_t kScoreGroup = 64;
 constexpr uint32_t kScoreChunkGroups = kScoreChunk / kScoreGroup;
 constexpr uint32_t kTopLogprobs = 128;    // alternatives a row at most
@@ -62,6 +63,7 @@ struct ScoreLaunch {
   const void *logits;
   uint64_t stride;
   uint32_t row_count, vocabulary;
+  uint32_t small;           // chunks of kSmallChunk tokens, otherwise kScoreChunk
   uint32_t segments;        // blocks a row
   uint32_t segment_chunks;  // chunks a block
   uint32_t groups;          // groups a row, padded to whole chunks
