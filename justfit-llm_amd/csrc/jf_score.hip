@@ -99,30 +99,40 @@ __device__ __forceinline__ const T *element(const T *row, uint32_t i) {
   return (const T *)((const char *)row + (uint32_t)(i * sizeof(T)));
 }
 
-constexpr uint32_t kMostItems = 32;  // groups, and then tokens, a thread holds at most
-constexpr uint32_t kListItems = 512;
+constexpr uint32_t kMostItems = 32;  // groups a thread holds at most
+constexpr uint32_t kWaveGroups = 128;  // groups a wave lists at most
+// Tokens a wave lists at most. A row whose best tokens are neighbours lists most
+// of their groups' tokens: ids in the order of their frequency come to hundreds.
+constexpr uint32_t kWaveItems = 512;
 // Lists of up to this many alternatives are cut by the best groups of 64 quads
 // of lanes, longer ones by those of the 256 threads: a cut by fewer units is
 // quicker to find and lists more groups.
 constexpr uint32_t kQuadTop = 32;
-constexpr uint32_t kIdBits = 20;  // tokens and groups are below 2^20
 
 struct TopLds {
-  uint32_t unit_key[256], unit_id[256];
-  uint2 item[kListItems];  // key, id
+  uint64_t item[4][kWaveItems + 8];  // each wave's tokens, then 0 up to a multiple of 8
+  uint32_t unit[256];                // the units' best keys
+  uint16_t group[4][kWaveGroups];
   uint32_t best[kTopLogprobs];
   uint64_t wave[2][4];
-  uint32_t count[2];
+  uint32_t count[4];
+  uint32_t crowded;
 };
 
-// The k-th largest (from 1) of the wave's 64 * U values below 2^BITS, two bits
-// a step: the largest t that k values reach.
+// An item as one number, larger ones ahead: its key, then the lower id.
+__device__ __forceinline__ uint64_t item_of(uint32_t key, uint32_t id) {
+  return (uint64_t)key << 32 | (0xffffffffu - id);
+}
+__device__ __forceinline__ uint32_t item_id(uint64_t item) { return 0xffffffffu - (uint32_t)item; }
+
+// The k-th largest (from 1) of the wave's 64 * U values, down to its top BITS
+// bits, two bits a step: the largest such t that k values reach.
 template <uint32_t U, int BITS>
 __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[U], uint32_t k) {
   static_assert(BITS % 2 == 0);
   uint32_t t = 0;
 #pragma unroll 2
-  for (int b = BITS - 2; b >= 0; b -= 2) {
+  for (int b = 30; b > 30 - BITS; b -= 2) {
     uint32_t reach[3] = {};
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
@@ -135,21 +145,19 @@ __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[U], uint32_t
   return t;
 }
 
-// The block's `k` best items one by one, in the order (key down, id up), to
-// put(place, key, id) of every thread; key 0 is no item. each(take) gives a
-// thread's items to take(key, id). Returns how many there are. Any order of
-// items takes k rounds: for those that crowd the list.
+// The block's `k` best items one by one to put(place, item) of every thread; 0
+// is no item. each(take) gives a thread's items to take(item). Returns how many
+// there are. Any order of items takes k rounds: for those that crowd the lists.
 template <class Each, class Put>
 __device__ __forceinline__ uint32_t pick_best(TopLds &s, uint32_t k, const Each &each,
                                               const Put &put) {
   uint64_t last = ~0ull;
+  const auto larger = [](uint64_t p, uint64_t q) { return p > q ? p : q; };
   for (uint32_t place = 0; place < k; ++place) {
     uint64_t best = 0;
-    each([&](uint32_t key, uint32_t id) {
-      const uint64_t item = (uint64_t)key << 32 | (0xffffffffu - id);
-      if (key && item < last && item > best) best = item;
+    each([&](uint64_t item) {
+      if (item < last && item > best) best = item;
     });
-    const auto larger = [](uint64_t p, uint64_t q) { return p > q ? p : q; };
     best = larger(best, xor_u64<1>(best));
     best = larger(best, xor_u64<2>(best));
     best = larger(best, xor_u64<4>(best));
@@ -161,194 +169,157 @@ __device__ __forceinline__ uint32_t pick_best(TopLds &s, uint32_t k, const Each 
     __syncthreads();
     last = larger(larger(slot[0], slot[1]), larger(slot[2], slot[3]));
     if (last == 0) return place;
-    put(place, (uint32_t)(last >> 32), 0xffffffffu - (uint32_t)last);
+    put(place, last);
   }
   return k;
 }
 
-// The place of an item among the n listed ones.
-__device__ __forceinline__ uint32_t place_of(const TopLds &s, uint32_t n, uint2 item) {
-  uint32_t place = 0;
-#pragma unroll 8
-  for (uint32_t j = 0; j < n; ++j) {
-    const uint2 other = s.item[j];
-    place += other.x > item.x || (other.x == item.x && other.y < item.y) ? 1u : 0u;
-  }
-  return place;
+// One alternative of a row at its place.
+__device__ __forceinline__ void put_best(const ScoreLaunch &a, uint32_t row, uint32_t place,
+                                         uint64_t item, const RowScore &score) {
+  const uint64_t at = (uint64_t)row * a.top + place;
+  a.out_top_ids[at] = item_id(item);
+  a.out_top_logprobs[at] = score.logprob(key_logit((uint32_t)(item >> 32)));
 }
 
-// The row's best groups by (maximum down, group up) into s.best: the k best
-// and, up to kTopLogprobs in all, perhaps more. Returns their number; `cut` is
-// a key that the k best groups' maxima reach (1 where there are fewer).
-//
-// A unit is four lanes (U = 1: 64 units) or one thread (U = 4: 256 of them).
-// The k-th of the units' best groups is not ahead of the row's k-th best one,
-// so the groups at or ahead of it hold the k best, with few others where the
-// best groups lie in different units.
-template <uint32_t N, uint32_t U>
-__device__ __forceinline__ uint32_t best_groups(TopLds &s, const float *maxima, uint32_t groups,
-                                                uint32_t k, uint32_t *cut_out) {
+// The alternatives of a row whose best groups or tokens crowd the lists: its k
+// best groups in rounds, then their k best tokens. Returns how many there are.
+template <int DT>
+__device__ __forceinline__ uint32_t crowded_best(TopLds &s, const ScoreLaunch &a, uint32_t row,
+                                                 const typename Logits<DT>::Element *x,
+                                                 const float *maxima, const RowScore &score) {
+  const uint32_t tid = threadIdx.x;
+  const uint32_t n = pick_best(
+      s, a.top,
+      [&](const auto &take) {
+#pragma unroll 4
+        for (uint32_t id = tid; id < a.groups; id += 256) {
+          const uint32_t key = listed_key(*element(maxima, id));
+          take(key ? item_of(key, id) : 0ull);
+        }
+      },
+      [&](uint32_t place, uint64_t item) {
+        if (tid == 0) s.best[place] = item_id(item);
+      });
+  __syncthreads();
+  return pick_best(
+      s, a.top,
+      [&](const auto &take) {
+#pragma unroll 4
+        for (uint32_t slot = tid >> 6; slot < n; slot += 4) {
+          const uint32_t id = s.best[slot] * kScoreGroup + (tid & 63u);
+          const uint32_t key =
+              id < a.vocabulary ? listed_key(logit_value(*element(x, id))) : 0u;
+          take(key ? item_of(key, id) : 0ull);
+        }
+      },
+      [&](uint32_t place, uint64_t item) {
+        if (tid == 0) put_best(a, row, place, item, score);
+      });
+}
+
+// A row's alternatives. A unit is four lanes (U = 1: 64 units) or one thread
+// (U = 4: 256 of them). At least k groups reach the k-th of the units' best
+// maxima, and so the row's k best tokens do: each wave finds that cut for
+// itself, lists its own groups that reach it, reads their tokens, a group a
+// load, and lists those that reach it. Few others do where the best groups lie
+// in different units. The cut's last bits are left out (each is half a step of
+// the search): of an f32 key the last 10, a bf16 key has 16.
+template <int DT, uint32_t N, uint32_t U>
+__device__ __forceinline__ void row_best(TopLds &s, const ScoreLaunch &a, uint32_t row,
+                                         const typename Logits<DT>::Element *x,
+                                         const float *maxima, const float (&m)[N],
+                                         const RowScore &score) {
   static_assert(N <= kMostItems && (U == 1 || U == 4));
-  const uint32_t tid = threadIdx.x, lane = tid & 63u;
-  float m[N];
-#pragma unroll
-  for (uint32_t i = 0; i < N; ++i) m[i] = *element(maxima, min(i * 256 + tid, groups - 1));
-  uint32_t key[N], best = 0, best_id = 0;
-  const auto id_of = [&](uint32_t i) { return i * 256 + tid; };
-  const auto take = [&](uint32_t other, uint32_t other_id) {
-    if (other > best || (other == best && other_id < best_id)) {
-      best = other;
-      best_id = other_id;
-    }
-  };
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, k = a.top;
+  uint32_t key[N], best = 0;
 #pragma unroll
   for (uint32_t i = 0; i < N; ++i) {
-    key[i] = id_of(i) < groups ? listed_key(m[i]) : 0u;
-    take(key[i], id_of(i));
+    key[i] = i * 256 + tid < a.groups ? listed_key(m[i]) : 0u;
+    best = max(best, key[i]);
   }
-  const uint32_t own = best;
   if constexpr (U == 1) {
-    take(xor_u32<1>(best), xor_u32<1>(best_id));
-    take(xor_u32<2>(best), xor_u32<2>(best_id));
-    if (tid % 4 == 0) {
-      s.unit_key[tid / 4] = best;
-      s.unit_id[tid / 4] = best_id;
-    }
+    best = max(best, xor_u32<1>(best));
+    best = max(best, xor_u32<2>(best));
+    if (tid % 4 == 0) s.unit[tid / 4] = best;
   } else {
-    s.unit_key[tid] = best;
-    s.unit_id[tid] = best_id;
+    s.unit[tid] = best;
   }
+  if (tid == 0) s.crowded = 0;
   __syncthreads();
-  // Every wave finds the cut by itself.
-  uint32_t unit[U], unit_id[U], present = 0;
+  uint32_t unit[U], present = 0;
 #pragma unroll
   for (uint32_t u = 0; u < U; ++u) {
-    unit[u] = s.unit_key[lane * U + u];
-    unit_id[u] = s.unit_id[lane * U + u];
+    unit[u] = s.unit[lane * U + u];
     present += (uint32_t)__popcll(ballot(unit[u] != 0));
   }
-  uint32_t cut = 1, cut_id = 0xffffffffu;  // everything
-  if (present >= k) {
-    cut = kth_largest<U, 32>(unit, k);
-    uint32_t ahead = 0, ties = 0, tie_id[U], last = 0;
+  // With fewer than k units that have a group, every group is listed.
+  uint32_t cut = 1;
+  if (present >= k) cut = max(kth_largest<U, DT == 0 ? 22 : 16>(unit, k), 1u);
+  uint32_t n = 0, tokens = 0;
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) {
-      ahead += (uint32_t)__popcll(ballot(unit[u] > cut));
-      ties += (uint32_t)__popcll(ballot(unit[u] == cut));
-      // Ids from the top down, so that the lowest is the largest.
-      tie_id[u] = unit[u] == cut ? (1u << kIdBits) - 1u - unit_id[u] : 0u;
-      last = max(last, unit[u] == cut ? unit_id[u] : 0u);
-    }
-    if (ahead + ties == k)
-      cut_id = wave_max_u32(last);
-    else
-      cut_id = (1u << kIdBits) - 1u - kth_largest<U, kIdBits>(tie_id, k - ahead);
+  for (uint32_t i = 0; i < N; ++i) {
+    const bool take = key[i] >= cut;
+    const uint64_t lanes = ballot(take);
+    const uint32_t at = n + mbcnt(lanes);
+    if (take && at < kWaveGroups) s.group[wave][at] = (uint16_t)(i * 256 + tid);
+    n += (uint32_t)__popcll(lanes);
   }
-  *cut_out = cut;
-  if (own >= cut) {
-#pragma unroll
-    for (uint32_t i = 0; i < N; ++i)
-      if (key[i] > cut || (key[i] == cut && id_of(i) <= cut_id)) {
-        const uint32_t at = atomicAdd(&s.count[0], 1u);
-        if (at < kListItems) s.item[at] = make_uint2(key[i], id_of(i));
-      }
-  }
-  __syncthreads();
-  const uint32_t n = s.count[0];
-  if (n <= kTopLogprobs) {
-    if (tid < n) s.best[tid] = s.item[tid].y;
-  } else if (n <= kListItems) {
-    for (uint32_t i = tid; i < n; i += 256) {
-      const uint32_t place = place_of(s, n, s.item[i]);
-      if (place < k) s.best[place] = s.item[i].y;
-    }
-  } else {
-    pick_best(
-        s, k,
-        [&](const auto &take_item) {
-          // Read again: held over the rounds they cost 150 registers.
-#pragma unroll 4
-          for (uint32_t id = tid; id < groups; id += 256)
-            take_item(listed_key(*element(maxima, id)), id);
-        },
-        [&](uint32_t place, uint32_t, uint32_t group) {
-          if (tid == 0) s.best[place] = group;
-        });
-  }
-  __syncthreads();
-  return n <= kTopLogprobs ? n : k;
-}
-
-// The row's k best tokens from its n best groups: a wave reads a group a load,
-// eight in flight. The k best reach the groups' cut.
-template <int DT>
-__device__ __forceinline__ void best_tokens(TopLds &s, const ScoreLaunch &a, uint32_t row,
-                                            const typename Logits<DT>::Element *x, uint32_t n,
-                                            uint32_t cut, const RowScore &score) {
-  const uint32_t tid = threadIdx.x, k = a.top;
-  uint32_t *ids = a.out_top_ids + (uint64_t)row * k;
-  float *logprobs = a.out_top_logprobs + (uint64_t)row * k;
-  constexpr uint32_t AHEAD = 8;
-  const auto each_token = [&](const auto &take) {
-    for (uint32_t first = 0; first < n; first += AHEAD * 4) {
+  __builtin_amdgcn_wave_barrier();  // the wave's own list, in order
+  bool fits = n <= kWaveGroups;
+  if (fits) {
+    constexpr uint32_t AHEAD = 8;
+    for (uint32_t first = 0; first < n; first += AHEAD) {
       uint32_t id[AHEAD];
       float v[AHEAD];
 #pragma unroll
       for (uint32_t i = 0; i < AHEAD; ++i) {
-        const uint32_t slot = first + i * 4 + (tid >> 6);
-        id[i] = s.best[min(slot, n - 1)] * kScoreGroup + (tid & 63u);
-        if (slot >= n) id[i] = a.vocabulary;
+        id[i] = s.group[wave][min(first + i, n - 1)] * kScoreGroup + lane;
         v[i] = logit_value(*element(x, min(id[i], a.vocabulary - 1)));
       }
 #pragma unroll
-      for (uint32_t i = 0; i < AHEAD; ++i)
-        take(id[i] < a.vocabulary ? listed_key(v[i]) : 0u, id[i]);
-    }
-  };
-  each_token([&](uint32_t key, uint32_t id) {
-    if (key >= cut) {
-      const uint32_t at = atomicAdd(&s.count[1], 1u);
-      if (at < kListItems) s.item[at] = make_uint2(key, id);
-    }
-  });
-  __syncthreads();
-  uint32_t m = s.count[1];
-  if (m <= kListItems) {
-    for (uint32_t i = tid; i < m; i += 256) {
-      const uint2 item = s.item[i];
-      const uint32_t place = place_of(s, m, item);
-      if (place < k) {
-        ids[place] = item.y;
-        logprobs[place] = score.logprob(key_logit(item.x));
+      for (uint32_t i = 0; i < AHEAD; ++i) {
+        const uint32_t item = listed_key(v[i]);
+        const bool take = first + i < n && id[i] < a.vocabulary && item >= cut;
+        const uint64_t lanes = ballot(take);
+        const uint32_t at = tokens + mbcnt(lanes);
+        if (take && at < kWaveItems) s.item[wave][at] = item_of(item, id[i]);
+        tokens += (uint32_t)__popcll(lanes);
       }
+    }
+    fits = tokens <= kWaveItems;
+  }
+  if (fits && lane < 8) s.item[wave][tokens + lane] = 0;
+  if (lane == 0) {
+    s.count[wave] = tokens;
+    if (!fits) s.crowded = 1;
+  }
+  __syncthreads();
+  uint32_t listed = 0;
+  if (!s.crowded) {
+    // Every item's place is the number of items ahead of it.
+    const uint32_t count[4] = {s.count[0], s.count[1], s.count[2], s.count[3]};
+    listed = count[0] + count[1] + count[2] + count[3];
+    const uint32_t most = max(max(count[0], count[1]), max(count[2], count[3]));
+    for (uint32_t own = tid / 4; own < most; own += 64) {
+      const uint64_t item = own < count[tid % 4] ? s.item[tid % 4][own] : 0ull;
+      uint32_t place = 0;
+#pragma unroll
+      for (uint32_t w = 0; w < 4; ++w) {
+        for (uint32_t j = 0; j < count[w]; j += 8) {
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e) place += s.item[w][j + e] > item ? 1u : 0u;
+        }
+      }
+      if (item && place < k) put_best(a, row, place, item, score);
     }
   } else {
-    m = pick_best(s, k, each_token, [&](uint32_t place, uint32_t key, uint32_t id) {
-      if (tid == 0) {
-        ids[place] = id;
-        logprobs[place] = score.logprob(key_logit(key));
-      }
-    });
+    listed = crowded_best<DT>(s, a, row, x, maxima, score);
   }
-  for (uint32_t i = m + tid; i < k; i += 256) {
-    ids[i] = kNoToken;
-    logprobs[i] = -__builtin_inff();
+  for (uint32_t i = listed + tid; i < k; i += 256) {
+    a.out_top_ids[(uint64_t)row * k + i] = kNoToken;
+    a.out_top_logprobs[(uint64_t)row * k + i] = -__builtin_inff();
   }
-}
-
-template <int DT, uint32_t U>
-__device__ __forceinline__ void row_best(TopLds &s, const ScoreLaunch &a, uint32_t row,
-                                         const typename Logits<DT>::Element *x,
-                                         const RowScore &score) {
-  const float *maxima = a.maxima + (uint64_t)row * a.groups;
-  uint32_t n, cut;
-  if (a.groups <= 10 * 256)
-    n = best_groups<10, U>(s, maxima, a.groups, a.top, &cut);
-  else if (a.groups <= 16 * 256)
-    n = best_groups<16, U>(s, maxima, a.groups, a.top, &cut);
-  else
-    n = best_groups<kMostItems, U>(s, maxima, a.groups, a.top, &cut);
-  best_tokens<DT>(s, a, row, x, n, cut, score);
 }
 
 // ---- finish -------------------------------------------------------------------
@@ -363,38 +334,56 @@ __device__ __forceinline__ MaxSum row_total(const ScoreLaunch &a, uint32_t row, 
   return wave_join(p, c);
 }
 
-// One row a block: 256 threads with alternatives, otherwise a wave.
-template <int DT, bool TOP>
-__global__ __launch_bounds__(TOP ? 256 : 64) void logprobs_kernel(ScoreLaunch a) {
-  const uint32_t tid = threadIdx.x, row = blockIdx.x;
+// A row's totals and its tokens' log-probabilities by one wave.
+template <int DT>
+__device__ __forceinline__ void put_tokens(const ScoreLaunch &a, uint32_t row,
+                                           const typename Logits<DT>::Element *x,
+                                           const RowScore &score) {
+  const uint32_t lane = threadIdx.x;
+  if (lane == 0 && a.out_lse) a.out_lse[row] = score.lse();
+  uint32_t ahead = 0;
+  if (a.out_ranks) {
+    for (uint32_t g = lane; g < a.segments; g += 64)
+      ahead += a.aheads[(uint64_t)row * a.segments + g];
+    ahead = wave_sum_u32(ahead);
+  }
+  for (uint32_t i = lane; i < a.token_count; i += 64) {
+    const uint32_t token = a.tokens[(uint64_t)row * a.token_stride + i];
+    const bool known = token < a.vocabulary;
+    a.out_logprobs[(uint64_t)row * a.token_count + i] =
+        known ? score.logprob(logit_value(x[token])) : -__builtin_inff();
+    if (i == 0 && a.out_ranks) a.out_ranks[row] = known ? ahead + 1u : 0u;
+  }
+}
+
+// One row a wave.
+template <int DT>
+__global__ __launch_bounds__(64) void logprobs_kernel(ScoreLaunch a) {
+  const uint32_t row = blockIdx.x;
   const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
   const float inv_t = inverse_temperature(a, row);
   const MaxSum total = row_total(a, row, inv_t * kLog2e);
+  put_tokens<DT>(a, row, x, RowScore{total.m, inv_t, logf(total.s)});
+}
+
+// One row a block, with alternatives: up to N groups a thread.
+template <int DT, uint32_t N>
+__global__ __launch_bounds__(256) void alternatives_kernel(ScoreLaunch a) {
+  __shared__ TopLds s;
+  const uint32_t tid = threadIdx.x, row = blockIdx.x;
+  const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
+  const float *maxima = a.maxima + (uint64_t)row * a.groups;
+  float m[N];
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i) m[i] = *element(maxima, min(i * 256 + tid, a.groups - 1));
+  const float inv_t = inverse_temperature(a, row);
+  const MaxSum total = row_total(a, row, inv_t * kLog2e);
   const RowScore score{total.m, inv_t, logf(total.s)};
-  if (tid < 64) {
-    if (tid == 0 && a.out_lse) a.out_lse[row] = score.lse();
-    uint32_t ahead = 0;
-    if (a.out_ranks) {
-      for (uint32_t g = tid; g < a.segments; g += 64)
-        ahead += a.aheads[(uint64_t)row * a.segments + g];
-      ahead = wave_sum_u32(ahead);
-    }
-    for (uint32_t i = tid; i < a.token_count; i += 64) {
-      const uint32_t token = a.tokens[(uint64_t)row * a.token_stride + i];
-      const bool known = token < a.vocabulary;
-      a.out_logprobs[(uint64_t)row * a.token_count + i] =
-          known ? score.logprob(logit_value(x[token])) : -__builtin_inff();
-      if (i == 0 && a.out_ranks) a.out_ranks[row] = known ? ahead + 1u : 0u;
-    }
-  }
-  if constexpr (TOP) {
-    __shared__ TopLds s;
-    if (tid < 2) s.count[tid] = 0;  // ordered by the units' barrier
-    if (a.top <= kQuadTop)
-      row_best<DT, 1>(s, a, row, x, score);
-    else
-      row_best<DT, 4>(s, a, row, x, score);
-  }
+  if (a.top <= kQuadTop)
+    row_best<DT, N, 1>(s, a, row, x, maxima, m, score);
+  else
+    row_best<DT, N, 4>(s, a, row, x, maxima, m, score);
+  if (tid < 64) put_tokens<DT>(a, row, x, score);
 }
 
 __device__ __forceinline__ float wave_sum_f32(float v) {
@@ -609,10 +598,14 @@ int launch_score(const ScoreLaunch &a, uint32_t dtype, void *stream) {
       hipLaunchKernelGGL((distill_loss_kernel<DT, 64>), rows, dim3(64), 0, st, a);        \
     else if (a.teacher_ids)                                                               \
       hipLaunchKernelGGL((distill_loss_kernel<DT, 256>), rows, dim3(256), 0, st, a);      \
-    else if (top)                                                                         \
-      hipLaunchKernelGGL((logprobs_kernel<DT, true>), rows, dim3(256), 0, st, a);         \
+    else if (!top)                                                                        \
+      hipLaunchKernelGGL((logprobs_kernel<DT>), rows, dim3(64), 0, st, a);                \
+    else if (a.groups <= 10 * 256)                                                        \
+      hipLaunchKernelGGL((alternatives_kernel<DT, 10>), rows, dim3(256), 0, st, a);       \
+    else if (a.groups <= 16 * 256)                                                        \
+      hipLaunchKernelGGL((alternatives_kernel<DT, 16>), rows, dim3(256), 0, st, a);       \
     else                                                                                  \
-      hipLaunchKernelGGL((logprobs_kernel<DT, false>), rows, dim3(64), 0, st, a);         \
+      hipLaunchKernelGGL((alternatives_kernel<DT, kMostItems>), rows, dim3(256), 0, st, a); \
   }
   JF_FINISH(0)
   JF_FINISH(1)
