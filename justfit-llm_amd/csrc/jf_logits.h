@@ -149,4 +149,103 @@ __device__ __forceinline__ void store_words(typename Logits<DT>::Element *row, u
     }
 }
 
+// ---- softmax statistics ---------------------------------------------------------
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+__device__ __forceinline__ float wave_sum_f32(float v) {
+  v += xor_f32<1>(v);
+  v += xor_f32<2>(v);
+  v += xor_f32<4>(v);
+  v += xor_f32<8>(v);
+  v += xor_f32<16>(v);
+  v += xor_f32<32>(v);
+  return v;
+}
+
+// Maxima of values as they are loaded: fmax quiets each of its operands first,
+// an instruction a value. A signalling NaN makes these NaN, a quiet one is
+// passed over.
+__device__ __forceinline__ float loaded_max(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ float loaded_max(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ float vector_max(const LogitWords &w) {
+  float v[Logits<DT>::VEC];
+  unpack<DT>(w, v);
+  float m = loaded_max(v[0], v[1], v[2]);
+  if constexpr (DT == 0) return loaded_max(m, v[3]);
+  m = loaded_max(m, v[3], v[4]);
+  return loaded_max(loaded_max(m, v[5], v[6]), v[7]);
+}
+
+// A running maximum and sum of exponentials. Nothing yet, or nothing but
+// -infinity: m = -infinity, s = 0. A NaN, or +infinity, makes s NaN for good.
+struct MaxSum {
+  float m, s;
+};
+// exp((x - m) / T) with c = log2(e) / T; m is at least x, and not -infinity.
+__device__ __forceinline__ float exp_below(float x, float m, float c) {
+  return __builtin_amdgcn_exp2f((x - m) * c);
+}
+__device__ __forceinline__ float finite_reference(float m) {
+  return m == -__builtin_inff() ? 0.0f : m;
+}
+__device__ __forceinline__ MaxSum join(MaxSum p, MaxSum q, float c) {
+  const float m = __builtin_fmaxf(p.m, q.m), r = finite_reference(m);
+  return {m, p.s * exp_below(p.m, r, c) + q.s * exp_below(q.m, r, c)};
+}
+__device__ __forceinline__ MaxSum wave_join(MaxSum p, float c) {
+  const float m = wave_max_f32(p.m);
+  return {m, wave_sum_f32(p.s * exp_below(p.m, finite_reference(m), c))};
+}
+// Adds a thread's N vectors, whose maxima are `part`.
+template <int DT, uint32_t N>
+__device__ __forceinline__ void add_vectors(MaxSum &run, const LogitWords (&w)[N],
+                                            const float (&part)[N], float c) {
+  float grown = run.m;
+#pragma unroll
+  for (uint32_t j = 0; j < N; ++j) grown = loaded_max(grown, part[j]);
+  const float r = finite_reference(grown);
+  float s = run.s * exp_below(run.m, r, c);
+#pragma unroll
+  for (uint32_t j = 0; j < N; ++j) {
+    float v[Logits<DT>::VEC];
+    unpack<DT>(w[j], v);
+#pragma unroll
+    for (uint32_t e = 0; e < Logits<DT>::VEC; ++e) s += exp_below(v[e], r, c);
+  }
+  run = {grown, s};
+}
+
+// The row's maximum and sum from its blocks' (every lane of the wave).
+__device__ __forceinline__ MaxSum row_total(const ScoreLaunch &a, uint32_t row, float c) {
+  MaxSum p{-__builtin_inff(), 0.0f};
+  for (uint32_t g = threadIdx.x & 63u; g < a.segments; g += 64) {
+    const float2 v = a.partials[(uint64_t)row * a.segments + g];
+    p = join(p, MaxSum{v.x, v.y}, c);
+  }
+  return wave_join(p, c);
+}
+
+// A row's totals as its outputs take them.
+struct RowScore {
+  float m, inv_t, log_sum;
+  __device__ __forceinline__ float logprob(float x) const {
+    // No token: -infinity has no probability, whatever the row.
+    return x == -__builtin_inff() ? x : (x - m) * inv_t - log_sum;
+  }
+  __device__ __forceinline__ float lse() const {
+    // ln 0: the row leaves nothing (a row of NaN has one for its sum).
+    return log_sum == -__builtin_inff() ? log_sum : m * inv_t + log_sum;
+  }
+};
+
 }  // namespace jf

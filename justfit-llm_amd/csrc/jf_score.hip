@@ -22,45 +22,11 @@ namespace jf {
 
 namespace {
 
-constexpr float kLog2e = 1.44269504088896341f;
-
 // A row's temperature: the sampler's 0 (a greedy row) and anything that is no
 // temperature leave the logits as they are.
 __device__ __forceinline__ float inverse_temperature(const ScoreLaunch &a, uint32_t row) {
   const float t = a.temperatures ? a.temperatures[row] : a.temperature;
   return t >= __FLT_MIN__ && t < __builtin_inff() ? 1.0f / t : 1.0f;
-}
-
-// A running maximum and sum of exponentials. Nothing yet, or nothing but
-// -infinity: m = -infinity, s = 0. A NaN, or +infinity, makes s NaN for good.
-struct MaxSum {
-  float m, s;
-};
-// exp((x - m) / T) with c = log2(e) / T; m is at least x, and not -infinity.
-__device__ __forceinline__ float exp_below(float x, float m, float c) {
-  return __builtin_amdgcn_exp2f((x - m) * c);
-}
-__device__ __forceinline__ float finite_reference(float m) {
-  return m == -__builtin_inff() ? 0.0f : m;
-}
-__device__ __forceinline__ MaxSum join(MaxSum p, MaxSum q, float c) {
-  const float m = __builtin_fmaxf(p.m, q.m), r = finite_reference(m);
-  return {m, p.s * exp_below(p.m, r, c) + q.s * exp_below(q.m, r, c)};
-}
-template <int M>
-__device__ __forceinline__ MaxSum join_xor(MaxSum p, float c) {
-  return join(p, MaxSum{xor_f32<M>(p.m), xor_f32<M>(p.s)}, c);
-}
-__device__ __forceinline__ MaxSum wave_join(MaxSum p, float c) {
-  const float m = wave_max_f32(p.m);
-  float s = p.s * exp_below(p.m, finite_reference(m), c);
-  s += xor_f32<1>(s);
-  s += xor_f32<2>(s);
-  s += xor_f32<4>(s);
-  s += xor_f32<8>(s);
-  s += xor_f32<16>(s);
-  s += xor_f32<32>(s);
-  return {m, s};
 }
 
 // The least float above x; a NaN, which nothing reaches, above +infinity and
@@ -76,19 +42,6 @@ __device__ __forceinline__ float next_up(float x) {
 __device__ __forceinline__ uint32_t listed_key(float x) {
   return x > -__builtin_inff() ? logit_key(x) : 0u;
 }
-
-// A row's totals as its outputs take them.
-struct RowScore {
-  float m, inv_t, log_sum;
-  __device__ __forceinline__ float logprob(float x) const {
-    // No token: -infinity has no probability, whatever the row.
-    return x == -__builtin_inff() ? x : (x - m) * inv_t - log_sum;
-  }
-  __device__ __forceinline__ float lse() const {
-    // ln 0: the row leaves nothing (a row of NaN has one for its sum).
-    return log_sum == -__builtin_inff() ? log_sum : m * inv_t + log_sum;
-  }
-};
 
 // ---- the best tokens ----------------------------------------------------------
 
@@ -118,6 +71,28 @@ struct TopLds {
   uint32_t count[4];
   uint32_t crowded;
 };
+
+// The group whose maximum is the i-th of its row: a chunk's groups are stored in
+// the order (lanes, vector), the passes' own (score_kernel).
+template <int DT>
+__device__ __forceinline__ uint32_t group_at(const ScoreLaunch &a, uint32_t i) {
+  constexpr uint32_t SLAB_GROUPS = kSlab<DT> / kScoreGroup;
+  const uint32_t vectors = (a.small ? kSmallChunk : kScoreChunk) / kSlab<DT>;
+  const uint32_t groups = vectors * SLAB_GROUPS, within = i % groups;
+  return i - within + within % vectors * SLAB_GROUPS + within / vectors;
+}
+// The maximum of a group of which the pass met a signalling NaN.
+template <int DT>
+__device__ __forceinline__ float group_max(const ScoreLaunch &a,
+                                           const typename Logits<DT>::Element *x, uint32_t group) {
+  float m = -__builtin_inff();
+  for (uint32_t e = 0; e < kScoreGroup; ++e) {
+    const uint32_t id = group * kScoreGroup + e;
+    const float v = id < a.vocabulary ? logit_value(x[id]) : m;
+    if (v > m) m = v;
+  }
+  return m;
+}
 
 // An item as one number, larger ones ahead: its key, then the lower id.
 __device__ __forceinline__ uint64_t item_of(uint32_t key, uint32_t id) {
@@ -193,8 +168,11 @@ __device__ __forceinline__ uint32_t crowded_best(TopLds &s, const ScoreLaunch &a
       s, a.top,
       [&](const auto &take) {
 #pragma unroll 4
-        for (uint32_t id = tid; id < a.groups; id += 256) {
-          const uint32_t key = listed_key(*element(maxima, id));
+        for (uint32_t i = tid; i < a.groups; i += 256) {
+          const uint32_t id = group_at<DT>(a, i);
+          float m = *element(maxima, i);
+          if (m != m) m = group_max<DT>(a, x, id);
+          const uint32_t key = listed_key(m);
           take(key ? item_of(key, id) : 0ull);
         }
       },
@@ -235,7 +213,9 @@ __device__ __forceinline__ void row_best(TopLds &s, const ScoreLaunch &a, uint32
   uint32_t key[N], best = 0;
 #pragma unroll
   for (uint32_t i = 0; i < N; ++i) {
-    key[i] = i * 256 + tid < a.groups ? listed_key(m[i]) : 0u;
+    float v = m[i];
+    if (v != v) v = group_max<DT>(a, x, group_at<DT>(a, min(i * 256 + tid, a.groups - 1)));
+    key[i] = i * 256 + tid < a.groups ? listed_key(v) : 0u;
     best = max(best, key[i]);
   }
   if constexpr (U == 1) {
@@ -262,7 +242,7 @@ __device__ __forceinline__ void row_best(TopLds &s, const ScoreLaunch &a, uint32
     const bool take = key[i] >= cut;
     const uint64_t lanes = ballot(take);
     const uint32_t at = n + mbcnt(lanes);
-    if (take && at < kWaveGroups) s.group[wave][at] = (uint16_t)(i * 256 + tid);
+    if (take && at < kWaveGroups) s.group[wave][at] = (uint16_t)group_at<DT>(a, i * 256 + tid);
     n += (uint32_t)__popcll(lanes);
   }
   __builtin_amdgcn_wave_barrier();  // the wave's own list, in order
@@ -324,16 +304,6 @@ __device__ __forceinline__ void row_best(TopLds &s, const ScoreLaunch &a, uint32
 
 // ---- finish -------------------------------------------------------------------
 
-// The row's maximum and sum from its blocks' (every lane of the wave).
-__device__ __forceinline__ MaxSum row_total(const ScoreLaunch &a, uint32_t row, float c) {
-  MaxSum p{-__builtin_inff(), 0.0f};
-  for (uint32_t g = threadIdx.x & 63u; g < a.segments; g += 64) {
-    const float2 v = a.partials[(uint64_t)row * a.segments + g];
-    p = join(p, MaxSum{v.x, v.y}, c);
-  }
-  return wave_join(p, c);
-}
-
 // A row's totals and its tokens' log-probabilities by one wave.
 template <int DT>
 __device__ __forceinline__ void put_tokens(const ScoreLaunch &a, uint32_t row,
@@ -386,89 +356,32 @@ __global__ __launch_bounds__(256) void alternatives_kernel(ScoreLaunch a) {
   if (tid < 64) put_tokens<DT>(a, row, x, score);
 }
 
-__device__ __forceinline__ float wave_sum_f32(float v) {
-  v += xor_f32<1>(v);
-  v += xor_f32<2>(v);
-  v += xor_f32<4>(v);
-  v += xor_f32<8>(v);
-  v += xor_f32<16>(v);
-  v += xor_f32<32>(v);
-  return v;
-}
-// Over a block of THREADS (a wave, or four); `lds` is written before one
-// barrier and read after it.
-template <uint32_t THREADS>
-__device__ __forceinline__ float block_max(float v, float (&lds)[4]) {
-  v = wave_max_f32(v);
-  if constexpr (THREADS == 64) return v;
-  if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return __builtin_fmaxf(__builtin_fmaxf(lds[0], lds[1]), __builtin_fmaxf(lds[2], lds[3]));
-}
-template <uint32_t THREADS>
-__device__ __forceinline__ float block_sum(float v, float (&lds)[4]) {
-  v = wave_sum_f32(v);
-  if constexpr (THREADS == 64) return v;
-  if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
-}
-
-// The distillation's loss of a row a block, one listed token a thread:
-// sum p_k (ln p_k - ln q_k), and what the backward pass takes: the row's
-// maximum, the list's mass over the row's sum, and each slot's probability
-// (-1: no token, or one that an earlier slot lists). Lists of up to 64 take a
-// wave, without a barrier.
-template <int DT, uint32_t THREADS>
-__global__ __launch_bounds__(THREADS) void distill_loss_kernel(ScoreLaunch a) {
-  __shared__ float lds[4][4];
-  __shared__ uint32_t listed[THREADS];
-  const uint32_t tid = threadIdx.x, row = blockIdx.x, K = a.teacher_count;
-  const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
-  uint32_t id = kNoToken;
-  float value = -__builtin_inff(), logit = 0.0f;
-  if (tid < K) {
-    id = a.teacher_ids[(uint64_t)row * a.teacher_stride + tid];
-    value = a.teacher_values[(uint64_t)row * a.teacher_stride + tid];
-  }
-  bool valid = id < a.vocabulary;
-  if (valid) logit = logit_value(x[id]);
-  listed[tid] = id;
-  const float inv_t = 1.0f / a.temperature;
-  const MaxSum total = row_total(a, row, inv_t * kLog2e);
-  const RowScore score{total.m, inv_t, logf(total.s)};
-  __syncthreads();
-#pragma unroll 8
-  for (uint32_t k = 0; k < K; ++k) valid = valid && !(k < tid && listed[k] == id);
-  float log_p = valid ? value : -__builtin_inff();
-  if (a.normalize) {
-    log_p *= inv_t;
-    log_p -= finite_reference(block_max<THREADS>(log_p, lds[0]));
-    const float log_sum = logf(block_sum<THREADS>(expf(log_p), lds[1]));
-    // -infinity stays: a list of nothing else has no mass.
-    if (log_p != -__builtin_inff()) log_p -= log_sum;
-  }
-  const float p = valid ? expf(log_p) : 0.0f;
-  // A token of no teacher probability adds nothing, whatever the student's.
-  const float loss =
-      block_sum<THREADS>(p == 0.0f ? 0.0f : p * (log_p - score.logprob(logit)), lds[2]);
-  const float mass = block_sum<THREADS>(p, lds[3]);
-  if (tid == 0) {
-    a.out_loss[row] = loss;
-    if (a.out_lse) a.out_lse[row] = score.lse();
-  }
-  if (a.saved) {
-    float *saved = a.saved + (uint64_t)row * (2 + K);
-    if (tid == 0) {
-      saved[0] = total.m;
-      // No list, or no student probability anywhere: no exponentials to add.
-      saved[1] = mass == 0.0f || total.s == 0.0f ? 0.0f : mass / total.s;
-    }
-    if (tid < K) saved[2 + tid] = valid ? p : -1.0f;
-  }
-}
-
 // ---- the pass -----------------------------------------------------------------
+
+// Each value's maximum with a neighbour's (as loaded_max takes it). A lane reads
+// its neighbour two instructions after the value was written at the earliest:
+// hence the wait in front.
+#define JF_MAX_DPP(V, CTRL) "v_max_f32_dpp " V ", " V ", " V " " CTRL " row_mask:0xf bank_mask:0xf\n"
+#define JF_MAX_STEP(NAME, CTRL)                                                                 \
+  template <uint32_t N>                                                                         \
+  __device__ __forceinline__ void NAME(float (&g)[N]) {                                         \
+    static_assert(N == 1 || N == 2 || N == 4 || N == 8);                                        \
+    if constexpr (N == 1)                                                                       \
+      asm("s_nop 1\n" JF_MAX_DPP("%0", CTRL) : "+v"(g[0]));                                     \
+    else if constexpr (N == 2)                                                                  \
+      asm("s_nop 1\n" JF_MAX_DPP("%0", CTRL) JF_MAX_DPP("%1", CTRL) : "+v"(g[0]), "+v"(g[1]));  \
+    else                                                                                        \
+      for (uint32_t j = 0; j < N; j += 4)                                                       \
+        asm("s_nop 1\n" JF_MAX_DPP("%0", CTRL) JF_MAX_DPP("%1", CTRL) JF_MAX_DPP("%2", CTRL)    \
+                JF_MAX_DPP("%3", CTRL)                                                          \
+            : "+v"(g[j]), "+v"(g[j + 1]), "+v"(g[j + 2]), "+v"(g[j + 3]));                      \
+  }
+JF_MAX_STEP(max_pairs, "quad_perm:[1,0,3,2]")
+JF_MAX_STEP(max_quads, "quad_perm:[2,3,0,1]")
+JF_MAX_STEP(max_eights, "row_half_mirror")  // of quads that agree
+JF_MAX_STEP(max_sixteens, "row_mirror")     // of eights that agree
+#undef JF_MAX_STEP
+#undef JF_MAX_DPP
 
 // A block's segment of a row: chunks of N slabs.
 template <int DT, uint32_t N, bool RANK, bool TOP>
@@ -498,27 +411,10 @@ __global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
     const uint32_t base = chunk * CHUNK;
     LogitWords w[N];
     load_chunk<DT>(x, base, V, kPastMinusInfinity<DT>, w);
-    float part[N], m = -__builtin_inff();
+    float part[N];
 #pragma unroll
-    for (uint32_t j = 0; j < N; ++j) {
-      float v[VEC];
-      unpack<DT>(w[j], v);
-      part[j] = v[0];
-#pragma unroll
-      for (uint32_t e = 1; e < VEC; ++e) part[j] = __builtin_fmaxf(part[j], v[e]);
-      m = __builtin_fmaxf(m, part[j]);
-    }
-    // A NaN maximum: every value of the thread is NaN.
-    const float grown = __builtin_fmaxf(run.m, m), r = finite_reference(grown);
-    float s = run.s * exp_below(run.m, r, c);
-#pragma unroll
-    for (uint32_t j = 0; j < N; ++j) {
-      float v[VEC];
-      unpack<DT>(w[j], v);
-#pragma unroll
-      for (uint32_t e = 0; e < VEC; ++e) s += exp_below(v[e], r, c);
-    }
-    run = {grown, s};
+    for (uint32_t j = 0; j < N; ++j) part[j] = vector_max<DT>(w[j]);
+    add_vectors<DT>(run, w, part, c);
     if constexpr (RANK) {
       if (target < V) {
         // Ids before the target's are ahead of it at equal logits too.
@@ -538,18 +434,19 @@ __global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
       }
     }
     if constexpr (TOP) {
-      // A group's 64 tokens lie in 16 (f32) or 8 (bf16) neighbouring lanes.
-      float *maxima = a.maxima + (uint64_t)row * a.groups + base / kScoreGroup;
+      // A group's 64 tokens lie in 16 (f32) or 8 (bf16) neighbouring lanes, of
+      // which the j-th writes the group of vector j: a wave's store is a run.
+      constexpr uint32_t LANES = kScoreGroup / VEC;
+      max_pairs(part);
+      max_quads(part);
+      max_eights(part);
+      if constexpr (DT == 0) max_sixteens(part);
+      float own = part[0];
 #pragma unroll
-      for (uint32_t j = 0; j < N; ++j) {
-        float g = part[j];
-        g = __builtin_fmaxf(g, xor_f32<1>(g));
-        g = __builtin_fmaxf(g, xor_f32<2>(g));
-        g = __builtin_fmaxf(g, xor_f32<4>(g));
-        if constexpr (DT == 0) g = __builtin_fmaxf(g, xor_f32<8>(g));
-        if (tid % (kScoreGroup / VEC) == 0)
-          maxima[(j * SLAB + tid * VEC) / kScoreGroup] = g;
-      }
+      for (uint32_t j = 1; j < N; ++j) own = tid % LANES == j ? part[j] : own;
+      if (tid % LANES < N)
+        a.maxima[(uint64_t)row * a.groups + base / kScoreGroup + tid / LANES * N + tid % LANES] =
+            own;
     }
   }
   run = wave_join(run, c);
@@ -572,13 +469,12 @@ __global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
 }  // namespace
 
 int launch_score(const ScoreLaunch &a, uint32_t dtype, void *stream) {
-  const hipStream_t st = (hipStream_t)stream;
-  const dim3 grid(a.row_count * a.segments), rows(a.row_count);
+  const dim3 grid(a.row_count * a.segments);
   const bool top = a.top != 0, rank = a.out_ranks != nullptr;
 #define JF_SCORE(DT, N, RANK, TOP)                                                       \
   if (dtype == DT && (a.small != 0) == (N * kSlab<DT> == kSmallChunk) && rank == RANK && \
       top == TOP)                                                                        \
-  hipLaunchKernelGGL((score_kernel<DT, N, RANK, TOP>), grid, dim3(256), 0, st, a)
+  hipLaunchKernelGGL((score_kernel<DT, N, RANK, TOP>), grid, dim3(256), 0, (hipStream_t)stream, a)
 #define JF_SCORE_ALL(DT, N)      \
   JF_SCORE(DT, N, false, false); \
   JF_SCORE(DT, N, false, true);  \
@@ -590,21 +486,21 @@ int launch_score(const ScoreLaunch &a, uint32_t dtype, void *stream) {
   JF_SCORE_ALL(1, kSmallChunk / kSlab<1>);
 #undef JF_SCORE_ALL
 #undef JF_SCORE
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return (int)e;
-#define JF_FINISH(DT)                                                                     \
-  if (dtype == DT) {                                                                      \
-    if (a.teacher_ids && a.teacher_count <= 64)                                           \
-      hipLaunchKernelGGL((distill_loss_kernel<DT, 64>), rows, dim3(64), 0, st, a);        \
-    else if (a.teacher_ids)                                                               \
-      hipLaunchKernelGGL((distill_loss_kernel<DT, 256>), rows, dim3(256), 0, st, a);      \
-    else if (!top)                                                                        \
-      hipLaunchKernelGGL((logprobs_kernel<DT>), rows, dim3(64), 0, st, a);                \
-    else if (a.groups <= 10 * 256)                                                        \
-      hipLaunchKernelGGL((alternatives_kernel<DT, 10>), rows, dim3(256), 0, st, a);       \
-    else if (a.groups <= 16 * 256)                                                        \
-      hipLaunchKernelGGL((alternatives_kernel<DT, 16>), rows, dim3(256), 0, st, a);       \
-    else                                                                                  \
+  return (int)hipGetLastError();
+}
+
+int launch_logprobs(const ScoreLaunch &a, uint32_t dtype, void *stream) {
+  const hipStream_t st = (hipStream_t)stream;
+  const dim3 rows(a.row_count);
+#define JF_FINISH(DT)                                                                       \
+  if (dtype == DT) {                                                                        \
+    if (!a.top)                                                                             \
+      hipLaunchKernelGGL((logprobs_kernel<DT>), rows, dim3(64), 0, st, a);                  \
+    else if (a.groups <= 10 * 256)                                                          \
+      hipLaunchKernelGGL((alternatives_kernel<DT, 10>), rows, dim3(256), 0, st, a);         \
+    else if (a.groups <= 16 * 256)                                                          \
+      hipLaunchKernelGGL((alternatives_kernel<DT, 16>), rows, dim3(256), 0, st, a);         \
+    else                                                                                    \
       hipLaunchKernelGGL((alternatives_kernel<DT, kMostItems>), rows, dim3(256), 0, st, a); \
   }
   JF_FINISH(0)

@@ -427,7 +427,8 @@ int jf_logprobs(jf_scorer *s, const jf_logprobs_args *a, void *stream) {
     L.top = a->top;
     L.out_top_ids = at(a->out_top_ids, (uint64_t)r * a->top);
     L.out_top_logprobs = at(a->out_top_logprobs, (uint64_t)r * a->top);
-    const int e = jf::launch_score(L, a->dtype, stream);
+    int e = jf::launch_score(L, a->dtype, stream);
+    if (e == hipSuccess) e = jf::launch_logprobs(L, a->dtype, stream);
     if (e != hipSuccess) return hip_fail((hipError_t)e, "log-probabilities launch");
   }
   return JF_OK;
@@ -474,39 +475,42 @@ static int distill(jf_scorer *s, const jf_distill_args *a, bool forward, bool ba
   for (uint32_t r = 0; r < a->rows; r += most) {
     const uint32_t n = std::min(most, a->rows - r);
     float *saved = a->saved ? a->saved + (uint64_t)r * (2 + K) : backward ? s->saved : nullptr;
+    jf::ScoreLaunch L = score_rows(s, a->logits, stride, a->dtype, r, n);
+    jf::DistillGradLaunch G{};
+    L.temperature = G.temperature = a->temperature;
+    L.teacher_ids = G.teacher_ids = a->teacher_ids + r * a->teacher_stride;
+    L.teacher_stride = G.teacher_stride = a->teacher_stride;
+    L.teacher_count = G.teacher_count = K;
+    L.saved = saved;
+    G.saved = saved;
     if (forward) {
-      jf::ScoreLaunch L = score_rows(s, a->logits, stride, a->dtype, r, n);
-      L.temperature = a->temperature;
       L.out_lse = at(a->out_lse, r);
-      L.teacher_ids = a->teacher_ids + r * a->teacher_stride;
       L.teacher_values = a->teacher_values + r * a->teacher_stride;
-      L.teacher_stride = a->teacher_stride;
-      L.teacher_count = K;
       L.normalize = a->normalize ? 1u : 0u;
       L.out_loss = a->out_loss + r;
-      L.saved = saved;
-      const int e = jf::launch_score(L, a->dtype, stream);
-      if (e != hipSuccess) return hip_fail((hipError_t)e, "distillation launch");
     }
     if (backward) {
-      jf::DistillGradLaunch L{};
-      L.logits = rows_at(a->logits, r, stride, a->dtype);
-      L.stride = stride;
-      L.grad = (void *)rows_at(a->grad, r, grad_stride, a->dtype);
-      L.grad_stride = grad_stride;
-      L.row_count = n;
-      L.vocabulary = s->vocabulary;
-      L.chunks = s->chunks;
-      L.temperature = a->temperature;
-      L.teacher_ids = a->teacher_ids + r * a->teacher_stride;
-      L.teacher_stride = a->teacher_stride;
-      L.teacher_count = K;
-      L.saved = saved;
-      L.grad_loss = a->grad_loss + r * a->grad_loss_stride;
-      L.grad_loss_stride = a->grad_loss_stride;
-      const int e = jf::launch_distill_grad(L, a->dtype, stream);
-      if (e != hipSuccess) return hip_fail((hipError_t)e, "distillation gradient launch");
+      G.logits = L.logits;
+      G.stride = stride;
+      G.grad = (void *)rows_at(a->grad, r, grad_stride, a->dtype);
+      G.grad_stride = grad_stride;
+      G.row_count = n;
+      G.vocabulary = s->vocabulary;
+      G.chunks = s->chunks;
+      G.grad_loss = a->grad_loss + r * a->grad_loss_stride;
+      G.grad_loss_stride = a->grad_loss_stride;
     }
+    int e = hipSuccess;
+    static const char *ev = getenv("JF_STEP");
+    if (forward && backward && n >= (ev ? atoi(ev) : 1000000)) {
+      L.saved = a->saved ? saved : nullptr;
+      e = jf::launch_distill_step(L, G, a->dtype, stream);
+    } else {
+      if (forward) e = jf::launch_score(L, a->dtype, stream);
+      if (forward && e == hipSuccess) e = jf::launch_distill_loss(L, a->dtype, stream);
+      if (backward && e == hipSuccess) e = jf::launch_distill_grad(G, a->dtype, stream);
+    }
+    if (e != hipSuccess) return hip_fail((hipError_t)e, "distillation launch");
   }
   return JF_OK;
 }

@@ -110,8 +110,13 @@ struct DistillGradLaunch {
 // dtypes as JF_DTYPE_*. Each returns a hipError_t. The rows of one launch are
 // bounded so that its grid stays below 2^32 threads.
 int launch_process(const ProcessLaunch &a, uint32_t dtype, uint32_t out_dtype, void *stream);
-// Log-probabilities (a.teacher_ids NULL) or the distillation's forward pass.
+// The pass over the rows, and what finishes it.
 int launch_score(const ScoreLaunch &a, uint32_t dtype, void *stream);
+int launch_logprobs(const ScoreLaunch &a, uint32_t dtype, void *stream);
+int launch_distill_loss(const ScoreLaunch &a, uint32_t dtype, void *stream);
 int launch_distill_grad(const DistillGradLaunch &a, uint32_t dtype, void *stream);
+// Losses and gradients of the same rows at once.
+int launch_distill_step(const ScoreLaunch &a, const DistillGradLaunch &g, uint32_t dtype,
+                        void *stream);
 
 }  // namespace jf
