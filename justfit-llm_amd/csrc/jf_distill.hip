@@ -10,10 +10,18 @@
 // lane that holds the token subtracts p in registers and every element is
 // stored once (also where the gradient overwrites the logits).
 //
-// Both at once, for many rows: a block takes a whole row, reads it for m and S
-// and reads it again for the gradient. The rows in flight (two a CU) fit the
-// Infinity Cache, which serves the second reading, so HBM sees one read and one
-// write.
+// Both at once, for many rows: a block takes a whole row, reads it for m and S,
+// and takes it again for the gradient, a third of a 300 KB row from registers,
+// the rest from the caches. What the caches serve counts as well (their fabric
+// carries about 6 TB/s, read and written), so what is held is time: 2048 rows x
+// 151,936 bf16, 622 MB read and as much written, take 260 us; reading every row
+// twice 290, and the passes apart 353. Holding the whole row takes a CU's
+// registers for one block, which then reads, computes and writes in turn: 280.
+// The listed tokens' elements are stored once more behind the row's: looking
+// every vector's up cost 40 us.
+//
+// Gradients go past the caches (nontemporal stores; 256 rows: 32 us against 41),
+// which keeps the rows being read there.
 #include <hip/hip_runtime.h>
 
 #include "jf_logits.h"
@@ -21,6 +29,12 @@
 namespace jf {
 
 namespace {
+
+// P / S; 0 with no list, or no student probability anywhere: then there are no
+// exponentials to add.
+__device__ __forceinline__ float list_weight(float mass, const MaxSum &total) {
+  return mass == 0.0f || total.s == 0.0f ? 0.0f : mass / total.s;
+}
 
 // A row's list, worked out by one wave, SLOTS slots a lane: slot i * 64 + lane
 // is element i of its lane.
@@ -108,16 +122,11 @@ struct Teacher {
     float *saved = a.saved + (uint64_t)row * (2 + K);
     if (lane == 0) {
       saved[0] = total.m;
-      saved[1] = weight(total);
+      saved[1] = list_weight(mass, total);
     }
 #pragma unroll
     for (uint32_t i = 0; i < SLOTS; ++i)
       if (i * 64 + lane < K) saved[2 + i * 64 + lane] = valid[i] ? p[i] : -1.0f;
-  }
-  // P / S; 0 with no list, or no student probability anywhere: then there are
-  // no exponentials to add.
-  __device__ __forceinline__ float weight(const MaxSum &total) const {
-    return mass == 0.0f || total.s == 0.0f ? 0.0f : mass / total.s;
   }
 };
 
@@ -133,103 +142,112 @@ __global__ __launch_bounds__(64) void distill_loss_kernel(ScoreLaunch a) {
   t.put(a, row, total, RowScore{total.m, inv_t, logf(total.s)});
 }
 
-constexpr uint32_t kStepThreads = 1024;
+// A training step's block: two of them on a CU, so that one reads while the
+// other computes or writes.
+constexpr uint32_t kStepThreads = 512;
 constexpr uint32_t kStepWaves = kStepThreads / 64;
-constexpr uint32_t kStepLoads = 2;  // vectors a thread has in flight
+constexpr uint32_t kQuad = 4;       // vectors a thread loads, adds and stores together
+constexpr uint32_t kHeldQuads = 3;  // of them held from the first pass to the second
 
 template <int DT, uint32_t SLOTS>
-__global__ __launch_bounds__(kStepThreads, 8) void distill_step_kernel(ScoreLaunch a,
+__global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaunch a,
                                                                        DistillGradLaunch g) {
-  constexpr uint32_t VEC = Logits<DT>::VEC, SLAB = kStepThreads * VEC;
-  extern __shared__ uint32_t marked[];  // a bit a token
+  constexpr uint32_t VEC = Logits<DT>::VEC, SLAB = kStepThreads * VEC, QUAD = kQuad * SLAB;
+  using Words = typename Logits<DT>::Words;
   __shared__ uint32_t listed[64 * SLOTS];
-  __shared__ float share[64 * SLOTS];
   __shared__ MaxSum part[kStepWaves];
-  __shared__ float weight;
+  __shared__ float mass;
   const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63u, row = blockIdx.x;
-  const uint32_t V = a.vocabulary;
+  const uint32_t V = a.vocabulary, quads = V / QUAD;
   const auto *z = row_of<DT>(a.logits, (uint64_t)row * a.stride);
   auto *dz = row_of<DT>(g.grad, (uint64_t)row * g.grad_stride);
   const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
   const float scale = g.grad_loss[(uint64_t)row * g.grad_loss_stride] * inv_t;
-  for (uint32_t i = tid; i < (V + 31) / 32; i += kStepThreads) marked[i] = 0;
-  MaxSum run{-__builtin_inff(), 0.0f};
-  for (uint32_t base = 0; base < V; base += kStepLoads * SLAB) {
-    LogitWords w[kStepLoads];
-    float top[kStepLoads];
-    if (base + kStepLoads * SLAB <= V) {
+  const auto load = [&](uint32_t quad, LogitWords (&w)[kQuad]) {
 #pragma unroll
-      for (uint32_t j = 0; j < kStepLoads; ++j)
-        w[j] = *(const typename Logits<DT>::Words *)(z + base + j * SLAB + tid * VEC);
-    } else {
+    for (uint32_t j = 0; j < kQuad; ++j)
+      w[j] = *(const Words *)(z + quad * QUAD + j * SLAB + tid * VEC);
+  };
+  // `rest`: the vectors past the last whole quad.
+  LogitWords held[kHeldQuads][kQuad], rest[kQuad];
 #pragma unroll
-      for (uint32_t j = 0; j < kStepLoads; ++j)
-        w[j] = load_words<DT>(z, base + j * SLAB + tid * VEC, V, kPastMinusInfinity<DT>);
-    }
+  for (uint32_t q = 0; q < kHeldQuads; ++q)
+    if (q < quads) load(q, held[q]);
 #pragma unroll
-    for (uint32_t j = 0; j < kStepLoads; ++j) top[j] = vector_max<DT>(w[j]);
-    add_vectors<DT>(run, w, top, c);
+  for (uint32_t j = 0; j < kQuad; ++j)
+    rest[j] = load_words<DT>(z, quads * QUAD + j * SLAB + tid * VEC, V, kPastMinusInfinity<DT>);
+  // The first wave works the list out while the row arrives.
+  Teacher<DT, SLOTS> t;
+  if (wave == 0) {
+    t.load(a, row, z, inv_t, listed);
+    if (lane == 0) mass = t.mass;
   }
+  MaxSum run{-__builtin_inff(), 0.0f};
+  const auto add = [&](const LogitWords (&w)[kQuad]) {
+    float top[kQuad];
+#pragma unroll
+    for (uint32_t j = 0; j < kQuad; ++j) top[j] = vector_max<DT>(w[j]);
+    add_vectors<DT>(run, w, top, c);
+  };
+#pragma unroll
+  for (uint32_t q = 0; q < kHeldQuads; ++q)
+    if (q < quads) add(held[q]);
+  for (uint32_t q = kHeldQuads; q < quads; ++q) {
+    LogitWords w[kQuad];
+    load(q, w);
+    add(w);
+  }
+  add(rest);
   run = wave_join(run, c);
   if (lane == 0) part[wave] = run;
   __syncthreads();
+  // The held words anew, or the compiler keeps the values it unpacked above,
+  // two registers a word.
+#pragma unroll
+  for (uint32_t q = 0; q < kHeldQuads; ++q)
+#pragma unroll
+    for (uint32_t j = 0; j < kQuad; ++j) asm volatile("" : "+v"(held[q][j]));
   MaxSum total = lane < kStepWaves ? part[lane] : MaxSum{-__builtin_inff(), 0.0f};
   total = wave_join(total, c);
-  if (wave == 0) {
-    Teacher<DT, SLOTS> t;
-    t.load(a, row, z, inv_t, listed);
-    t.put(a, row, total, RowScore{total.m, inv_t, logf(total.s)});
-    if (lane == 0) weight = scale * t.weight(total);
-#pragma unroll
-    for (uint32_t i = 0; i < SLOTS; ++i) {
-      share[i * 64 + lane] = t.valid[i] ? scale * t.p[i] : 0.0f;
-      if (t.valid[i] && scale != 0.0f) atomicOr(&marked[t.id[i] >> 5], 1u << (t.id[i] & 31u));
-    }
-  }
-  __syncthreads();
-  const float weight_ = weight;
+  const float m = total.m, weight = scale * list_weight(mass, total);
   // A row with no list, or whose loss nothing follows from, has no gradient.
-  const bool any = weight_ != 0.0f && scale != 0.0f;
-  const float m = total.m;
-  for (uint32_t base = 0; base < V; base += kStepLoads * SLAB) {
-    LogitWords w[kStepLoads];
-    if (any) {
-      if (base + kStepLoads * SLAB <= V) {
+  const bool any = weight != 0.0f && scale != 0.0f;
+  const auto pulled = [&](float logit) { return any ? weight * exp_below(logit, m, c) : 0.0f; };
+  const auto gradient = [&](const LogitWords &w) {
+    float v[VEC];
+    unpack<DT>(w, v);
 #pragma unroll
-        for (uint32_t j = 0; j < kStepLoads; ++j)
-          w[j] = *(const typename Logits<DT>::Words *)(z + base + j * SLAB + tid * VEC);
-      } else {
+    for (uint32_t e = 0; e < VEC; ++e) v[e] = pulled(v[e]);
+    return pack<DT>(v);
+  };
+  const auto put = [&](uint32_t quad, const LogitWords (&w)[kQuad]) {
 #pragma unroll
-        for (uint32_t j = 0; j < kStepLoads; ++j)
-          w[j] = load_words<DT>(z, base + j * SLAB + tid * VEC, V, 0);
-      }
-    }
+    for (uint32_t j = 0; j < kQuad; ++j)
+      __builtin_nontemporal_store(gradient(w[j]),
+                                  (Words *)(dz + quad * QUAD + j * SLAB + tid * VEC));
+  };
+  // The quads read again come first, the last read before the others.
+  for (uint32_t q = quads; q-- > kHeldQuads;) {
+    LogitWords w[kQuad];
+    load(q, w);
+    put(q, w);
+  }
 #pragma unroll
-    for (uint32_t j = 0; j < kStepLoads; ++j) {
-      const uint32_t token = base + j * SLAB + tid * VEC;
-      if (token >= V) continue;
-      float v[VEC];
-      if (any) {
-        unpack<DT>(w[j], v);
+  for (uint32_t q = 0; q < kHeldQuads; ++q)
+    if (q < quads) put(q, held[q]);
 #pragma unroll
-        for (uint32_t e = 0; e < VEC; ++e)
-          v[e] = weight_ * exp_below(v[e], m, c);
-      } else {
+  for (uint32_t j = 0; j < kQuad; ++j) {
+    const uint32_t token = quads * QUAD + j * SLAB + tid * VEC;
+    if (token < V) store_words<DT>(dz, token, V, gradient(rest[j]));
+  }
+  if (wave == 0) t.put(a, row, total, RowScore{total.m, inv_t, logf(total.s)});
+  // The listed tokens' elements anew, once every store above has completed.
+  wait_memory();
+  __syncthreads();
+  if (wave == 0 && scale != 0.0f) {
 #pragma unroll
-        for (uint32_t e = 0; e < VEC; ++e) v[e] = 0.0f;
-      }
-      const uint32_t bits = (marked[token >> 5] >> (token & 31u)) & ((1u << VEC) - 1u);
-      if (bits) {
-#pragma unroll
-        for (uint32_t e = 0; e < VEC; ++e)
-          if (bits >> e & 1u) {
-            uint32_t k = 0;
-            while (listed[k] != token + e) ++k;
-            v[e] -= share[k];
-          }
-      }
-      store_words<DT>(dz, token, V, pack<DT>(v));
-    }
+    for (uint32_t i = 0; i < SLOTS; ++i)
+      if (t.valid[i]) dz[t.id[i]] = logit_of<DT>(pulled(t.logit[i]) - scale * t.p[i]);
   }
 }
 
@@ -284,7 +302,10 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillGradLaunch a) 
       for (uint32_t e = 0; e < VEC; ++e)
         if (bits >> e & 1u) v[e] -= share[slot[at + e]];
     }
-    store_words<DT>(dz, token, V, pack<DT>(v));
+    if (token + VEC <= V)
+      __builtin_nontemporal_store(pack<DT>(v), (typename Logits<DT>::Words *)(dz + token));
+    else
+      store_words<DT>(dz, token, V, pack<DT>(v));
   }
 }
 
@@ -309,16 +330,15 @@ int launch_distill_step(const ScoreLaunch &a, const DistillGradLaunch &g, uint32
                         void *stream) {
   const dim3 rows(a.row_count), block(kStepThreads);
   const hipStream_t st = (hipStream_t)stream;
-  const uint32_t bits = (a.vocabulary + 31) / 32 * sizeof(uint32_t);  // 64 KB at most
   const bool one = a.teacher_count <= 64;
   if (dtype == 0 && one)
-    hipLaunchKernelGGL((distill_step_kernel<0, 1>), rows, block, bits, st, a, g);
+    hipLaunchKernelGGL((distill_step_kernel<0, 1>), rows, block, 0, st, a, g);
   else if (dtype == 0)
-    hipLaunchKernelGGL((distill_step_kernel<0, 4>), rows, block, bits, st, a, g);
+    hipLaunchKernelGGL((distill_step_kernel<0, 4>), rows, block, 0, st, a, g);
   else if (one)
-    hipLaunchKernelGGL((distill_step_kernel<1, 1>), rows, block, bits, st, a, g);
+    hipLaunchKernelGGL((distill_step_kernel<1, 1>), rows, block, 0, st, a, g);
   else
-    hipLaunchKernelGGL((distill_step_kernel<1, 4>), rows, block, bits, st, a, g);
+    hipLaunchKernelGGL((distill_step_kernel<1, 4>), rows, block, 0, st, a, g);
   return (int)hipGetLastError();
 }
 

@@ -464,6 +464,18 @@ static int check_distill(const jf_scorer *s, const jf_distill_args *a, bool forw
   return JF_OK;
 }
 
+// Whether a training step takes its rows whole, a block each, in one launch. A
+// short row is done before three launches would be (32,000 tokens bf16: 7.5 us
+// against 13.6 at 16 rows, 14.9 against 24.8 at 512). A long one keeps its block
+// busy longer than the rows' chunks spread over the GPU would take, unless there
+// are rows for every CU: with 4 KB of a row for each row (151,936 bf16, 64 rows
+// 21.3 us against 17.7 and 128 rows 22.7 against 25.9; fp32, 128 rows 44.3
+// against 42.6 and 256 rows 74.9 against 77.8).
+static bool whole_rows(uint32_t rows, uint32_t vocabulary, uint32_t dtype) {
+  const size_t row_bytes = vocabulary * element_size(dtype);
+  return row_bytes <= (128u << 10) || rows >= row_bytes / 4096;
+}
+
 static int distill(jf_scorer *s, const jf_distill_args *a, bool forward, bool backward,
                    void *stream) {
   if (!s || !a) return fail(JF_ERR_INVALID_ARGUMENT, "null scorer or arguments");
@@ -501,8 +513,7 @@ static int distill(jf_scorer *s, const jf_distill_args *a, bool forward, bool ba
       G.grad_loss_stride = a->grad_loss_stride;
     }
     int e = hipSuccess;
-    static const char *ev = getenv("JF_STEP");
-    if (forward && backward && n >= (ev ? atoi(ev) : 1000000)) {
+    if (forward && backward && whole_rows(n, s->vocabulary, a->dtype)) {
       L.saved = a->saved ? saved : nullptr;
       e = jf::launch_distill_step(L, G, a->dtype, stream);
     } else {
