@@ -11,10 +11,11 @@
 // place of the word's first entry. Then the chunk's vectors go from registers
 // to the output; the lane that holds an edited token finds its entry by the
 // word's first place and the bits before it. That keeps a block at 13 KB of
-// LDS, eight blocks on a CU: what bounds the kernel is the chain of dependent
-// loads (row record, list bounds and mask, entries and vectors, entries'
-// logits), and the chunks in flight hide it. (A tile of 8192 values in LDS held
-// four blocks: 256 masked rows x 248,320 bf16 took 73 us.)
+// LDS, eight blocks on a CU: what bounds a call of few rows is the chain of
+// dependent loads (row record, list bounds and mask, entries and vectors,
+// entries' logits), and the chunks in flight hide it in larger ones. (A tile of
+// 8192 values in LDS held four blocks: 256 masked rows x 248,320 bf16 took 73
+// us, 46.7 as here; with nontemporal stores, 28.7.)
 //
 // A vector is loaded only if one of its tokens is admitted, and in place
 // written only if one of them changes: a grammar's row, which drops nearly all
@@ -29,21 +30,85 @@ namespace jf {
 
 namespace {
 
-constexpr uint32_t kMapWords = kScoreChunk / 32;
 constexpr uint32_t kStaged = 1024;  // a list's entries in LDS; later ones stay in memory
 
 // A list's entries of the chunk.
+template <uint32_t CHUNK>
 struct ListLds {
-  uint32_t bits[kMapWords];
-  uint16_t first[kMapWords];  // of a word with any bit
+  uint32_t bits[CHUNK / 32];
+  uint16_t first[CHUNK / 32];  // of a word with any bit
   float value[kStaged];
 };
+template <uint32_t CHUNK>
 struct ProcessLds {
-  ListLds penalty, bias;
-  uint32_t admitted[kMapWords];
-  uint32_t extra_bits[kMapWords];  // extra tokens that the table does not hold
+  ListLds<CHUNK> penalty, bias;
+  uint32_t admitted[CHUNK / 32];
+  uint32_t extra_bits[CHUNK / 32];  // extra tokens that the table does not hold
   uint32_t extras[kMaxExtra];
   float extra_value[kMaxExtra];
+};
+
+// VEC tokens of a row of type DT as a lane loads or stores them: 16 bytes, or 8
+// bytes of bf16 where the other side is f32, so that a wave's loads and its
+// stores both cover whole lines.
+template <int DT, uint32_t VEC>
+struct Tokens {
+  using Element = typename Logits<DT>::Element;
+  static constexpr uint32_t WORDS = VEC * sizeof(Element) / 4;
+  typedef uint32_t Words __attribute__((ext_vector_type(WORDS)));
+  typedef Words WordsAt __attribute__((aligned(sizeof(Element))));
+
+  static __device__ __forceinline__ Words load(const Element *row, uint32_t token, uint32_t V) {
+    if (token + VEC <= V) return *(const WordsAt *)(row + token);
+    Words w{};
+#pragma unroll
+    for (uint32_t e = 0; e < VEC; ++e)
+      if (token + e < V) {
+        if constexpr (DT == 0)
+          w[e] = f2u(row[token + e]);
+        else
+          w[e / 2] |= (uint32_t)row[token + e] << (16 * (e & 1));
+      }
+    return w;
+  }
+  template <bool NT>
+  static __device__ __forceinline__ void store(Element *row, uint32_t token, uint32_t V, Words w) {
+    if (token + VEC <= V) {
+      if constexpr (NT)
+        __builtin_nontemporal_store(w, (WordsAt *)(row + token));
+      else
+        *(WordsAt *)(row + token) = w;
+      return;
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < VEC; ++e)
+      if (token + e < V) {
+        if constexpr (DT == 0)
+          row[token + e] = u2f(w[e]);
+        else
+          row[token + e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+      }
+  }
+  static __device__ __forceinline__ void unpack(Words w, float (&v)[VEC]) {
+#pragma unroll
+    for (uint32_t e = 0; e < VEC; ++e) {
+      if constexpr (DT == 0)
+        v[e] = u2f(w[e]);
+      else
+        v[e] = u2f(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    }
+  }
+  static __device__ __forceinline__ Words pack(const float (&v)[VEC]) {
+    Words w;
+#pragma unroll
+    for (uint32_t i = 0; i < WORDS; ++i) {
+      if constexpr (DT == 0)
+        w[i] = f2u(v[i]);
+      else
+        w[i] = floats_to_bf16(v[2 * i], v[2 * i + 1]);
+    }
+    return w;
+  }
 };
 
 // VEC bits of a bitmap from token `at` of the chunk (a multiple of VEC).
@@ -55,25 +120,31 @@ __device__ __forceinline__ bool bit_at(const uint32_t *map, uint32_t at) {
   return map[at >> 5] >> (at & 31u) & 1u;
 }
 // The place in its list's chunk of the entry of token `at`, which it holds.
-__device__ __forceinline__ uint32_t place_at(const ListLds &l, uint32_t at) {
+template <class List>
+__device__ __forceinline__ uint32_t place_at(const List &l, uint32_t at) {
   return l.first[at >> 5] + __popc(l.bits[at >> 5] & ((1u << (at & 31u)) - 1u));
 }
 // Entry i of a list's chunk: its bit, and its place if it begins a word.
-__device__ __forceinline__ void mark(ListLds &l, const PenaltyEntry *list, uint32_t i,
+template <class List>
+__device__ __forceinline__ void mark(List &l, const PenaltyEntry *list, uint32_t i,
                                      uint32_t token, uint32_t base) {
   const uint32_t at = token - base;
   atomicOr(&l.bits[at >> 5], 1u << (at & 31u));
   if (i == 0 || (list[i - 1].token - base) >> 5 != at >> 5) l.first[at >> 5] = (uint16_t)i;
 }
 
-template <int DI, int DO>
+// A chunk of N vectors a thread.
+template <int DI, int DO, uint32_t N, bool NT>
 __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
-  constexpr uint32_t VEC = Logits<DI>::VEC, SLAB = kSlab<DI>, LOADS = kLoads<DI>;
+  constexpr uint32_t VEC = DI == 1 && DO == 1 ? 8 : 4, SLAB = 256 * VEC, CHUNK = N * SLAB;
   constexpr uint32_t ALL = (1u << VEC) - 1u;
-  __shared__ ProcessLds s;
+  static_assert(CHUNK % kPenaltyBucket == 0 && CHUNK / 32 <= 256);
+  using In = Tokens<DI, VEC>;
+  using Out = Tokens<DO, VEC>;
+  __shared__ ProcessLds<CHUNK> s;
   const uint32_t tid = threadIdx.x;
   const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks;
-  const uint32_t base = chunk * kScoreChunk, V = a.vocabulary;
+  const uint32_t base = chunk * CHUNK, V = a.vocabulary;
   const ProcessRow p = a.rows[row];
   const auto *x = row_of<DI>(a.logits, (uint64_t)row * a.stride);
   auto *y = row_of<DO>(a.out, (uint64_t)row * a.out_stride);
@@ -81,12 +152,21 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
 
   // An unmasked row that is written elsewhere needs every vector: ask first.
   const bool whole = !masked && !a.in_place;
-  LogitWords w[LOADS];
-  if (whole) load_chunk<DI>(x, base, V, 0, w);
+  typename In::Words w[N];
+  if (whole) {
+    if (base + CHUNK <= V) {
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j)
+        w[j] = *(const typename In::WordsAt *)(x + base + j * SLAB + tid * VEC);
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) w[j] = In::load(x, base + j * SLAB + tid * VEC, V);
+    }
+  }
 
   uint32_t pen0 = 0, pens = 0, bias0 = 0, biases = 0;
-  const uint32_t b0 = chunk * (kScoreChunk / kPenaltyBucket);
-  const uint32_t b1 = min(b0 + kScoreChunk / kPenaltyBucket, a.buckets);
+  const uint32_t b0 = chunk * (CHUNK / kPenaltyBucket);
+  const uint32_t b1 = min(b0 + CHUNK / kPenaltyBucket, a.buckets);
   if (p.penalty_row != kNoRow) {
     const uint32_t *off = a.pen_offsets + (uint64_t)p.penalty_row * (a.buckets + 1);
     pen0 = off[b0];
@@ -97,8 +177,9 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
     bias0 = off[b0];
     biases = off[b1] - bias0;
   }
-  s.penalty.bits[tid] = s.bias.bits[tid] = s.extra_bits[tid] = 0;
-  if (masked) {
+  const bool has_word = tid < CHUNK / 32;
+  if (has_word) s.penalty.bits[tid] = s.bias.bits[tid] = s.extra_bits[tid] = 0;
+  if (masked && has_word) {
     // Tokens past the vocabulary are never stored; words past it not read.
     const uint32_t word = base / 32 + tid;
     uint32_t bits = 0xffffffffu;
@@ -115,10 +196,10 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
   if (edits || masked) __syncthreads();
   if (!whole && !a.in_place) {
 #pragma unroll
-    for (uint32_t j = 0; j < LOADS; ++j) {
+    for (uint32_t j = 0; j < N; ++j) {
       const uint32_t at = j * SLAB + tid * VEC;
-      w[j] = LogitWords{};
-      if (base + at < V && bits_at<VEC>(s.admitted, at)) w[j] = load_words<DI>(x, base + at, V, 0);
+      w[j] = typename In::Words{};
+      if (base + at < V && bits_at<VEC>(s.admitted, at)) w[j] = In::load(x, base + at, V);
     }
   }
   const PenaltyEntry *pen_list =
@@ -147,7 +228,7 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
     if (tid < p.extra_count) {
       const PenaltyEntry e{s.extras[tid], 0};
       const uint32_t at = e.token - base;
-      if (e.token < V && at < kScoreChunk && !bit_at(s.penalty.bits, at)) {
+      if (e.token < V && at < CHUNK && !bit_at(s.penalty.bits, at)) {
         // A token that comes more than once leaves the same value each time.
         s.extra_value[tid] = penalized(e, logit_value(x[e.token]));
         atomicOr(&s.extra_bits[at >> 5], 1u << (at & 31u));
@@ -164,30 +245,32 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
   };
   if (a.in_place) {
 #pragma unroll
-    for (uint32_t j = 0; j < LOADS; ++j) {
+    for (uint32_t j = 0; j < N; ++j) {
       const uint32_t at = j * SLAB + tid * VEC;
-      w[j] = LogitWords{};
+      w[j] = typename In::Words{};
       if (base + at >= V) continue;
       const uint32_t admitted = masked ? bits_at<VEC>(s.admitted, at) : ALL;
       if (admitted && (admitted != ALL || edited_at(at)))
-        w[j] = load_words<DI>(x, base + at, V, 0);
+        w[j] = In::load(x, base + at, V);
     }
     // A neighbour's edit reads no logit that this block writes: every read of
     // a list's logit came before the barrier above.
   }
 #pragma unroll
-  for (uint32_t j = 0; j < LOADS; ++j) {
+  for (uint32_t j = 0; j < N; ++j) {
     const uint32_t at = j * SLAB + tid * VEC, token = base + at;
     if (token >= V) continue;
     const uint32_t admitted = masked ? bits_at<VEC>(s.admitted, at) : ALL;
     const uint32_t edited = edited_at(at) & admitted;
     if (a.in_place && !edited && admitted == ALL) continue;
-    if (DI == DO && !edited && admitted == ALL) {
-      store_words<DO>(y, token, V, w[j]);
-      continue;
+    if constexpr (DI == DO) {
+      if (!edited && admitted == ALL) {
+        Out::template store<NT>(y, token, V, w[j]);
+        continue;
+      }
     }
     float v[VEC];
-    unpack<DI>(w[j], v);
+    In::unpack(w[j], v);
     if (edited) {
 #pragma unroll
       for (uint32_t e = 0; e < VEC; ++e) {
@@ -211,41 +294,56 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
 #pragma unroll
     for (uint32_t e = 0; e < VEC; ++e)
       if (!(admitted >> e & 1u)) v[e] = -__builtin_inff();
-    if constexpr (DI == DO) {
-      store_words<DO>(y, token, V, pack<DO>(v));
-    } else if constexpr (DI == 1) {
-      float half[4];
-#pragma unroll
-      for (uint32_t h = 0; h < 2; ++h) {
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) half[e] = v[h * 4 + e];
-        if (token + h * 4 < V) store_words<0>(y, token + h * 4, V, pack<0>(half));
-      }
-    } else if (token + VEC <= V) {
-      typedef uint32_t Pair __attribute__((ext_vector_type(2)));
-      typedef Pair PairAt2 __attribute__((aligned(2)));
-      *(PairAt2 *)(y + token) = Pair{floats_to_bf16(v[0], v[1]), floats_to_bf16(v[2], v[3])};
-    } else {
-#pragma unroll
-      for (uint32_t e = 0; e < VEC; ++e)
-        if (token + e < V) y[token + e] = logit_of<DO>(v[e]);
-    }
+    Out::template store<NT>(y, token, V, Out::pack(v));
   }
+}
+
+// Outputs of more than this go past the caches (nontemporal stores): alone, 256
+// masked rows x 248,320 bf16 take 28.7 us so, 46.5 otherwise, and 67.3 or 67.6
+// with a pass that reads them behind; 64 rows x 151,936 in f32, 39 MB, 15.0 or
+// 16.3, and 26.0 or 26.5. A smaller output is found there by its reader: 16 such
+// rows 6.6 or 7.3, but 14.7 or 14.2 with the reader.
+constexpr uint64_t kCachedOutput = 24u << 20;
+
+template <int DI, int DO, uint32_t CHUNK>
+void launch_chunks(ProcessLaunch a, hipStream_t stream) {
+  constexpr uint32_t N = CHUNK / (256 * (DI == 1 && DO == 1 ? 8 : 4));
+  a.chunks = (a.vocabulary + CHUNK - 1) / CHUNK;
+  const dim3 grid(a.row_count * a.chunks), block(256);
+  if ((uint64_t)a.row_count * a.vocabulary * sizeof(typename Logits<DO>::Element) > kCachedOutput)
+    hipLaunchKernelGGL((process_kernel<DI, DO, N, true>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((process_kernel<DI, DO, N, false>), grid, block, 0, stream, a);
+}
+
+// Small chunks while there are few, for blocks on every CU (16 rows x 151,936:
+// 6.6 us in chunks of 2048 tokens, 7.8 of 4096, 11.0 of 8192; 48 rows 12.4, 11.0
+// and 13.3; 128 rows 25.7, 23.4 and 26.0). Masked rows are mostly written without
+// being read, and then a chunk's cost is that of its block: 256 such rows x
+// 248,320 bf16 48.3, 33.2 and 28.6.
+template <int DI, int DO>
+void launch_types(const ProcessLaunch &a, hipStream_t stream) {
+  const uint64_t tokens = (uint64_t)a.row_count * a.vocabulary;
+  if (tokens <= 512u * 8192u)
+    launch_chunks<DI, DO, 2048>(a, stream);
+  else if (a.all_masked && tokens > 2048u * 8192u)
+    launch_chunks<DI, DO, 8192>(a, stream);
+  else
+    launch_chunks<DI, DO, 4096>(a, stream);
 }
 
 }  // namespace
 
 int launch_process(const ProcessLaunch &a, uint32_t dtype, uint32_t out_dtype, void *stream) {
-  const dim3 grid(a.row_count * a.chunks), block(256);
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == 0 && out_dtype == 0)
-    hipLaunchKernelGGL((process_kernel<0, 0>), grid, block, 0, st, a);
+    launch_types<0, 0>(a, st);
   else if (dtype == 0)
-    hipLaunchKernelGGL((process_kernel<0, 1>), grid, block, 0, st, a);
+    launch_types<0, 1>(a, st);
   else if (out_dtype == 0)
-    hipLaunchKernelGGL((process_kernel<1, 0>), grid, block, 0, st, a);
+    launch_types<1, 0>(a, st);
   else
-    hipLaunchKernelGGL((process_kernel<1, 1>), grid, block, 0, st, a);
+    launch_types<1, 1>(a, st);
   return (int)hipGetLastError();
 }
 

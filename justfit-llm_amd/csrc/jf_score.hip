@@ -383,7 +383,7 @@ JF_MAX_STEP(max_sixteens, "row_mirror")     // of eights that agree
 #undef JF_MAX_STEP
 #undef JF_MAX_DPP
 
-// A block's segment of a row: chunks of N slabs.
+// A block's chunk of a row, N slabs.
 template <int DT, uint32_t N, bool RANK, bool TOP>
 __global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
   constexpr uint32_t VEC = Logits<DT>::VEC, SLAB = kSlab<DT>, CHUNK = N * SLAB;
@@ -405,49 +405,45 @@ __global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
     }
   }
   MaxSum run{-__builtin_inff(), 0.0f};
-  const uint32_t first = segment * a.segment_chunks;
-  const uint32_t last = min(first + a.segment_chunks, (V + CHUNK - 1) / CHUNK);
-  for (uint32_t chunk = first; chunk < last; ++chunk) {
-    const uint32_t base = chunk * CHUNK;
-    LogitWords w[N];
-    load_chunk<DT>(x, base, V, kPastMinusInfinity<DT>, w);
-    float part[N];
+  const uint32_t base = segment * CHUNK;
+  LogitWords w[N];
+  load_chunk<DT>(x, base, V, kPastMinusInfinity<DT>, w);
+  float part[N];
 #pragma unroll
-    for (uint32_t j = 0; j < N; ++j) part[j] = vector_max<DT>(w[j]);
-    add_vectors<DT>(run, w, part, c);
-    if constexpr (RANK) {
-      if (target < V) {
-        // Ids before the target's are ahead of it at equal logits too.
-        const bool mixed = target - base < CHUNK;
-        const float least = base < target ? at_target : above_target;
+  for (uint32_t j = 0; j < N; ++j) part[j] = vector_max<DT>(w[j]);
+  add_vectors<DT>(run, w, part, c);
+  if constexpr (RANK) {
+    if (target < V) {
+      // Ids before the target's are ahead of it at equal logits too.
+      const bool mixed = target - base < CHUNK;
+      const float least = base < target ? at_target : above_target;
 #pragma unroll
-        for (uint32_t j = 0; j < N; ++j) {
-          float v[VEC];
-          unpack<DT>(w[j], v);
+      for (uint32_t j = 0; j < N; ++j) {
+        float v[VEC];
+        unpack<DT>(w[j], v);
 #pragma unroll
-          for (uint32_t e = 0; e < VEC; ++e) {
-            const float from =
-                mixed && base + j * SLAB + tid * VEC + e >= target ? above_target : least;
-            ahead += v[e] >= from ? 1u : 0u;
-          }
+        for (uint32_t e = 0; e < VEC; ++e) {
+          const float from =
+              mixed && base + j * SLAB + tid * VEC + e >= target ? above_target : least;
+          ahead += v[e] >= from ? 1u : 0u;
         }
       }
     }
-    if constexpr (TOP) {
-      // A group's 64 tokens lie in 16 (f32) or 8 (bf16) neighbouring lanes, of
-      // which the j-th writes the group of vector j: a wave's store is a run.
-      constexpr uint32_t LANES = kScoreGroup / VEC;
-      max_pairs(part);
-      max_quads(part);
-      max_eights(part);
-      if constexpr (DT == 0) max_sixteens(part);
-      float own = part[0];
+  }
+  if constexpr (TOP) {
+    // A group's 64 tokens lie in 16 (f32) or 8 (bf16) neighbouring lanes, of
+    // which the j-th writes the group of vector j: a wave's store is a run.
+    constexpr uint32_t LANES = kScoreGroup / VEC;
+    max_pairs(part);
+    max_quads(part);
+    max_eights(part);
+    if constexpr (DT == 0) max_sixteens(part);
+    float own = part[0];
 #pragma unroll
-      for (uint32_t j = 1; j < N; ++j) own = tid % LANES == j ? part[j] : own;
-      if (tid % LANES < N)
-        a.maxima[(uint64_t)row * a.groups + base / kScoreGroup + tid / LANES * N + tid % LANES] =
-            own;
-    }
+    for (uint32_t j = 1; j < N; ++j) own = tid % LANES == j ? part[j] : own;
+    if (tid % LANES < N)
+      a.maxima[(uint64_t)row * a.groups + base / kScoreGroup + tid / LANES * N + tid % LANES] =
+          own;
   }
   run = wave_join(run, c);
   if constexpr (RANK) ahead = wave_sum_u32(ahead);

@@ -44,8 +44,10 @@ struct ProcessLaunch {
   void *out;
   uint64_t stride, out_stride;
   const ProcessRow *rows;
-  uint32_t row_count, vocabulary, chunks;
+  uint32_t row_count, vocabulary;
+  uint32_t chunks;  // of a row: the launch's own
   uint32_t in_place;
+  uint32_t all_masked;
   const uint32_t *masks;
   uint64_t mask_stride;
   uint32_t stop0, stop1;
@@ -64,8 +66,7 @@ struct ScoreLaunch {
   uint64_t stride;
   uint32_t row_count, vocabulary;
   uint32_t small;           // chunks of kSmallChunk tokens, otherwise kScoreChunk
-  uint32_t segments;        // blocks a row
-  uint32_t segment_chunks;  // chunks a block
+  uint32_t segments;        // blocks a row, one a chunk
   uint32_t groups;          // groups a row, padded to whole chunks
   const float *temperatures;  // device, or NULL: `temperature` for every row
   float temperature;
