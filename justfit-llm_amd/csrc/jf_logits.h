@@ -164,8 +164,8 @@ __device__ __forceinline__ float wave_sum_f32(float v) {
 }
 
 // Maxima of values as they are loaded: fmax quiets each of its operands first,
-// an instruction a value. A signalling NaN makes these NaN, a quiet one is
-// passed over.
+// an instruction a value. A quiet NaN is passed over; a signalling one may
+// take others' places, but then the sum of their exponentials is NaN as well.
 __device__ __forceinline__ float loaded_max(float a, float b) {
   float r;
   asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));

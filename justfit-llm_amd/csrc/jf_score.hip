@@ -52,6 +52,8 @@ __device__ __forceinline__ const T *element(const T *row, uint32_t i) {
   return (const T *)((const char *)row + (uint32_t)(i * sizeof(T)));
 }
 
+// A row's block: four waves for its alternatives, one for its totals.
+constexpr uint32_t kTopWaves = 5;
 constexpr uint32_t kMostItems = 32;  // groups a thread holds at most
 constexpr uint32_t kWaveGroups = 128;  // groups a wave lists at most
 // Tokens a wave lists at most. A row whose best tokens are neighbours lists most
@@ -67,33 +69,24 @@ struct TopLds {
   uint32_t unit[256];                // the units' best keys
   uint16_t group[4][kWaveGroups];
   uint32_t best[kTopLogprobs];
-  uint64_t wave[2][4];
+  uint64_t wave[2][kTopWaves];
   uint32_t count[4];
   uint32_t crowded;
+  RowScore score;
 };
 
 // The group whose maximum is the i-th of its row: a chunk's groups are stored in
-// the order (lanes, vector), the passes' own (score_kernel).
+// the order (lanes, vector), the pass's own (score_kernel).
 template <int DT>
 __device__ __forceinline__ uint32_t group_at(const ScoreLaunch &a, uint32_t i) {
-  constexpr uint32_t SLAB_GROUPS = kSlab<DT> / kScoreGroup;
-  const uint32_t vectors = (a.small ? kSmallChunk : kScoreChunk) / kSlab<DT>;
-  const uint32_t groups = vectors * SLAB_GROUPS, within = i % groups;
-  return i - within + within % vectors * SLAB_GROUPS + within / vectors;
+  // Of a chunk: 2^lv vectors of 2^ls groups.
+  constexpr uint32_t ls = DT == 0 ? 4 : 5;
+  static_assert(kSlab<DT> / kScoreGroup == 1u << ls);
+  const uint32_t lv = (DT == 0 ? 3u : 2u) - (a.small ? 2u : 0u);
+  static_assert(kScoreChunk / kSlab<DT> == (DT == 0 ? 8 : 4) && kScoreChunk / kSmallChunk == 4);
+  const uint32_t within = i & ((1u << (lv + ls)) - 1u);
+  return i - within + ((within & ((1u << lv) - 1u)) << ls) + (within >> lv);
 }
-// The maximum of a group of which the pass met a signalling NaN.
-template <int DT>
-__device__ __forceinline__ float group_max(const ScoreLaunch &a,
-                                           const typename Logits<DT>::Element *x, uint32_t group) {
-  float m = -__builtin_inff();
-  for (uint32_t e = 0; e < kScoreGroup; ++e) {
-    const uint32_t id = group * kScoreGroup + e;
-    const float v = id < a.vocabulary ? logit_value(x[id]) : m;
-    if (v > m) m = v;
-  }
-  return m;
-}
-
 // An item as one number, larger ones ahead: its key, then the lower id.
 __device__ __forceinline__ uint64_t item_of(uint32_t key, uint32_t id) {
   return (uint64_t)key << 32 | (0xffffffffu - id);
@@ -106,7 +99,6 @@ template <uint32_t U, int BITS>
 __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[U], uint32_t k) {
   static_assert(BITS % 2 == 0);
   uint32_t t = 0;
-#pragma unroll 2
   for (int b = 30; b > 30 - BITS; b -= 2) {
     uint32_t reach[3] = {};
 #pragma unroll
@@ -142,7 +134,8 @@ __device__ __forceinline__ uint32_t pick_best(TopLds &s, uint32_t k, const Each 
     uint64_t *slot = s.wave[place & 1u];
     if ((threadIdx.x & 63u) == 0) slot[threadIdx.x >> 6] = best;
     __syncthreads();
-    last = larger(larger(slot[0], slot[1]), larger(slot[2], slot[3]));
+    last = slot[0];
+    for (uint32_t w = 1; w < kTopWaves; ++w) last = larger(last, slot[w]);
     if (last == 0) return place;
     put(place, last);
   }
@@ -161,18 +154,16 @@ __device__ __forceinline__ void put_best(const ScoreLaunch &a, uint32_t row, uin
 // best groups in rounds, then their k best tokens. Returns how many there are.
 template <int DT>
 __device__ __forceinline__ uint32_t crowded_best(TopLds &s, const ScoreLaunch &a, uint32_t row,
-                                                 const typename Logits<DT>::Element *x,
-                                                 const float *maxima, const RowScore &score) {
+                                              const typename Logits<DT>::Element *x,
+                                              const float *maxima) {
+  constexpr uint32_t THREADS = kTopWaves * 64;
   const uint32_t tid = threadIdx.x;
   const uint32_t n = pick_best(
       s, a.top,
       [&](const auto &take) {
-#pragma unroll 4
-        for (uint32_t i = tid; i < a.groups; i += 256) {
+        for (uint32_t i = tid; i < a.groups; i += THREADS) {
           const uint32_t id = group_at<DT>(a, i);
-          float m = *element(maxima, i);
-          if (m != m) m = group_max<DT>(a, x, id);
-          const uint32_t key = listed_key(m);
+          const uint32_t key = listed_key(*element(maxima, i));
           take(key ? item_of(key, id) : 0ull);
         }
       },
@@ -184,7 +175,7 @@ __device__ __forceinline__ uint32_t crowded_best(TopLds &s, const ScoreLaunch &a
       s, a.top,
       [&](const auto &take) {
 #pragma unroll 4
-        for (uint32_t slot = tid >> 6; slot < n; slot += 4) {
+        for (uint32_t slot = tid >> 6; slot < n; slot += kTopWaves) {
           const uint32_t id = s.best[slot] * kScoreGroup + (tid & 63u);
           const uint32_t key =
               id < a.vocabulary ? listed_key(logit_value(*element(x, id))) : 0u;
@@ -192,41 +183,21 @@ __device__ __forceinline__ uint32_t crowded_best(TopLds &s, const ScoreLaunch &a
         }
       },
       [&](uint32_t place, uint64_t item) {
-        if (tid == 0) put_best(a, row, place, item, score);
+        if (tid == 0) put_best(a, row, place, item, s.score);
       });
 }
 
-// A row's alternatives. A unit is four lanes (U = 1: 64 units) or one thread
-// (U = 4: 256 of them). At least k groups reach the k-th of the units' best
-// maxima, and so the row's k best tokens do: each wave finds that cut for
-// itself, lists its own groups that reach it, reads their tokens, a group a
-// load, and lists those that reach it. Few others do where the best groups lie
+// The wave's own groups whose maxima reach the k-th best of the units', and of
+// their tokens those that reach it, into its lists. A unit is four lanes (U = 1:
+// 64 units) or one thread (U = 4: 256 of them). At least k groups reach that
+// cut, and so the row's k best tokens do; few others where the best groups lie
 // in different units. The cut's last bits are left out (each is half a step of
 // the search): of an f32 key the last 10, a bf16 key has 16.
 template <int DT, uint32_t N, uint32_t U>
-__device__ __forceinline__ void row_best(TopLds &s, const ScoreLaunch &a, uint32_t row,
-                                         const typename Logits<DT>::Element *x,
-                                         const float *maxima, const float (&m)[N],
-                                         const RowScore &score) {
-  static_assert(N <= kMostItems && (U == 1 || U == 4));
+__device__ __forceinline__ void list_wave(TopLds &s, const ScoreLaunch &a,
+                                          const typename Logits<DT>::Element *x,
+                                          const uint32_t (&key)[N]) {
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, k = a.top;
-  uint32_t key[N], best = 0;
-#pragma unroll
-  for (uint32_t i = 0; i < N; ++i) {
-    float v = m[i];
-    if (v != v) v = group_max<DT>(a, x, group_at<DT>(a, min(i * 256 + tid, a.groups - 1)));
-    key[i] = i * 256 + tid < a.groups ? listed_key(v) : 0u;
-    best = max(best, key[i]);
-  }
-  if constexpr (U == 1) {
-    best = max(best, xor_u32<1>(best));
-    best = max(best, xor_u32<2>(best));
-    if (tid % 4 == 0) s.unit[tid / 4] = best;
-  } else {
-    s.unit[tid] = best;
-  }
-  if (tid == 0) s.crowded = 0;
-  __syncthreads();
   uint32_t unit[U], present = 0;
 #pragma unroll
   for (uint32_t u = 0; u < U; ++u) {
@@ -241,20 +212,22 @@ __device__ __forceinline__ void row_best(TopLds &s, const ScoreLaunch &a, uint32
   for (uint32_t i = 0; i < N; ++i) {
     const bool take = key[i] >= cut;
     const uint64_t lanes = ballot(take);
+    if (!lanes) continue;
     const uint32_t at = n + mbcnt(lanes);
-    if (take && at < kWaveGroups) s.group[wave][at] = (uint16_t)group_at<DT>(a, i * 256 + tid);
+    if (take && at < kWaveGroups) s.group[wave][at] = (uint16_t)(i * 256 + tid);
     n += (uint32_t)__popcll(lanes);
   }
   __builtin_amdgcn_wave_barrier();  // the wave's own list, in order
   bool fits = n <= kWaveGroups;
   if (fits) {
     constexpr uint32_t AHEAD = 8;
+#pragma unroll 1
     for (uint32_t first = 0; first < n; first += AHEAD) {
       uint32_t id[AHEAD];
       float v[AHEAD];
 #pragma unroll
       for (uint32_t i = 0; i < AHEAD; ++i) {
-        id[i] = s.group[wave][min(first + i, n - 1)] * kScoreGroup + lane;
+        id[i] = group_at<DT>(a, s.group[wave][min(first + i, n - 1)]) * kScoreGroup + lane;
         v[i] = logit_value(*element(x, min(id[i], a.vocabulary - 1)));
       }
 #pragma unroll
@@ -274,32 +247,6 @@ __device__ __forceinline__ void row_best(TopLds &s, const ScoreLaunch &a, uint32
     s.count[wave] = tokens;
     if (!fits) s.crowded = 1;
   }
-  __syncthreads();
-  uint32_t listed = 0;
-  if (!s.crowded) {
-    // Every item's place is the number of items ahead of it.
-    const uint32_t count[4] = {s.count[0], s.count[1], s.count[2], s.count[3]};
-    listed = count[0] + count[1] + count[2] + count[3];
-    const uint32_t most = max(max(count[0], count[1]), max(count[2], count[3]));
-    for (uint32_t own = tid / 4; own < most; own += 64) {
-      const uint64_t item = own < count[tid % 4] ? s.item[tid % 4][own] : 0ull;
-      uint32_t place = 0;
-#pragma unroll
-      for (uint32_t w = 0; w < 4; ++w) {
-        for (uint32_t j = 0; j < count[w]; j += 8) {
-#pragma unroll
-          for (uint32_t e = 0; e < 8; ++e) place += s.item[w][j + e] > item ? 1u : 0u;
-        }
-      }
-      if (item && place < k) put_best(a, row, place, item, score);
-    }
-  } else {
-    listed = crowded_best<DT>(s, a, row, x, maxima, score);
-  }
-  for (uint32_t i = listed + tid; i < k; i += 256) {
-    a.out_top_ids[(uint64_t)row * k + i] = kNoToken;
-    a.out_top_logprobs[(uint64_t)row * k + i] = -__builtin_inff();
-  }
 }
 
 // ---- finish -------------------------------------------------------------------
@@ -309,7 +256,7 @@ template <int DT>
 __device__ __forceinline__ void put_tokens(const ScoreLaunch &a, uint32_t row,
                                            const typename Logits<DT>::Element *x,
                                            const RowScore &score) {
-  const uint32_t lane = threadIdx.x;
+  const uint32_t lane = threadIdx.x & 63u;
   if (lane == 0 && a.out_lse) a.out_lse[row] = score.lse();
   uint32_t ahead = 0;
   if (a.out_ranks) {
@@ -336,24 +283,79 @@ __global__ __launch_bounds__(64) void logprobs_kernel(ScoreLaunch a) {
   put_tokens<DT>(a, row, x, RowScore{total.m, inv_t, logf(total.s)});
 }
 
-// One row a block, with alternatives: up to N groups a thread.
+// One row a block, with alternatives: up to N groups a thread. The fifth wave
+// takes the row's totals and tokens while the others list.
 template <int DT, uint32_t N>
-__global__ __launch_bounds__(256) void alternatives_kernel(ScoreLaunch a) {
+__global__ __launch_bounds__(kTopWaves * 64) void alternatives_kernel(ScoreLaunch a) {
+  static_assert(N <= kMostItems);
   __shared__ TopLds s;
-  const uint32_t tid = threadIdx.x, row = blockIdx.x;
+  const uint32_t tid = threadIdx.x, row = blockIdx.x, k = a.top;
   const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
   const float *maxima = a.maxima + (uint64_t)row * a.groups;
-  float m[N];
+  uint32_t key[N];
+  if (tid < 256) {
+    float m[N];
 #pragma unroll
-  for (uint32_t i = 0; i < N; ++i) m[i] = *element(maxima, min(i * 256 + tid, a.groups - 1));
-  const float inv_t = inverse_temperature(a, row);
-  const MaxSum total = row_total(a, row, inv_t * kLog2e);
-  const RowScore score{total.m, inv_t, logf(total.s)};
-  if (a.top <= kQuadTop)
-    row_best<DT, N, 1>(s, a, row, x, maxima, m, score);
-  else
-    row_best<DT, N, 4>(s, a, row, x, maxima, m, score);
-  if (tid < 64) put_tokens<DT>(a, row, x, score);
+    for (uint32_t i = 0; i < N; ++i) m[i] = *element(maxima, min(i * 256 + tid, a.groups - 1));
+    uint32_t best = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+      key[i] = i * 256 + tid < a.groups ? listed_key(m[i]) : 0u;
+      best = max(best, key[i]);
+    }
+    if (k <= kQuadTop) {
+      best = max(best, xor_u32<1>(best));
+      best = max(best, xor_u32<2>(best));
+      if (tid % 4 == 0) s.unit[tid / 4] = best;
+    } else {
+      s.unit[tid] = best;
+    }
+  }
+  if (tid == 0) s.crowded = 0;
+  __syncthreads();
+  if (tid >= 256) {
+    const float inv_t = inverse_temperature(a, row);
+    const MaxSum total = row_total(a, row, inv_t * kLog2e);
+    const RowScore score{total.m, inv_t, logf(total.s)};
+    if (tid == 256) s.score = score;
+    put_tokens<DT>(a, row, x, score);
+  } else if (k <= kQuadTop) {
+    list_wave<DT, N, 1>(s, a, x, key);
+  } else {
+    list_wave<DT, N, 4>(s, a, x, key);
+  }
+  __syncthreads();
+  uint32_t listed;
+  if (!s.crowded) {
+    // Every item's place is the number of items ahead of it: four lanes an item,
+    // a wave's list each.
+    const uint32_t c0 = s.count[0], c1 = c0 + s.count[1], c2 = c1 + s.count[2];
+    listed = c2 + s.count[3];
+    const RowScore score = s.score;
+    const uint32_t own = s.count[tid % 4];
+    const uint64_t *list = s.item[tid % 4];
+    for (uint32_t first = 0; first < listed; first += kTopWaves * 16) {
+      const uint32_t i = first + tid / 4;
+      const uint32_t w = (i >= c0) + (i >= c1) + (i >= c2);
+      const uint32_t at = i - (w == 0 ? 0u : w == 1 ? c0 : w == 2 ? c1 : c2);
+      const uint64_t item = i < listed ? s.item[w][at] : 0ull;
+      uint32_t place = 0;
+#pragma unroll 1
+      for (uint32_t j = 0; j < own; j += 8) {
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) place += list[j + e] > item ? 1u : 0u;
+      }
+      place += xor_u32<1>(place);
+      place += xor_u32<2>(place);
+      if (item && place < k && tid % 4 == 0) put_best(a, row, place, item, score);
+    }
+  } else {
+    listed = crowded_best<DT>(s, a, row, x, maxima);
+  }
+  for (uint32_t i = listed + tid; i < k; i += kTopWaves * 64) {
+    a.out_top_ids[(uint64_t)row * k + i] = kNoToken;
+    a.out_top_logprobs[(uint64_t)row * k + i] = -__builtin_inff();
+  }
 }
 
 // ---- the pass -----------------------------------------------------------------
@@ -434,6 +436,17 @@ __global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
     // A group's 64 tokens lie in 16 (f32) or 8 (bf16) neighbouring lanes, of
     // which the j-th writes the group of vector j: a wave's store is a run.
     constexpr uint32_t LANES = kScoreGroup / VEC;
+    if (ballot(run.s != run.s)) {
+      // A NaN among them: a signalling one has taken others' places.
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) {
+        float v[VEC];
+        unpack<DT>(w[j], v);
+        part[j] = -__builtin_inff();
+#pragma unroll
+        for (uint32_t e = 0; e < VEC; ++e) part[j] = v[e] > part[j] ? v[e] : part[j];
+      }
+    }
     max_pairs(part);
     max_quads(part);
     max_eights(part);
@@ -493,11 +506,11 @@ int launch_logprobs(const ScoreLaunch &a, uint32_t dtype, void *stream) {
     if (!a.top)                                                                             \
       hipLaunchKernelGGL((logprobs_kernel<DT>), rows, dim3(64), 0, st, a);                  \
     else if (a.groups <= 10 * 256)                                                          \
-      hipLaunchKernelGGL((alternatives_kernel<DT, 10>), rows, dim3(256), 0, st, a);         \
+      hipLaunchKernelGGL((alternatives_kernel<DT, 10>), rows, dim3(kTopWaves * 64), 0, st, a);         \
     else if (a.groups <= 16 * 256)                                                          \
-      hipLaunchKernelGGL((alternatives_kernel<DT, 16>), rows, dim3(256), 0, st, a);         \
+      hipLaunchKernelGGL((alternatives_kernel<DT, 16>), rows, dim3(kTopWaves * 64), 0, st, a);         \
     else                                                                                    \
-      hipLaunchKernelGGL((alternatives_kernel<DT, kMostItems>), rows, dim3(256), 0, st, a); \
+      hipLaunchKernelGGL((alternatives_kernel<DT, kMostItems>), rows, dim3(kTopWaves * 64), 0, st, a); \
   }
   JF_FINISH(0)
   JF_FINISH(1)

@@ -286,3 +286,30 @@ def test_refusals():
             J.Scorer(vocabulary, max_rows)
         assert message in e.value.message
     s.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_signalling_nan_hides_no_other_token(dtype):
+    """A NaN that signals, in the groups of the best tokens: the lists hold the
+    other tokens all the same."""
+    import torch
+    rng = np.random.default_rng(40)
+    V = 12000
+    x = bf16(rng.normal(0, 3, (2, V)).astype(np.float32))
+    best = order(x[0])[:30]
+    t, _ = device_rows(x, dtype)
+    at = torch.from_numpy((best[:3] // 64 * 64 + (best[:3] % 64 + 1) % 64).copy()).cuda()
+    if dtype == "f32":
+        t.view(torch.int32)[0, at] = 0x7F810000
+    else:
+        t.view(torch.int16)[0, at] = 0x7F81
+    ids = torch.zeros((2, 20), dtype=torch.int32, device="cuda")
+    lps = torch.zeros((2, 20), device="cuda")
+    s = J.Scorer(V, 2)
+    s.logprobs(t, top_ids=ids, top_logprobs=lps)
+    seen = x.copy()
+    seen[0, at.cpu().numpy()] = np.nan
+    for r in range(2):
+        np.testing.assert_array_equal(ids[r].cpu().numpy(), order(seen[r])[:20])
+    assert torch.isnan(lps[0]).all() and not torch.isnan(lps[1]).any()
+    s.close()
