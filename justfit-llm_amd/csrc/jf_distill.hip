@@ -251,15 +251,15 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
   }
 }
 
-template <int DT>
+template <int DT, uint32_t N>
 __global__ __launch_bounds__(256) void distill_grad_kernel(DistillGradLaunch a) {
-  constexpr uint32_t VEC = Logits<DT>::VEC, SLAB = kSlab<DT>, LOADS = kLoads<DT>;
-  __shared__ uint32_t listed[kScoreChunk / 32];
-  __shared__ uint8_t slot[kScoreChunk];  // read at listed tokens only
+  constexpr uint32_t VEC = Logits<DT>::VEC, SLAB = kSlab<DT>, CHUNK = N * SLAB;
+  __shared__ uint32_t listed[CHUNK / 32];
+  __shared__ uint8_t slot[CHUNK];  // read at listed tokens only
   __shared__ float share[kTeacherTokens];
   const uint32_t tid = threadIdx.x;
   const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks;
-  const uint32_t base = chunk * kScoreChunk, V = a.vocabulary, K = a.teacher_count;
+  const uint32_t base = chunk * CHUNK, V = a.vocabulary, K = a.teacher_count;
   const auto *z = row_of<DT>(a.logits, (uint64_t)row * a.stride);
   auto *dz = row_of<DT>(a.grad, (uint64_t)row * a.grad_stride);
   const float *saved = a.saved + (uint64_t)row * (2 + K);
@@ -268,14 +268,14 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillGradLaunch a) 
   const float m = saved[0], weight = scale * saved[1];
   // A row with no list, or whose loss nothing follows from, is not read.
   const bool read = weight != 0.0f && scale != 0.0f;
-  LogitWords w[LOADS];
+  LogitWords w[N];
   if (read) load_chunk<DT>(z, base, V, 0, w);
-  listed[tid] = 0;
+  if (tid < CHUNK / 32) listed[tid] = 0;
   __syncthreads();
   if (tid < K && scale != 0.0f) {
     const uint32_t id = a.teacher_ids[(uint64_t)row * a.teacher_stride + tid], at = id - base;
     const float p = saved[2 + tid];
-    if (at < kScoreChunk && id < V && p >= 0.0f) {
+    if (at < CHUNK && id < V && p >= 0.0f) {
       share[tid] = scale * p;
       slot[at] = (uint8_t)tid;
       atomicOr(&listed[at >> 5], 1u << (at & 31u));
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillGradLaunch a) 
   }
   __syncthreads();
 #pragma unroll
-  for (uint32_t j = 0; j < LOADS; ++j) {
+  for (uint32_t j = 0; j < N; ++j) {
     const uint32_t at = j * SLAB + tid * VEC, token = base + at;
     if (token >= V) continue;
     float v[VEC];
@@ -344,10 +344,15 @@ int launch_distill_step(const ScoreLaunch &a, const DistillGradLaunch &g, uint32
 
 int launch_distill_grad(const DistillGradLaunch &a, uint32_t dtype, void *stream) {
   const dim3 grid(a.row_count * a.chunks), block(256);
-  if (dtype == 0)
-    hipLaunchKernelGGL((distill_grad_kernel<0>), grid, block, 0, (hipStream_t)stream, a);
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == 0 && a.vectors == 2)
+    hipLaunchKernelGGL((distill_grad_kernel<0, 2>), grid, block, 0, st, a);
+  else if (dtype == 0)
+    hipLaunchKernelGGL((distill_grad_kernel<0, 4>), grid, block, 0, st, a);
+  else if (a.vectors == 2)
+    hipLaunchKernelGGL((distill_grad_kernel<1, 2>), grid, block, 0, st, a);
   else
-    hipLaunchKernelGGL((distill_grad_kernel<1>), grid, block, 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL((distill_grad_kernel<1, 4>), grid, block, 0, st, a);
   return (int)hipGetLastError();
 }
 

@@ -1,8 +1,7 @@
 // Device access to rows of logits, f32 (DT 0) or bf16 (DT 1), for the
 // operators that read or write whole rows: 16-byte vectors at any element's
-// alignment, a chunk of 8192 tokens a block at a time. Token
-// chunk * 8192 + j * SLAB + tid * VEC + e is element e of thread tid's j-th
-// vector.
+// alignment, in chunks of N slabs of 256 vectors: element e of thread tid's j-th
+// vector is token j * SLAB + tid * VEC + e of the chunk.
 #pragma once
 
 #include "jf_device.h"
@@ -30,8 +29,6 @@ struct Logits<1> {
 };
 template <int DT>
 constexpr uint32_t kSlab = 256 * Logits<DT>::VEC;
-template <int DT>
-constexpr uint32_t kLoads = kScoreChunk / kSlab<DT>;
 
 template <int DT>
 __device__ __forceinline__ const typename Logits<DT>::Element *row_of(const void *logits,

@@ -82,8 +82,7 @@ __device__ __forceinline__ uint32_t group_at(const ScoreLaunch &a, uint32_t i) {
   // Of a chunk: 2^lv vectors of 2^ls groups.
   constexpr uint32_t ls = DT == 0 ? 4 : 5;
   static_assert(kSlab<DT> / kScoreGroup == 1u << ls);
-  const uint32_t lv = (DT == 0 ? 3u : 2u) - (a.small ? 2u : 0u);
-  static_assert(kScoreChunk / kSlab<DT> == (DT == 0 ? 8 : 4) && kScoreChunk / kSmallChunk == 4);
+  const uint32_t lv = a.vectors == 4 ? 2 : 1;
   const uint32_t within = i & ((1u << (lv + ls)) - 1u);
   return i - within + ((within & ((1u << lv) - 1u)) << ls) + (within >> lv);
 }
@@ -367,16 +366,13 @@ __global__ __launch_bounds__(kTopWaves * 64) void alternatives_kernel(ScoreLaunc
 #define JF_MAX_STEP(NAME, CTRL)                                                                 \
   template <uint32_t N>                                                                         \
   __device__ __forceinline__ void NAME(float (&g)[N]) {                                         \
-    static_assert(N == 1 || N == 2 || N == 4 || N == 8);                                        \
-    if constexpr (N == 1)                                                                       \
-      asm("s_nop 1\n" JF_MAX_DPP("%0", CTRL) : "+v"(g[0]));                                     \
-    else if constexpr (N == 2)                                                                  \
+    static_assert(N == 2 || N == 4);                                                            \
+    if constexpr (N == 2)                                                                       \
       asm("s_nop 1\n" JF_MAX_DPP("%0", CTRL) JF_MAX_DPP("%1", CTRL) : "+v"(g[0]), "+v"(g[1]));  \
     else                                                                                        \
-      for (uint32_t j = 0; j < N; j += 4)                                                       \
-        asm("s_nop 1\n" JF_MAX_DPP("%0", CTRL) JF_MAX_DPP("%1", CTRL) JF_MAX_DPP("%2", CTRL)    \
-                JF_MAX_DPP("%3", CTRL)                                                          \
-            : "+v"(g[j]), "+v"(g[j + 1]), "+v"(g[j + 2]), "+v"(g[j + 3]));                      \
+      asm("s_nop 1\n" JF_MAX_DPP("%0", CTRL) JF_MAX_DPP("%1", CTRL) JF_MAX_DPP("%2", CTRL)      \
+              JF_MAX_DPP("%3", CTRL)                                                            \
+          : "+v"(g[0]), "+v"(g[1]), "+v"(g[2]), "+v"(g[3]));                                    \
   }
 JF_MAX_STEP(max_pairs, "quad_perm:[1,0,3,2]")
 JF_MAX_STEP(max_quads, "quad_perm:[2,3,0,1]")
@@ -480,19 +476,18 @@ __global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
 int launch_score(const ScoreLaunch &a, uint32_t dtype, void *stream) {
   const dim3 grid(a.row_count * a.segments);
   const bool top = a.top != 0, rank = a.out_ranks != nullptr;
-#define JF_SCORE(DT, N, RANK, TOP)                                                       \
-  if (dtype == DT && (a.small != 0) == (N * kSlab<DT> == kSmallChunk) && rank == RANK && \
-      top == TOP)                                                                        \
+#define JF_SCORE(DT, N, RANK, TOP)                                     \
+  if (dtype == DT && a.vectors == N && rank == RANK && top == TOP)     \
   hipLaunchKernelGGL((score_kernel<DT, N, RANK, TOP>), grid, dim3(256), 0, (hipStream_t)stream, a)
 #define JF_SCORE_ALL(DT, N)      \
   JF_SCORE(DT, N, false, false); \
   JF_SCORE(DT, N, false, true);  \
   JF_SCORE(DT, N, true, false);  \
   JF_SCORE(DT, N, true, true)
-  JF_SCORE_ALL(0, kScoreChunk / kSlab<0>);
-  JF_SCORE_ALL(0, kSmallChunk / kSlab<0>);
-  JF_SCORE_ALL(1, kScoreChunk / kSlab<1>);
-  JF_SCORE_ALL(1, kSmallChunk / kSlab<1>);
+  JF_SCORE_ALL(0, 2);
+  JF_SCORE_ALL(0, 4);
+  JF_SCORE_ALL(1, 2);
+  JF_SCORE_ALL(1, 4);
 #undef JF_SCORE_ALL
 #undef JF_SCORE
   return (int)hipGetLastError();

@@ -24,13 +24,15 @@ using namespace jf::host;
 
 constexpr uint32_t kMaxVocabulary = 524288;
 constexpr uint32_t kMaxRows = 1u << 22;
-// Calls of up to this many chunks take small ones.
-constexpr uint32_t kFewChunks = 512;
-// Blocks of one launch at most: its threads stay below 2^32.
-constexpr uint32_t kMaxBlocks = 1u << 23;
+// Tokens of one launch at most: the threads of its grid stay below 2^32.
+constexpr uint64_t kMaxTokens = 1ull << 33;
 
-uint32_t chunks_of(uint32_t vocabulary) {
-  return (vocabulary + jf::kScoreChunk - 1) / jf::kScoreChunk;
+constexpr uint32_t kLeastChunk = jf::chunk_tokens(JF_DTYPE_F32, 2);
+constexpr uint32_t kMostChunk = jf::chunk_tokens(JF_DTYPE_BF16, 4);
+uint32_t blocks_of(uint32_t vocabulary, uint32_t chunk) { return (vocabulary + chunk - 1) / chunk; }
+// Rows of one launch at most.
+uint32_t launch_rows(uint32_t vocabulary) {
+  return (uint32_t)(kMaxTokens / ((uint64_t)blocks_of(vocabulary, kMostChunk) * kMostChunk));
 }
 size_t element_size(uint32_t dtype) { return dtype == JF_DTYPE_F32 ? 4 : 2; }
 
@@ -60,12 +62,11 @@ struct jf_bias_table {
 struct jf_scorer {
   uint32_t vocabulary = 0;
   uint32_t max_rows = 0;
-  uint32_t chunks = 0;
   int device = 0;
   jf::ProcessRow *rows = nullptr;  // [max_rows]
   float2 *partials = nullptr;      // a chunk each, row by row
   uint32_t *aheads = nullptr;      // likewise
-  float *maxima = nullptr;         // [min(max_rows, kTopRows)][chunks * kScoreChunkGroups]
+  float *maxima = nullptr;         // those of min(max_rows, kTopRows) rows' chunks
   float *saved = nullptr;          // [max_rows][2 + kTeacherTokens]
   uint64_t workspace_bytes = 0;
   std::vector<jf::ProcessRow> last_rows;  // what the device's rows hold
@@ -194,15 +195,13 @@ int jf_scorer_create(uint32_t vocabulary, uint32_t max_rows, jf_scorer **out) {
   if (!s) return fail(JF_ERR_NO_MEMORY, "scorer allocation failed");
   s->vocabulary = vocabulary;
   s->max_rows = max_rows;
-  s->chunks = chunks_of(vocabulary);
   int rc = JF_OK;
   const hipError_t e = hipGetDevice(&s->device);
   if (e != hipSuccess) rc = hip_fail(e, "hipGetDevice");
-  const uint64_t blocks = (uint64_t)max_rows * s->chunks;
-  const uint64_t parts =
-      std::max(blocks, std::min<uint64_t>(blocks, kFewChunks) * (jf::kScoreChunk / jf::kSmallChunk));
-  const uint64_t maxima = (uint64_t)std::min(max_rows, jf::kTopRows) * s->chunks *
-                          jf::kScoreChunkGroups;
+  // The rows' blocks and groups, whatever the chunk.
+  const uint64_t parts = (uint64_t)max_rows * blocks_of(vocabulary, kLeastChunk);
+  const uint64_t maxima = (uint64_t)std::min(max_rows, jf::kTopRows) *
+                          blocks_of(vocabulary, kMostChunk) * (kMostChunk / jf::kScoreGroup);
   const uint64_t saved = (uint64_t)max_rows * (2 + jf::kTeacherTokens);
   if (rc == JF_OK) rc = device_alloc(&s->rows, max_rows, "row records");
   if (rc == JF_OK) rc = device_alloc(&s->partials, parts, "row partials");
@@ -332,7 +331,7 @@ int jf_process_logits(jf_scorer *s, const jf_process_args *a, void *stream) {
   }
   const uint64_t stride = a->rows > 1 ? a->logits_stride : s->vocabulary;
   const uint64_t out_stride = a->rows > 1 ? a->out_stride : s->vocabulary;
-  const uint32_t most = kMaxBlocks / (s->chunks * (jf::kScoreChunk / jf::kSmallChunk));
+  const uint32_t most = launch_rows(s->vocabulary);
   const bool all_masked = std::all_of(s->host_rows.begin(), s->host_rows.end(),
                                       [](const jf::ProcessRow &p) { return p.flags != 0; });
   for (uint32_t r = 0; r < a->rows; r += most) {
@@ -370,15 +369,13 @@ int jf_process_logits(jf_scorer *s, const jf_process_args *a, void *stream) {
 
 // ---- the pass over a row -----------------------------------------------------
 
-// A row's blocks: one a chunk (several chunks a block cost 1024 rows x 151,936
-// bf16 61.5 us against 59.4, and 28 rows f32 9.4 against 9.2), small chunks
-// while there are few (one row with alternatives 11.4 us against 12.3, 64 rows
-// 24.5 against 22.3).
-static void split_rows(const jf_scorer *s, uint32_t rows, jf::ScoreLaunch *L) {
-  L->small = rows * s->chunks <= kFewChunks;
-  const uint32_t chunk = L->small ? jf::kSmallChunk : jf::kScoreChunk;
-  L->segments = (s->vocabulary + chunk - 1) / chunk;
-  L->groups = L->segments * (chunk / jf::kScoreGroup);
+// The vectors a thread takes of a row at a time, two while four would leave the
+// GPU with few blocks (20 alternatives of one f32 row x 151,936: 9.1 us against
+// 9.6, of 64 rows 17.3 against 16.2; of 8 bf16 rows 10.8 against 11.1, of 64
+// rows 14.8 against 14.5; gradients of 32 bf16 rows 4.4 against 5.2).
+static uint32_t chunk_vectors(uint32_t rows, uint32_t vocabulary, uint32_t dtype) {
+  const uint64_t tokens = (uint64_t)rows * vocabulary;
+  return tokens <= (dtype == JF_DTYPE_F32 ? 1u << 20 : 8u << 20) ? 2 : 4;
 }
 
 static jf::ScoreLaunch score_rows(const jf_scorer *s, const void *logits, uint64_t stride,
@@ -388,7 +385,10 @@ static jf::ScoreLaunch score_rows(const jf_scorer *s, const void *logits, uint64
   L.stride = stride;
   L.row_count = rows;
   L.vocabulary = s->vocabulary;
-  split_rows(s, rows, &L);
+  L.vectors = chunk_vectors(rows, s->vocabulary, dtype);
+  const uint32_t chunk = jf::chunk_tokens(dtype, L.vectors);
+  L.segments = blocks_of(s->vocabulary, chunk);
+  L.groups = L.segments * (chunk / jf::kScoreGroup);
   L.temperature = 1.0f;
   // Launches of one call follow one another on its stream: each takes the
   // scratch of the first rows again.
@@ -419,7 +419,7 @@ int jf_logprobs(jf_scorer *s, const jf_logprobs_args *a, void *stream) {
   if (!a->top && !a->token_count && !a->out_lse)
     return fail(JF_ERR_INVALID_ARGUMENT, "nothing to score");
   const uint64_t stride = a->rows > 1 ? a->logits_stride : s->vocabulary;
-  const uint32_t most = a->top ? jf::kTopRows : kMaxBlocks / s->chunks;
+  const uint32_t most = a->top ? jf::kTopRows : launch_rows(s->vocabulary);
   for (uint32_t r = 0; r < a->rows; r += most) {
     jf::ScoreLaunch L = score_rows(s, a->logits, stride, a->dtype, r, std::min(most, a->rows - r));
     L.temperatures = at(a->temperatures, r);
@@ -488,7 +488,7 @@ static int distill(jf_scorer *s, const jf_distill_args *a, bool forward, bool ba
   if (rc != JF_OK) return rc;
   const uint64_t stride = a->rows > 1 ? a->logits_stride : s->vocabulary;
   const uint64_t grad_stride = a->rows > 1 ? a->grad_stride : s->vocabulary;
-  const uint32_t most = kMaxBlocks / s->chunks, K = a->teacher_count;
+  const uint32_t most = launch_rows(s->vocabulary), K = a->teacher_count;
   for (uint32_t r = 0; r < a->rows; r += most) {
     const uint32_t n = std::min(most, a->rows - r);
     float *saved = a->saved ? a->saved + (uint64_t)r * (2 + K) : backward ? s->saved : nullptr;
@@ -513,7 +513,8 @@ static int distill(jf_scorer *s, const jf_distill_args *a, bool forward, bool ba
       G.grad_stride = grad_stride;
       G.row_count = n;
       G.vocabulary = s->vocabulary;
-      G.chunks = s->chunks;
+      G.vectors = L.vectors;
+      G.chunks = L.segments;
       G.grad_loss = a->grad_loss + r * a->grad_loss_stride;
       G.grad_loss_stride = a->grad_loss_stride;
     }

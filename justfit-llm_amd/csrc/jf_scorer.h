@@ -10,12 +10,12 @@
 
 namespace jf {
 
-// A block's tokens at a time, and the tokens whose maximum the score pass
-// keeps (a power of two that divides a chunk).
-constexpr uint32_t kScoreChunk = 8192;
-constexpr uint32_t kSmallChunk = 2048;  // for calls of few rows
+// A block's 256 threads take a chunk of a row, a few vectors of 16 bytes each.
+constexpr uint32_t chunk_tokens(uint32_t dtype, uint32_t vectors) {
+  return vectors * 256 * (dtype == 0 ? 4 : 8);
+}
+// The tokens whose maximum the pass keeps (a power of two that divides a chunk).
 constexpr uint32_t kScoreGroup = 64;
-constexpr uint32_t kScoreChunkGroups = kScoreChunk / kScoreGroup;
 constexpr uint32_t kTopLogprobs = 128;    // alternatives a row at most
 constexpr uint32_t kTeacherTokens = 256;  // a teacher's list at most: one a thread
 // Rows of one launch with alternatives: bounds the groups' scratch.
@@ -65,7 +65,7 @@ struct ScoreLaunch {
   const void *logits;
   uint64_t stride;
   uint32_t row_count, vocabulary;
-  uint32_t small;           // chunks of kSmallChunk tokens, otherwise kScoreChunk
+  uint32_t vectors;         // a thread: 2 or 4
   uint32_t segments;        // blocks a row, one a chunk
   uint32_t groups;          // groups a row, padded to whole chunks
   const float *temperatures;  // device, or NULL: `temperature` for every row
@@ -98,7 +98,9 @@ struct DistillGradLaunch {
   uint64_t stride;
   void *grad;
   uint64_t grad_stride;
-  uint32_t row_count, vocabulary, chunks;
+  uint32_t row_count, vocabulary;
+  uint32_t vectors;  // a thread: 2 or 4
+  uint32_t chunks;   // blocks a row
   float temperature;
   const uint32_t *teacher_ids;
   uint64_t teacher_stride;
