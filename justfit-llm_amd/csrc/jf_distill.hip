@@ -136,9 +136,10 @@ __global__ __launch_bounds__(64) void distill_loss_kernel(ScoreLaunch a) {
   const uint32_t row = blockIdx.x;
   const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
   const float inv_t = 1.0f / a.temperature;
+  const MaxSum part = row_part(a, row);
   Teacher<DT, SLOTS> t;
   t.load(a, row, x, inv_t, listed);
-  const MaxSum total = row_total(a, row, inv_t * kLog2e);
+  const MaxSum total = row_total(a, row, part, inv_t * kLog2e);
   t.put(a, row, total, RowScore{total.m, inv_t, logf(total.s)});
 }
 
@@ -147,12 +148,16 @@ __global__ __launch_bounds__(64) void distill_loss_kernel(ScoreLaunch a) {
 constexpr uint32_t kStepThreads = 512;
 constexpr uint32_t kStepWaves = kStepThreads / 64;
 constexpr uint32_t kQuad = 4;       // vectors a thread loads, adds and stores together
-constexpr uint32_t kHeldQuads = 3;  // of them held from the first pass to the second
+// Of them held from the first pass to the second: what the registers take
+// beside a list of SLOTS a lane.
+template <uint32_t SLOTS>
+constexpr uint32_t kHeld = SLOTS == 1 ? 3 : 2;
 
 template <int DT, uint32_t SLOTS>
 __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaunch a,
                                                                        DistillGradLaunch g) {
-  constexpr uint32_t VEC = Logits<DT>::VEC, SLAB = kStepThreads * VEC, QUAD = kQuad * SLAB;
+  constexpr uint32_t VEC = Logits<DT>::VEC, SLAB = kStepThreads * VEC, QUAD = kQuad * SLAB,
+                     HELD = kHeld<SLOTS>;
   using Words = typename Logits<DT>::Words;
   __shared__ uint32_t listed[64 * SLOTS];
   __shared__ MaxSum part[kStepWaves];
@@ -169,9 +174,9 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
       w[j] = *(const Words *)(z + quad * QUAD + j * SLAB + tid * VEC);
   };
   // `rest`: the vectors past the last whole quad.
-  LogitWords held[kHeldQuads][kQuad], rest[kQuad];
+  LogitWords held[HELD][kQuad], rest[kQuad];
 #pragma unroll
-  for (uint32_t q = 0; q < kHeldQuads; ++q)
+  for (uint32_t q = 0; q < HELD; ++q)
     if (q < quads) load(q, held[q]);
 #pragma unroll
   for (uint32_t j = 0; j < kQuad; ++j)
@@ -190,9 +195,9 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
     add_vectors<DT>(run, w, top, c);
   };
 #pragma unroll
-  for (uint32_t q = 0; q < kHeldQuads; ++q)
+  for (uint32_t q = 0; q < HELD; ++q)
     if (q < quads) add(held[q]);
-  for (uint32_t q = kHeldQuads; q < quads; ++q) {
+  for (uint32_t q = HELD; q < quads; ++q) {
     LogitWords w[kQuad];
     load(q, w);
     add(w);
@@ -204,7 +209,7 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
   // The held words anew, or the compiler keeps the values it unpacked above,
   // two registers a word.
 #pragma unroll
-  for (uint32_t q = 0; q < kHeldQuads; ++q)
+  for (uint32_t q = 0; q < HELD; ++q)
 #pragma unroll
     for (uint32_t j = 0; j < kQuad; ++j) asm volatile("" : "+v"(held[q][j]));
   MaxSum total = lane < kStepWaves ? part[lane] : MaxSum{-__builtin_inff(), 0.0f};
@@ -227,13 +232,13 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
                                   (Words *)(dz + quad * QUAD + j * SLAB + tid * VEC));
   };
   // The quads read again come first, the last read before the others.
-  for (uint32_t q = quads; q-- > kHeldQuads;) {
+  for (uint32_t q = quads; q-- > HELD;) {
     LogitWords w[kQuad];
     load(q, w);
     put(q, w);
   }
 #pragma unroll
-  for (uint32_t q = 0; q < kHeldQuads; ++q)
+  for (uint32_t q = 0; q < HELD; ++q)
     if (q < quads) put(q, held[q]);
 #pragma unroll
   for (uint32_t j = 0; j < kQuad; ++j) {
@@ -263,13 +268,18 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillGradLaunch a) 
   const auto *z = row_of<DT>(a.logits, (uint64_t)row * a.stride);
   auto *dz = row_of<DT>(a.grad, (uint64_t)row * a.grad_stride);
   const float *saved = a.saved + (uint64_t)row * (2 + K);
+  // A call of few rows asks for the chunk at once, whatever its row comes to.
+  constexpr bool EARLY = N == 2;
+  LogitWords w[N];
+  if constexpr (EARLY) load_chunk<DT>(z, base, V, 0, w);
   const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
   const float scale = a.grad_loss[(uint64_t)row * a.grad_loss_stride] * inv_t;
   const float m = saved[0], weight = scale * saved[1];
   // A row with no list, or whose loss nothing follows from, is not read.
   const bool read = weight != 0.0f && scale != 0.0f;
-  LogitWords w[N];
-  if (read) load_chunk<DT>(z, base, V, 0, w);
+  if constexpr (!EARLY) {
+    if (read) load_chunk<DT>(z, base, V, 0, w);
+  }
   if (tid < CHUNK / 32) listed[tid] = 0;
   __syncthreads();
   if (tid < K && scale != 0.0f) {

@@ -222,10 +222,18 @@ __device__ __forceinline__ void add_vectors(MaxSum &run, const LogitWords (&w)[N
   run = {grown, s};
 }
 
-// The row's maximum and sum from its blocks' (every lane of the wave).
-__device__ __forceinline__ MaxSum row_total(const ScoreLaunch &a, uint32_t row, float c) {
-  MaxSum p{-__builtin_inff(), 0.0f};
-  for (uint32_t g = threadIdx.x & 63u; g < a.segments; g += 64) {
+// A lane's first block of a row.
+__device__ __forceinline__ MaxSum row_part(const ScoreLaunch &a, uint32_t row) {
+  const uint32_t lane = threadIdx.x & 63u;
+  if (lane >= a.segments) return MaxSum{-__builtin_inff(), 0.0f};
+  const float2 v = a.partials[(uint64_t)row * a.segments + lane];
+  return MaxSum{v.x, v.y};
+}
+// The row's maximum and sum from its blocks' (every lane of the wave); `p` is
+// the lane's row_part, which may have been asked for before.
+__device__ __forceinline__ MaxSum row_total(const ScoreLaunch &a, uint32_t row, MaxSum p,
+                                            float c) {
+  for (uint32_t g = (threadIdx.x & 63u) + 64; g < a.segments; g += 64) {
     const float2 v = a.partials[(uint64_t)row * a.segments + g];
     p = join(p, MaxSum{v.x, v.y}, c);
   }

@@ -145,15 +145,10 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
   const uint32_t tid = threadIdx.x;
   const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks;
   const uint32_t base = chunk * CHUNK, V = a.vocabulary;
-  const ProcessRow p = a.rows[row];
   const auto *x = row_of<DI>(a.logits, (uint64_t)row * a.stride);
   auto *y = row_of<DO>(a.out, (uint64_t)row * a.out_stride);
-  const bool masked = (p.flags & (kProcessMasked | kProcessStops)) != 0;
-
-  // An unmasked row that is written elsewhere needs every vector: ask first.
-  const bool whole = !masked && !a.in_place;
   typename In::Words w[N];
-  if (whole) {
+  const auto load_all = [&] {
     if (base + CHUNK <= V) {
 #pragma unroll
       for (uint32_t j = 0; j < N; ++j)
@@ -162,7 +157,15 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
 #pragma unroll
       for (uint32_t j = 0; j < N; ++j) w[j] = In::load(x, base + j * SLAB + tid * VEC, V);
     }
-  }
+  };
+  // An unmasked row that is written elsewhere needs every vector: asked for
+  // before anything else, the row's record too where no row is masked.
+  const bool early = !a.any_masked && !a.in_place;
+  if (early) load_all();
+  const ProcessRow p = a.rows[row];
+  const bool masked = (p.flags & (kProcessMasked | kProcessStops)) != 0;
+  const bool whole = !masked && !a.in_place;
+  if (whole && !early) load_all();
 
   uint32_t pen0 = 0, pens = 0, bias0 = 0, biases = 0;
   const uint32_t b0 = chunk * (CHUNK / kPenaltyBucket);

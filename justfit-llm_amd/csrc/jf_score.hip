@@ -219,7 +219,7 @@ __device__ __forceinline__ void list_wave(TopLds &s, const ScoreLaunch &a,
   __builtin_amdgcn_wave_barrier();  // the wave's own list, in order
   bool fits = n <= kWaveGroups;
   if (fits) {
-    constexpr uint32_t AHEAD = 8;
+    constexpr uint32_t AHEAD = U == 1 ? 8 : 16;  // groups asked for at once
 #pragma unroll 1
     for (uint32_t first = 0; first < n; first += AHEAD) {
       uint32_t id[AHEAD];
@@ -277,8 +277,9 @@ template <int DT>
 __global__ __launch_bounds__(64) void logprobs_kernel(ScoreLaunch a) {
   const uint32_t row = blockIdx.x;
   const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
+  const MaxSum part = row_part(a, row);
   const float inv_t = inverse_temperature(a, row);
-  const MaxSum total = row_total(a, row, inv_t * kLog2e);
+  const MaxSum total = row_total(a, row, part, inv_t * kLog2e);
   put_tokens<DT>(a, row, x, RowScore{total.m, inv_t, logf(total.s)});
 }
 
@@ -314,7 +315,7 @@ __global__ __launch_bounds__(kTopWaves * 64) void alternatives_kernel(ScoreLaunc
   __syncthreads();
   if (tid >= 256) {
     const float inv_t = inverse_temperature(a, row);
-    const MaxSum total = row_total(a, row, inv_t * kLog2e);
+    const MaxSum total = row_total(a, row, row_part(a, row), inv_t * kLog2e);
     const RowScore score{total.m, inv_t, logf(total.s)};
     if (tid == 256) s.score = score;
     put_tokens<DT>(a, row, x, score);
@@ -391,6 +392,11 @@ __global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
   const uint32_t row = blockIdx.x / a.segments, segment = blockIdx.x - row * a.segments;
   const uint32_t V = a.vocabulary;
   const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
+  // The chunk first: what the row's temperature and target are is asked for
+  // while it arrives.
+  const uint32_t base = segment * CHUNK;
+  LogitWords w[N];
+  load_chunk<DT>(x, base, V, kPastMinusInfinity<DT>, w);
   const float c = inverse_temperature(a, row) * kLog2e;
   uint32_t target = 0xffffffffu;
   float at_target = 0.0f, above_target = 0.0f;
@@ -403,9 +409,6 @@ __global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
     }
   }
   MaxSum run{-__builtin_inff(), 0.0f};
-  const uint32_t base = segment * CHUNK;
-  LogitWords w[N];
-  load_chunk<DT>(x, base, V, kPastMinusInfinity<DT>, w);
   float part[N];
 #pragma unroll
   for (uint32_t j = 0; j < N; ++j) part[j] = vector_max<DT>(w[j]);

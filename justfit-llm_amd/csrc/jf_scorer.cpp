@@ -30,6 +30,9 @@ constexpr uint64_t kMaxTokens = 1ull << 33;
 constexpr uint32_t kLeastChunk = jf::chunk_tokens(JF_DTYPE_F32, 2);
 constexpr uint32_t kMostChunk = jf::chunk_tokens(JF_DTYPE_BF16, 4);
 uint32_t blocks_of(uint32_t vocabulary, uint32_t chunk) { return (vocabulary + chunk - 1) / chunk; }
+// Rows of one training step's launches at most where the scorer holds what the
+// forward pass saves.
+constexpr uint32_t kSavedRows = 65536;
 // Rows of one launch at most.
 uint32_t launch_rows(uint32_t vocabulary) {
   return (uint32_t)(kMaxTokens / ((uint64_t)blocks_of(vocabulary, kMostChunk) * kMostChunk));
@@ -67,7 +70,7 @@ struct jf_scorer {
   float2 *partials = nullptr;      // a chunk each, row by row
   uint32_t *aheads = nullptr;      // likewise
   float *maxima = nullptr;         // those of min(max_rows, kTopRows) rows' chunks
-  float *saved = nullptr;          // [max_rows][2 + kTeacherTokens]
+  float *saved = nullptr;          // [min(max_rows, kSavedRows)][2 + kTeacherTokens]
   uint64_t workspace_bytes = 0;
   std::vector<jf::ProcessRow> last_rows;  // what the device's rows hold
   std::vector<jf::ProcessRow> host_rows;  // the call's rows, reused across calls
@@ -202,7 +205,7 @@ int jf_scorer_create(uint32_t vocabulary, uint32_t max_rows, jf_scorer **out) {
   const uint64_t parts = (uint64_t)max_rows * blocks_of(vocabulary, kLeastChunk);
   const uint64_t maxima = (uint64_t)std::min(max_rows, jf::kTopRows) *
                           blocks_of(vocabulary, kMostChunk) * (kMostChunk / jf::kScoreGroup);
-  const uint64_t saved = (uint64_t)max_rows * (2 + jf::kTeacherTokens);
+  const uint64_t saved = (uint64_t)std::min(max_rows, kSavedRows) * (2 + jf::kTeacherTokens);
   if (rc == JF_OK) rc = device_alloc(&s->rows, max_rows, "row records");
   if (rc == JF_OK) rc = device_alloc(&s->partials, parts, "row partials");
   if (rc == JF_OK) rc = device_alloc(&s->aheads, parts, "rank partials");
@@ -332,8 +335,9 @@ int jf_process_logits(jf_scorer *s, const jf_process_args *a, void *stream) {
   const uint64_t stride = a->rows > 1 ? a->logits_stride : s->vocabulary;
   const uint64_t out_stride = a->rows > 1 ? a->out_stride : s->vocabulary;
   const uint32_t most = launch_rows(s->vocabulary);
-  const bool all_masked = std::all_of(s->host_rows.begin(), s->host_rows.end(),
-                                      [](const jf::ProcessRow &p) { return p.flags != 0; });
+  const auto masked = [](const jf::ProcessRow &p) { return p.flags != 0; };
+  const bool any_masked = std::any_of(s->host_rows.begin(), s->host_rows.end(), masked);
+  const bool all_masked = std::all_of(s->host_rows.begin(), s->host_rows.end(), masked);
   for (uint32_t r = 0; r < a->rows; r += most) {
     jf::ProcessLaunch L{};
     L.logits = rows_at(a->logits, r, stride, a->dtype);
@@ -344,6 +348,7 @@ int jf_process_logits(jf_scorer *s, const jf_process_args *a, void *stream) {
     L.row_count = std::min(most, a->rows - r);
     L.vocabulary = s->vocabulary;
     L.in_place = in_place ? 1u : 0u;
+    L.any_masked = any_masked ? 1u : 0u;
     L.all_masked = all_masked ? 1u : 0u;
     L.masks = a->masks;
     L.mask_stride = a->mask_stride;
@@ -488,7 +493,9 @@ static int distill(jf_scorer *s, const jf_distill_args *a, bool forward, bool ba
   if (rc != JF_OK) return rc;
   const uint64_t stride = a->rows > 1 ? a->logits_stride : s->vocabulary;
   const uint64_t grad_stride = a->rows > 1 ? a->grad_stride : s->vocabulary;
-  const uint32_t most = launch_rows(s->vocabulary), K = a->teacher_count;
+  const uint32_t K = a->teacher_count;
+  uint32_t most = launch_rows(s->vocabulary);
+  if (forward && backward && !a->saved) most = std::min(most, kSavedRows);
   for (uint32_t r = 0; r < a->rows; r += most) {
     const uint32_t n = std::min(most, a->rows - r);
     float *saved = a->saved ? a->saved + (uint64_t)r * (2 + K) : backward ? s->saved : nullptr;

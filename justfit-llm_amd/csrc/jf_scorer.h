@@ -47,7 +47,7 @@ struct ProcessLaunch {
   uint32_t row_count, vocabulary;
   uint32_t chunks;  // of a row: the launch's own
   uint32_t in_place;
-  uint32_t all_masked;
+  uint32_t any_masked, all_masked;
   const uint32_t *masks;
   uint64_t mask_stride;
   uint32_t stop0, stop1;
