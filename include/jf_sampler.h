@@ -600,7 +600,8 @@ int jf_bias_table_set(jf_bias_table *table, uint32_t row,
  * there. `out` may be the logits themselves, with the same dtype and
  * stride: then only edited and dropped tokens are written. Otherwise the two
  * share no element. Row records are uploaded when they differ from the last
- * call's (as jf_sample's); a call that repeats them may be captured. */
+ * call's (as jf_sample's). A call that repeats them may be captured into a HIP
+ * graph; its replays read the records that the scorer's last call left. */
 typedef struct jf_process_args {
   uint32_t rows;
   uint32_t dtype;

@@ -214,9 +214,10 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
     for (uint32_t j = 0; j < kQuad; ++j) asm volatile("" : "+v"(held[q][j]));
   MaxSum total = lane < kStepWaves ? part[lane] : MaxSum{-__builtin_inff(), 0.0f};
   total = wave_join(total, c);
-  const float m = total.m, weight = scale * list_weight(mass, total);
   // A row with no list, or whose loss nothing follows from, has no gradient.
-  const bool any = weight != 0.0f && scale != 0.0f;
+  const float m = total.m, listed_weight = list_weight(mass, total);
+  const float weight = scale * listed_weight;
+  const bool any = listed_weight != 0.0f && scale != 0.0f;
   const auto pulled = [&](float logit) { return any ? weight * exp_below(logit, m, c) : 0.0f; };
   const auto gradient = [&](const LogitWords &w) {
     float v[VEC];
@@ -274,11 +275,11 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillGradLaunch a) 
   if constexpr (EARLY) load_chunk<DT>(z, base, V, 0, w);
   const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
   const float scale = a.grad_loss[(uint64_t)row * a.grad_loss_stride] * inv_t;
-  const float m = saved[0], weight = scale * saved[1];
-  // A row with no list, or whose loss nothing follows from, is not read.
-  const bool read = weight != 0.0f && scale != 0.0f;
+  const float m = saved[0], listed_weight = saved[1], weight = scale * listed_weight;
+  // A row with no list, or whose loss nothing follows from, has no gradient.
+  const bool any = listed_weight != 0.0f && scale != 0.0f;
   if constexpr (!EARLY) {
-    if (read) load_chunk<DT>(z, base, V, 0, w);
+    if (any) load_chunk<DT>(z, base, V, 0, w);
   }
   if (tid < CHUNK / 32) listed[tid] = 0;
   __syncthreads();
@@ -297,7 +298,7 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillGradLaunch a) 
     const uint32_t at = j * SLAB + tid * VEC, token = base + at;
     if (token >= V) continue;
     float v[VEC];
-    if (read) {
+    if (any) {
       unpack<DT>(w[j], v);
 #pragma unroll
       for (uint32_t e = 0; e < VEC; ++e)

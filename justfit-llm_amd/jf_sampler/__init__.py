@@ -702,6 +702,10 @@ class Scorer:
         a.logits, a.logits_stride = logits.data_ptr(), logits.stride(0)
         a.out, a.out_stride = out.data_ptr(), out.stride(0)
         if masks is not None:
+            used = rows if mask_rows is None else max(mask_rows) + 1
+            if (masks.dim() != 2 or masks.element_size() != 4 or masks.stride(1) != 1
+                    or masks.shape[0] < used or masks.shape[1] * 32 < self.vocabulary):
+                raise ValueError(f"masks of shape {tuple(masks.shape)} do not cover the rows")
             a.masks = masks.data_ptr()
             a.mask_stride = masks.stride(0)
         pol = (JfPolicy * rows)(*policies)

@@ -19,6 +19,7 @@ class _DistillLoss(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
         logits, teacher_ids, teacher_values, saved = ctx.saved_tensors
         grad = torch.empty_like(logits, memory_format=torch.contiguous_format)

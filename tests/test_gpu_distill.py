@@ -327,3 +327,22 @@ def test_refusals():
         s.distill_args(t, ids.long(), values)
     assert not grad.any() and not loss.any() and not saved.any()
     s.close()
+
+
+@pytest.mark.parametrize("rows", [6, 200])
+def test_a_row_without_a_list_has_no_gradient_whatever_comes_in(rows):
+    """NaN and infinite loss gradients of rows with empty lists (few rows by
+    chunks, many by whole rows), separate passes and the step."""
+    rng = np.random.default_rng(41)
+    V = 70000
+    z = bf16(rng.normal(0, 2, (rows, V)).astype(np.float32))
+    ids = np.tile(np.uint32([5, 6]), (rows, 1))
+    ids[:3] = NO
+    g = np.ones(rows, np.float32)
+    g[0], g[1], g[4] = np.nan, np.inf, np.nan
+    for mode in ("separate", "step"):
+        got = run(z, ids, np.zeros((rows, 2), np.float32), 1.0, True, g, "bf16", mode)
+        assert not got["grad"][:3].any()
+        assert np.isnan(got["grad"][4]).all()
+        check(z[3:4], ids[3:4], np.zeros((1, 2), np.float32), 1.0, True, g[3:4], "bf16",
+              dict(grad=got["grad"][3:4]))

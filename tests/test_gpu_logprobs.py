@@ -41,7 +41,8 @@ def run(x, dtype="f32", tokens=None, temperatures=None, top=0, ranks=True, pad=0
 
 
 def near(got, want, bound, what):
-    got, want, bound = np.broadcast_arrays(np.float64(got), np.float64(want), np.float64(bound))
+    got, want, bound = np.broadcast_arrays(*(np.asarray(v, np.float64)
+                                             for v in (got, want, bound)))
     finite = np.isfinite(want)
     np.testing.assert_array_equal(got[~finite], want[~finite], err_msg=str(what))
     off = np.abs(got[finite] - want[finite])

@@ -314,6 +314,12 @@ def test_refusals():
         s.process_args(t.half(), pol, out)
     with pytest.raises(ValueError):
         s.process_args(t, pol, out, bias_rows=[0])
+    for masks, mask_rows in ((torch.zeros((2, 3), dtype=torch.int32), None),
+                             (torch.zeros((1, 4), dtype=torch.int32), None),
+                             (torch.zeros((2, 4), dtype=torch.int32), [0, 2]),
+                             (torch.zeros((2, 4), dtype=torch.int64), None)):
+        with pytest.raises(ValueError):
+            s.process_args(t, pol, out, masks=masks.cuda(), mask_rows=mask_rows)
     # Nothing above reached the output.
     assert not out.any()
     s.close()
