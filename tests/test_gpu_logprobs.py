@@ -142,6 +142,17 @@ def test_orders_that_crowd_the_best(how, top, V):
     both(x, "bf16", top=top)
 
 
+# Around the vocabularies at which a finishing thread takes 4, 8, 12 and 16 groups.
+@pytest.mark.parametrize("V", [n * 16384 + d for n in (4, 8, 12, 16) for d in (0, 1)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_groups_a_thread_takes(V, dtype):
+    rng = np.random.default_rng(V)
+    x = rng.normal(0, 3, (2, V)).astype(np.float32)
+    x[0, V - 1], x[1, V - 70] = 40.0, 40.0
+    for top in (3, 40, 128):
+        both(x, dtype, top=top)
+
+
 def test_the_largest_vocabulary():
     rng = np.random.default_rng(9)
     V = 524288
