@@ -651,12 +651,20 @@ def _dtype(t, what):
     raise ValueError(f"{what} are f32 or bf16, not {t.dtype}")
 
 
+def _device(t, what):
+    """The address of a tensor in device memory."""
+    if not t.is_cuda:
+        raise ValueError(f"{what} are on {t.device}, not on the GPU")
+    return t.data_ptr()
+
+
 def _rows(t, vocabulary, rows, what):
-    """Checks a [rows, vocabulary] tensor of contiguous rows."""
+    """The address of a [rows, vocabulary] tensor of contiguous rows."""
     if t.dim() != 2 or t.shape[1] != vocabulary or (rows is not None and t.shape[0] != rows):
         raise ValueError(f"{what} have shape {tuple(t.shape)}")
     if vocabulary > 1 and t.stride(1) != 1:
         raise ValueError(f"{what} have no contiguous rows")
+    return _device(t, what)
 
 
 def _plain(t, shape, what, floating):
@@ -668,7 +676,7 @@ def _plain(t, shape, what, floating):
         raise ValueError(f"{what} is no contiguous tensor of shape {shape}")
     if t.dtype not in ((torch.float32,) if floating else (torch.int32, torch.uint32)):
         raise ValueError(f"{what} holds {t.dtype}")
-    return t.data_ptr()
+    return _device(t, what)
 
 
 class Scorer:
@@ -694,19 +702,19 @@ class Scorer:
         """Builds a JfProcessArgs (kept-alive host arrays ride along). bias_rows:
         the bias table's row of each row, None for a row without biases."""
         rows = logits.shape[0]
-        _rows(logits, self.vocabulary, None, "logits")
-        _rows(out, self.vocabulary, rows, "processed logits")
         a = JfProcessArgs()
         a.rows = rows
         a.dtype, a.out_dtype = _dtype(logits, "logits"), _dtype(out, "processed logits")
-        a.logits, a.logits_stride = logits.data_ptr(), logits.stride(0)
-        a.out, a.out_stride = out.data_ptr(), out.stride(0)
+        a.logits, a.logits_stride = _rows(logits, self.vocabulary, None, "logits"), logits.stride(0)
+        a.out = _rows(out, self.vocabulary, rows, "processed logits")
+        a.out_stride = out.stride(0)
         if masks is not None:
             used = rows if mask_rows is None else max(mask_rows) + 1
             if (masks.dim() != 2 or masks.element_size() != 4 or masks.stride(1) != 1
-                    or masks.shape[0] < used or masks.shape[1] * 32 < self.vocabulary):
+                    or masks.shape[0] < used or masks.shape[1] * 32 < self.vocabulary
+                    or (mask_rows is not None and min(mask_rows) < 0)):
                 raise ValueError(f"masks of shape {tuple(masks.shape)} do not cover the rows")
-            a.masks = masks.data_ptr()
+            a.masks = _device(masks, "masks")
             a.mask_stride = masks.stride(0)
         pol = (JfPolicy * rows)(*policies)
         a.policies = pol
@@ -715,7 +723,7 @@ class Scorer:
         if penalties is not None:
             a.penalties = penalties.handle
         if extra_tokens is not None:
-            a.extra_tokens = extra_tokens.data_ptr()
+            a.extra_tokens = _device(extra_tokens, "extra tokens")
             a.extra_stride = extra_stride
         if biases is not None:
             a.biases = biases.handle
@@ -748,10 +756,9 @@ class Scorer:
         logprobs [rows, n], lse, ranks and temperatures [rows], top_ids and
         top_logprobs [rows, k]."""
         rows = logits.shape[0]
-        _rows(logits, self.vocabulary, None, "logits")
         a = JfLogprobsArgs()
         a.rows, a.dtype = rows, _dtype(logits, "logits")
-        a.logits, a.logits_stride = logits.data_ptr(), logits.stride(0)
+        a.logits, a.logits_stride = _rows(logits, self.vocabulary, None, "logits"), logits.stride(0)
         a.temperatures = _plain(temperatures, (rows,), "temperatures", True)
         if tokens is not None:
             a.token_count = tokens.shape[1]
@@ -780,10 +787,9 @@ class Scorer:
         loss and lse [rows], saved [rows, 2 + k], grad_loss [rows] (also
         expanded from one value), grad as the logits."""
         rows, k = teacher_ids.shape
-        _rows(logits, self.vocabulary, rows, "logits")
         a = JfDistillArgs()
         a.rows, a.dtype = rows, _dtype(logits, "logits")
-        a.logits, a.logits_stride = logits.data_ptr(), logits.stride(0)
+        a.logits, a.logits_stride = _rows(logits, self.vocabulary, rows, "logits"), logits.stride(0)
         a.temperature, a.normalize = temperature, 1 if normalize else 0
         a.teacher_ids = _plain(teacher_ids, (rows, k), "teacher_ids", False)
         a.teacher_values = _plain(teacher_values, (rows, k), "teacher_values", True)
@@ -795,12 +801,12 @@ class Scorer:
             import torch
             if tuple(grad_loss.shape) != (rows,) or grad_loss.dtype != torch.float32:
                 raise ValueError(f"grad_loss is no f32 tensor of {rows} rows")
-            a.grad_loss, a.grad_loss_stride = grad_loss.data_ptr(), grad_loss.stride(0)
+            a.grad_loss = _device(grad_loss, "loss gradients")
+            a.grad_loss_stride = grad_loss.stride(0)
         if grad is not None:
-            _rows(grad, self.vocabulary, rows, "gradients")
             if grad.dtype != logits.dtype:
                 raise ValueError("gradients have the logits' dtype")
-            a.grad, a.grad_stride = grad.data_ptr(), grad.stride(0)
+            a.grad, a.grad_stride = _rows(grad, self.vocabulary, rows, "gradients"), grad.stride(0)
         return a
 
     def launch_distill(self, a, stream=None):

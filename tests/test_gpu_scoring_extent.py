@@ -121,3 +121,31 @@ def test_largest_vocabulary(rows, dtype):
         got = host(grad[r:r + 1])[0]
         assert np.all(excess(got, want, bound + 4 * U * np.abs(want) + 1e-37, dtype) <= 1)
     s.close()
+
+
+def test_host_tensors_are_refused():
+    """A host address would fault the device: every tensor is asked for."""
+    import torch
+    V, rows = 64, 2
+    t = torch.zeros((rows, V), device="cuda")
+    ids, values = (torch.zeros((rows, 3), dtype=d, device="cuda")
+                   for d in (torch.int32, torch.float32))
+    each = torch.zeros(rows, device="cuda")
+    masks = torch.zeros((rows, 2), dtype=torch.int32, device="cuda")
+    s = J.Scorer(V, rows)
+    pol = [J.policy()] * rows
+    process = dict(logits=t, policies=pol, out=t, masks=masks, extra_tokens=masks)
+    logprobs = dict(logits=t, tokens=ids, temperatures=each, lse=each, logprobs=values,
+                    ranks=masks[:, 0].contiguous(), top_ids=ids, top_logprobs=values)
+    distill = dict(logits=t, teacher_ids=ids, teacher_values=values, loss=each, lse=each,
+                   saved=torch.zeros((rows, 5), device="cuda"), grad_loss=each, grad=t)
+    for build, kw in ((s.process_args, process), (s.logprobs_args, logprobs),
+                      (s.distill_args, distill)):
+        build(**kw)
+        for name, value in kw.items():
+            if torch.is_tensor(value):
+                with pytest.raises(ValueError, match="not on the GPU"):
+                    build(**dict(kw, **{name: value.cpu()}))
+    with pytest.raises(ValueError):
+        s.process_args(**dict(process, mask_rows=[0, -1]))
+    s.close()
