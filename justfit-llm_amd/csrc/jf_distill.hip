@@ -269,18 +269,13 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillGradLaunch a) 
   const auto *z = row_of<DT>(a.logits, (uint64_t)row * a.stride);
   auto *dz = row_of<DT>(a.grad, (uint64_t)row * a.grad_stride);
   const float *saved = a.saved + (uint64_t)row * (2 + K);
-  // A call of few rows asks for the chunk at once, whatever its row comes to.
-  constexpr bool EARLY = N == 2;
-  LogitWords w[N];
-  if constexpr (EARLY) load_chunk<DT>(z, base, V, 0, w);
   const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
   const float scale = a.grad_loss[(uint64_t)row * a.grad_loss_stride] * inv_t;
   const float m = saved[0], listed_weight = saved[1], weight = scale * listed_weight;
   // A row with no list, or whose loss nothing follows from, has no gradient.
   const bool any = listed_weight != 0.0f && scale != 0.0f;
-  if constexpr (!EARLY) {
-    if (any) load_chunk<DT>(z, base, V, 0, w);
-  }
+  LogitWords w[N];
+  if (any) load_chunk<DT>(z, base, V, 0, w);
   if (tid < CHUNK / 32) listed[tid] = 0;
   __syncthreads();
   if (tid < K && scale != 0.0f) {

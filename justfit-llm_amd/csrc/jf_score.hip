@@ -67,7 +67,9 @@ constexpr uint32_t kWaveGroups = 128;  // groups a wave lists at most
 constexpr uint32_t kWaveItems = 512;
 // Lists of up to this many alternatives are cut by the best groups of 64 quads
 // of lanes, longer ones by those of the 256 threads: a cut by fewer units is
-// quicker to find and lists more groups.
+// quicker to find and lists more groups (64 rows x 151,936 in f32: 5 alternatives
+// 15.2 us by quads, 16.8 by threads; 20 16.3 and 16.8; 33 17.7 and 18.2; 48 20.9
+// and 19.0).
 constexpr uint32_t kQuadTop = 32;
 
 struct TopLds {
@@ -117,34 +119,124 @@ __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[U], uint32_t
   return t;
 }
 
-// The block's `k` best items one by one to put(place, item) of every thread; 0
-// is no item. each(take) gives a thread's items to take(item). Returns how many
-// there are. Any order of items takes k rounds: for those that crowd the lists.
-template <class Each, class Put>
-__device__ __forceinline__ uint32_t pick_best(TopLds &s, uint32_t k, const Each &each,
-                                              const Put &put) {
-  uint64_t last = ~0ull;
-  const auto larger = [](uint64_t p, uint64_t q) { return p > q ? p : q; };
-  for (uint32_t place = 0; place < k; ++place) {
-    uint64_t best = 0;
-    each([&](uint64_t item) {
-      if (item < last && item > best) best = item;
-    });
-    best = larger(best, xor_u64<1>(best));
-    best = larger(best, xor_u64<2>(best));
-    best = larger(best, xor_u64<4>(best));
-    best = larger(best, xor_u64<8>(best));
-    best = larger(best, xor_u64<16>(best));
-    best = larger(best, xor_u64<32>(best));
-    uint64_t *slot = s.wave[place & 1u];
-    if ((threadIdx.x & 63u) == 0) slot[threadIdx.x >> 6] = best;
-    __syncthreads();
-    last = slot[0];
-    for (uint32_t w = 1; w < kTopWaves; ++w) last = larger(last, slot[w]);
-    if (last == 0) return place;
-    put(place, last);
+// A search for the k-th largest of some values, two bits a step from bits b and
+// b + 1 down: t is the largest prefix so far that k of them reach.
+struct Search {
+  uint32_t t;
+  int b;
+  // After a step's counts of the values that reach t with 1, 2 and 3 in its bits.
+  __device__ __forceinline__ void take(uint32_t one, uint32_t two, uint32_t three, uint32_t k) {
+    t |= (three >= k ? 3u : two >= k ? 2u : one >= k ? 1u : 0u) << b;
+    b -= 2;
   }
-  return k;
+};
+// The search among at least k values from `least` to `most`: the bits that they
+// share are no steps.
+__device__ __forceinline__ Search search_between(uint32_t least, uint32_t most) {
+  if (least == most) return {most, -2};
+  const int b = (31 - __builtin_clz(least ^ most)) & ~1;
+  return {b == 30 ? 0u : most >> (b + 2) << (b + 2), b};
+}
+// A lane's part of a step's counts: those of 1 and, shifted by 16, of 2; of 3.
+// (For many values a lane; for few, counting a ballot's bits each is quicker.)
+template <uint32_t M>
+__device__ __forceinline__ void count_reach(const uint32_t (&v)[M], const Search &f,
+                                            uint32_t &low, uint32_t &high) {
+  uint32_t reach[3] = {};
+#pragma unroll
+  for (uint32_t m = 0; m < M; ++m) {
+#pragma unroll
+    for (uint32_t q = 0; q < 3; ++q) reach[q] += v[m] >= (f.t | (q + 1) << f.b) ? 1u : 0u;
+  }
+  low = reach[0] | reach[1] << 16;
+  high = reach[2];
+}
+// A lane's least value but 0, and its largest.
+template <uint32_t M>
+__device__ __forceinline__ void extent(const uint32_t (&v)[M], uint32_t &least, uint32_t &most) {
+  least = 0xffffffffu;
+  most = 0;
+#pragma unroll
+  for (uint32_t m = 0; m < M; ++m) {
+    least = v[m] && v[m] < least ? v[m] : least;
+    most = max(most, v[m]);
+  }
+}
+
+// The search through the whole block's values, to their last bit.
+template <uint32_t M>
+__device__ __forceinline__ uint32_t block_kth_largest(TopLds &s, const uint32_t (&v)[M],
+                                                      Search f, uint32_t k, uint32_t &phase) {
+  static_assert(kTopWaves * 64 * M < 1u << 16);
+#pragma unroll 1
+  while (f.b >= 0) {
+    uint32_t low, high;
+    count_reach(v, f, low, high);
+    low = wave_sum_u32(low);
+    high = wave_sum_u32(high);
+    // Two rows of counts in turn: a step's are read before the next but one's.
+    uint64_t *counts = s.wave[phase];
+    phase ^= 1u;
+    if ((threadIdx.x & 63u) == 0) counts[threadIdx.x >> 6] = low | (uint64_t)high << 32;
+    __syncthreads();
+    uint64_t all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kTopWaves; ++w) all += counts[w];
+    f.take((uint32_t)all & 0xffffu, (uint32_t)all >> 16, (uint32_t)(all >> 32), k);
+  }
+  return f.t;
+}
+// The k-th largest of the block's keys; 0 if fewer of them are not 0.
+template <uint32_t M>
+__device__ __forceinline__ uint32_t block_kth_key(TopLds &s, const uint32_t (&key)[M], uint32_t k,
+                                                  uint32_t &phase) {
+  uint32_t least, most, keys = 0;
+  extent(key, least, most);
+#pragma unroll
+  for (uint32_t m = 0; m < M; ++m) keys += key[m] ? 1u : 0u;
+  least = wave_min_u32(least);
+  most = wave_max_u32(most);
+  keys = wave_sum_u32(keys);
+  uint32_t(*waves)[kTopWaves] = (uint32_t(*)[kTopWaves])s.unit;  // no longer read
+  if ((threadIdx.x & 63u) == 0) {
+    const uint32_t w = threadIdx.x >> 6;
+    waves[0][w] = least;
+    waves[1][w] = most;
+    waves[2][w] = keys;
+  }
+  __syncthreads();
+  keys = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < kTopWaves; ++w) {
+    least = min(least, waves[0][w]);
+    most = max(most, waves[1][w]);
+    keys += waves[2][w];
+  }
+  return keys < k ? 0u : block_kth_largest(s, key, search_between(least, most), k, phase);
+}
+
+// The block's `k` best of M keys a thread, each with an id (0 is no
+// key), to put(place, key, id) of their threads, in no order; returns how many.
+// Whatever the ties: the k-th key, then the k-th of the ids that have it.
+template <uint32_t M, int ID_BITS, class Id, class Put>
+__device__ __forceinline__ uint32_t pick_best(TopLds &s, const uint32_t (&key)[M], uint32_t k,
+                                              uint32_t &phase, const Id &id_of, const Put &put) {
+  constexpr uint32_t AHEAD = (1u << ID_BITS) - 1u;  // above every id's number
+  if (threadIdx.x == 0) s.count[0] = 0;
+  const uint32_t t = block_kth_key(s, key, k, phase);
+  uint32_t number[M];
+#pragma unroll
+  for (uint32_t m = 0; m < M; ++m)
+    number[m] = key[m] > t ? AHEAD : key[m] == t && t ? AHEAD - 1u - id_of(m) : 0u;
+  const uint32_t cut =
+      max(block_kth_largest(s, number, Search{0u, ID_BITS - 2}, k, phase), 1u);
+#pragma unroll
+  for (uint32_t m = 0; m < M; ++m)
+    if (number[m] >= cut) put(atomicAdd(&s.count[0], 1u), key[m], id_of(m));
+  __syncthreads();
+  const uint32_t n = s.count[0];
+  __syncthreads();
+  return n;
 }
 
 // One alternative of a row at its place.
@@ -155,41 +247,54 @@ __device__ __forceinline__ void put_best(const ScoreLaunch &a, uint32_t row, uin
   a.out_top_logprobs[at] = score.logprob(key_logit((uint32_t)(item >> 32)));
 }
 
-// The alternatives of a row whose best groups or tokens crowd the lists: its k
-// best groups in rounds, then their k best tokens. Returns how many there are.
-template <int DT>
+// The alternatives of a row whose best groups or tokens crowd the lists (many
+// equal maxima, as of a constant row, one masked by a lowest value down to fewer
+// than k tokens, or one that falls from its first token on): its k best groups,
+// then their k best tokens. Returns how many there are. 64 rows x 151,936 in
+// f32, constant: 20 alternatives 32 us, 128 of them 35, and masked by the lowest
+// value 57 and 62 (in random order 14 and 24; in k rounds of a maximum each 67
+// and 975).
+template <int DT, uint32_t N>
 __device__ __forceinline__ uint32_t crowded_best(TopLds &s, const ScoreLaunch &a, uint32_t row,
                                               const typename Logits<DT>::Element *x,
                                               const float *maxima) {
-  constexpr uint32_t THREADS = kTopWaves * 64;
-  const uint32_t tid = threadIdx.x;
-  const uint32_t n = pick_best(
-      s, a.top,
-      [&](const auto &take) {
-        for (uint32_t i = tid; i < a.groups; i += THREADS) {
-          const uint32_t id = group_at<DT>(a, i);
-          const uint32_t key = listed_key(*element(maxima, i));
-          take(key ? item_of(key, id) : 0ull);
-        }
-      },
-      [&](uint32_t place, uint64_t item) {
-        if (tid == 0) s.best[place] = item_id(item);
-      });
-  __syncthreads();
-  return pick_best(
-      s, a.top,
-      [&](const auto &take) {
-#pragma unroll 4
-        for (uint32_t slot = tid >> 6; slot < n; slot += kTopWaves) {
-          const uint32_t id = s.best[slot] * kScoreGroup + (tid & 63u);
-          const uint32_t key =
-              id < a.vocabulary ? listed_key(logit_value(*element(x, id))) : 0u;
-          take(key ? item_of(key, id) : 0ull);
-        }
-      },
-      [&](uint32_t place, uint64_t item) {
-        if (tid == 0) put_best(a, row, place, item, s.score);
-      });
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  uint32_t phase = 0, n;
+  {
+    uint32_t key[N];
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+      const uint32_t at = i * 256 + tid;
+      key[i] = tid < 256 && at < a.groups ? listed_key(*element(maxima, at)) : 0u;
+    }
+    n = pick_best<N, 14>(
+        s, key, a.top, phase, [&](uint32_t i) { return group_at<DT>(a, i * 256 + tid); },
+        [&](uint32_t place, uint32_t, uint32_t id) { s.best[place] = id; });
+  }
+  if (n == 0) return 0;
+  constexpr uint32_t EACH = (kTopLogprobs + kTopWaves - 1) / kTopWaves;  // groups a wave
+  uint32_t key[EACH];
+  const auto id_of = [&](uint32_t i) {
+    return s.best[min(i * kTopWaves + wave, n - 1)] * kScoreGroup + lane;
+  };
+  float v[EACH];
+#pragma unroll
+  for (uint32_t i = 0; i < EACH; ++i)
+    v[i] = logit_value(*element(x, min(id_of(i), a.vocabulary - 1)));
+#pragma unroll
+  for (uint32_t i = 0; i < EACH; ++i)
+    key[i] = i * kTopWaves + wave < n && id_of(i) < a.vocabulary ? listed_key(v[i]) : 0u;
+  uint64_t *items = s.item[0];
+  const uint32_t listed = pick_best<EACH, 20>(
+      s, key, a.top, phase, id_of,
+      [&](uint32_t place, uint32_t key, uint32_t id) { items[place] = item_of(key, id); });
+  if (tid < listed) {
+    const uint64_t item = items[tid];
+    uint32_t place = 0;
+    for (uint32_t i = 0; i < listed; ++i) place += items[i] > item ? 1u : 0u;
+    put_best(a, row, place, item, s.score);
+  }
+  return listed;
 }
 
 // The wave's own groups whose maxima reach the k-th best of the units', and of
@@ -356,7 +461,7 @@ __global__ __launch_bounds__(kTopWaves * 64) void alternatives_kernel(ScoreLaunc
       if (item && place < k && tid % 4 == 0) put_best(a, row, place, item, score);
     }
   } else {
-    listed = crowded_best<DT>(s, a, row, x, maxima);
+    listed = crowded_best<DT, N>(s, a, row, x, maxima);
   }
   for (uint32_t i = listed + tid; i < k; i += kTopWaves * 64) {
     a.out_top_ids[(uint64_t)row * k + i] = kNoToken;

@@ -142,6 +142,21 @@ def test_orders_that_crowd_the_best(how, top, V):
     both(x, "bf16", top=top)
 
 
+# Masks of the lowest value that leave fewer tokens than are listed, as many and more.
+@pytest.mark.parametrize("V", [300, 30000, 151936])
+@pytest.mark.parametrize("top", [20, 128])
+def test_rows_masked_by_the_lowest_value(V, top):
+    rng = np.random.default_rng(V)
+    x = rng.normal(0, 3, (6, V)).astype(np.float32)
+    for r, left in enumerate((0, 1, 5, top - 1, top, top + 1)):
+        keep = rng.choice(V, left, replace=False)
+        row = np.full(V, -3.3895314e38, np.float32)  # the lowest bf16
+        row[keep] = x[r, keep]
+        x[r] = row
+    both(x, "f32", top=top)
+    both(x, "bf16", top=top)
+
+
 # Around the vocabularies at which a finishing thread takes 4, 8, 12 and 16 groups.
 @pytest.mark.parametrize("V", [n * 16384 + d for n in (4, 8, 12, 16) for d in (0, 1)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
