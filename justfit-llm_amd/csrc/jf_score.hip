@@ -49,6 +49,9 @@ __device__ __forceinline__ uint32_t listed_key(float x) {
   return x > -__builtin_inff() ? logit_key(x) : 0u;
 }
 
+// That of the least finite logit.
+constexpr uint32_t kLeastKey = 0x00800000u;
+
 // ---- the best tokens ----------------------------------------------------------
 
 // Element i of a row at a uniform address, by a 32-bit offset (a row's bytes
@@ -58,27 +61,29 @@ __device__ __forceinline__ const T *element(const T *row, uint32_t i) {
   return (const T *)((const char *)row + (uint32_t)(i * sizeof(T)));
 }
 
-// A row's block: four waves for its alternatives, one for its totals.
-constexpr uint32_t kTopWaves = 5;
-constexpr uint32_t kMostItems = 32;  // groups a thread holds at most
+// A row's block: eight waves list its alternatives, one takes its totals.
+constexpr uint32_t kListWaves = 8;
+constexpr uint32_t kListThreads = kListWaves * 64;
+constexpr uint32_t kTopWaves = kListWaves + 1;
+constexpr uint32_t kMostItems = 16;  // groups a thread holds at most
 constexpr uint32_t kWaveGroups = 128;  // groups a wave lists at most
 // Tokens a wave lists at most. A row whose best tokens are neighbours lists most
 // of their groups' tokens: ids in the order of their frequency come to hundreds.
 constexpr uint32_t kWaveItems = 512;
-// Lists of up to this many alternatives are cut by the best groups of 64 quads
-// of lanes, longer ones by those of the 256 threads: a cut by fewer units is
+// Lists of up to this many alternatives are cut by the best groups of 64 units of
+// eight lanes, longer ones by those of 256 pairs: a cut by fewer units is
 // quicker to find and lists more groups (64 rows x 151,936 in f32: 5 alternatives
 // 15.2 us by quads, 16.8 by threads; 20 16.3 and 16.8; 33 17.7 and 18.2; 48 20.9
 // and 19.0).
-constexpr uint32_t kQuadTop = 32;
+constexpr uint32_t kShortTop = 32;
 
 struct TopLds {
-  uint64_t item[4][kWaveItems + 8];  // each wave's tokens, then 0 up to a multiple of 8
+  uint64_t item[kListWaves][kWaveItems + 8];  // each wave's tokens, then 0 up to a multiple of 8
   uint32_t unit[256];                // the units' best keys
-  uint16_t group[4][kWaveGroups];
+  uint16_t group[kListWaves][kWaveGroups];
   uint32_t best[kTopLogprobs];
   uint64_t wave[2][kTopWaves];
-  uint32_t count[4];
+  uint32_t count[kListWaves];
   uint32_t crowded;
   RowScore score;
 };
@@ -264,11 +269,11 @@ __device__ __forceinline__ uint32_t crowded_best(TopLds &s, const ScoreLaunch &a
     uint32_t key[N];
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i) {
-      const uint32_t at = i * 256 + tid;
-      key[i] = tid < 256 && at < a.groups ? listed_key(*element(maxima, at)) : 0u;
+      const uint32_t at = i * kListThreads + tid;
+      key[i] = tid < kListThreads && at < a.groups ? listed_key(*element(maxima, at)) : 0u;
     }
     n = pick_best<N, 14>(
-        s, key, a.top, phase, [&](uint32_t i) { return group_at<DT>(a, i * 256 + tid); },
+        s, key, a.top, phase, [&](uint32_t i) { return group_at<DT>(a, i * kListThreads + tid); },
         [&](uint32_t place, uint32_t, uint32_t id) { s.best[place] = id; });
   }
   if (n == 0) return 0;
@@ -298,8 +303,8 @@ __device__ __forceinline__ uint32_t crowded_best(TopLds &s, const ScoreLaunch &a
 }
 
 // The wave's own groups whose maxima reach the k-th best of the units', and of
-// their tokens those that reach it, into its lists. A unit is four lanes (U = 1:
-// 64 units) or one thread (U = 4: 256 of them). At least k groups reach that
+// their tokens those that reach it, into its lists. A unit is eight lanes (U = 1:
+// 64 units) or two (U = 4: 256 of them). At least k groups reach that
 // cut, and so the row's k best tokens do; few others where the best groups lie
 // in different units. The cut's last bits are left out (each is half a step of
 // the search): of an f32 key the last 10, a bf16 key has 16.
@@ -324,29 +329,32 @@ __device__ __forceinline__ void list_wave(TopLds &s, const ScoreLaunch &a,
     const uint64_t lanes = ballot(take);
     if (!lanes) continue;
     const uint32_t at = n + mbcnt(lanes);
-    if (take && at < kWaveGroups) s.group[wave][at] = (uint16_t)(i * 256 + tid);
+    if (take && at < kWaveGroups) s.group[wave][at] = (uint16_t)(i * kListThreads + tid);
     n += (uint32_t)__popcll(lanes);
   }
   __builtin_amdgcn_wave_barrier();  // the wave's own list, in order
   bool fits = n <= kWaveGroups;
   if (fits) {
-    constexpr uint32_t AHEAD = U == 1 ? 8 : 16;  // groups asked for at once
+    constexpr uint32_t AHEAD = 8;  // groups asked for at once
+    const float least = key_logit(max(cut, kLeastKey));
 #pragma unroll 1
     for (uint32_t first = 0; first < n; first += AHEAD) {
-      uint32_t id[AHEAD];
+      // A lane's group is a load's for all.
+      const uint32_t mine = group_at<DT>(a, s.group[wave][min(first + lane % AHEAD, n - 1)]);
       float v[AHEAD];
 #pragma unroll
       for (uint32_t i = 0; i < AHEAD; ++i) {
-        id[i] = group_at<DT>(a, s.group[wave][min(first + i, n - 1)]) * kScoreGroup + lane;
-        v[i] = logit_value(*element(x, min(id[i], a.vocabulary - 1)));
+        const uint32_t base = __builtin_amdgcn_readlane(mine, i) * kScoreGroup;
+        v[i] = logit_value(*element(x + base, min(lane, a.vocabulary - 1 - base)));
       }
 #pragma unroll
       for (uint32_t i = 0; i < AHEAD; ++i) {
-        const uint32_t item = listed_key(v[i]);
-        const bool take = first + i < n && id[i] < a.vocabulary && item >= cut;
+        if (first + i >= n) break;
+        const uint32_t base = __builtin_amdgcn_readlane(mine, i) * kScoreGroup;
+        const bool take = v[i] >= least && lane < a.vocabulary - base;
         const uint64_t lanes = ballot(take);
         const uint32_t at = tokens + mbcnt(lanes);
-        if (take && at < kWaveItems) s.item[wave][at] = item_of(item, id[i]);
+        if (take && at < kWaveItems) s.item[wave][at] = item_of(logit_key(v[i]), base + lane);
         tokens += (uint32_t)__popcll(lanes);
       }
     }
@@ -359,42 +367,106 @@ __device__ __forceinline__ void list_wave(TopLds &s, const ScoreLaunch &a,
   }
 }
 
-// ---- finish -------------------------------------------------------------------
-
-// A row's totals and its tokens' log-probabilities by one wave.
-template <int DT>
-__device__ __forceinline__ void put_tokens(const ScoreLaunch &a, uint32_t row,
-                                           const typename Logits<DT>::Element *x,
-                                           const RowScore &score) {
-  const uint32_t lane = threadIdx.x & 63u;
-  if (lane == 0 && a.out_lse) a.out_lse[row] = score.lse();
-  uint32_t ahead = 0;
-  if (a.out_ranks) {
-    for (uint32_t g = lane; g < a.segments; g += 64)
-      ahead += a.aheads[(uint64_t)row * a.segments + g];
-    ahead = wave_sum_u32(ahead);
-  }
-  for (uint32_t i = lane; i < a.token_count; i += 64) {
-    const uint32_t token = a.tokens[(uint64_t)row * a.token_stride + i];
-    const bool known = token < a.vocabulary;
-    a.out_logprobs[(uint64_t)row * a.token_count + i] =
-        known ? score.logprob(logit_value(x[token])) : -__builtin_inff();
-    if (i == 0 && a.out_ranks) a.out_ranks[row] = known ? ahead + 1u : 0u;
+// Every item's place is the number of items ahead of it: eight lanes take R items
+// at a time, a wave's list each.
+template <uint32_t R>
+__device__ __forceinline__ void place_items(const TopLds &s, const ScoreLaunch &a, uint32_t row,
+                                            uint32_t listed) {
+  constexpr uint32_t STEP = kTopWaves * 64 / kListWaves;
+  const uint32_t tid = threadIdx.x, own = s.count[tid % kListWaves];
+  const uint64_t *list = s.item[tid % kListWaves];
+  const RowScore score = s.score;
+  for (uint32_t first = 0; first < listed; first += R * STEP) {
+    uint64_t item[R];
+    uint32_t place[R] = {};
+#pragma unroll
+    for (uint32_t r = 0; r < R; ++r) {
+      const uint32_t i = first + r * STEP + tid / kListWaves;
+      uint32_t w = 0, at = i;
+#pragma unroll
+      for (uint32_t j = 0; j + 1 < kListWaves; ++j) {
+        const uint32_t n = s.count[j];
+        const bool past = w == j && at >= n;
+        at -= past ? n : 0u;
+        w += past ? 1u : 0u;
+      }
+      item[r] = i < listed ? s.item[w][at] : 0ull;
+    }
+#pragma unroll 1
+    for (uint32_t j = 0; j < own; j += 8) {
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) {
+        const uint64_t other = list[j + e];
+#pragma unroll
+        for (uint32_t r = 0; r < R; ++r) place[r] += other > item[r] ? 1u : 0u;
+      }
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < R; ++r) {
+      place[r] += xor_u32<1>(place[r]);
+      place[r] += xor_u32<2>(place[r]);
+      place[r] += xor_u32<4>(place[r]);
+      if (item[r] && place[r] < a.top && tid % kListWaves == 0)
+        put_best(a, row, place[r], item[r], score);
+    }
   }
 }
+
+// ---- finish -------------------------------------------------------------------
+
+// A row's totals and its tokens' log-probabilities by one wave. What they are
+// worked out from is asked for at once, the lane's first token among it.
+template <int DT>
+struct RowWave {
+  float inv_t;
+  MaxSum part;
+  uint32_t token, ahead;
+
+  __device__ __forceinline__ void load(const ScoreLaunch &a, uint32_t row) {
+    const uint32_t lane = threadIdx.x & 63u;
+    part = row_part(a, row);
+    token = lane < a.token_count ? a.tokens[(uint64_t)row * a.token_stride + lane] : kNoToken;
+    ahead = 0;
+    if (a.out_ranks) {
+      for (uint32_t g = lane; g < a.segments; g += 64)
+        ahead += a.aheads[(uint64_t)row * a.segments + g];
+    }
+    inv_t = inverse_temperature(a, row);
+  }
+  __device__ __forceinline__ RowScore put(const ScoreLaunch &a, uint32_t row,
+                                          const typename Logits<DT>::Element *x) const {
+    const uint32_t lane = threadIdx.x & 63u;
+    float logit = token < a.vocabulary ? logit_value(x[token]) : -__builtin_inff();
+    const MaxSum total = row_total(a, row, part, inv_t * kLog2e);
+    const RowScore score{total.m, inv_t, logf(total.s)};
+    if (lane == 0 && a.out_lse) a.out_lse[row] = score.lse();
+    uint32_t id = token;
+    for (uint32_t i = lane; i < a.token_count; i += 64) {
+      if (i != lane) {
+        id = a.tokens[(uint64_t)row * a.token_stride + i];
+        logit = id < a.vocabulary ? logit_value(x[id]) : -__builtin_inff();
+      }
+      a.out_logprobs[(uint64_t)row * a.token_count + i] = score.logprob(logit);
+    }
+    if (a.out_ranks) {
+      const uint32_t rank = wave_sum_u32(ahead) + 1u;
+      if (lane == 0) a.out_ranks[row] = token < a.vocabulary ? rank : 0u;
+    }
+    return score;
+  }
+};
 
 // One row a wave.
 template <int DT>
 __global__ __launch_bounds__(64) void logprobs_kernel(ScoreLaunch a) {
   const uint32_t row = blockIdx.x;
   const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
-  const MaxSum part = row_part(a, row);
-  const float inv_t = inverse_temperature(a, row);
-  const MaxSum total = row_total(a, row, part, inv_t * kLog2e);
-  put_tokens<DT>(a, row, x, RowScore{total.m, inv_t, logf(total.s)});
+  RowWave<DT> wave;
+  wave.load(a, row);
+  wave.put(a, row, x);
 }
 
-// One row a block, with alternatives: up to N groups a thread. The fifth wave
+// One row a block, with alternatives: up to N groups a thread. The last wave
 // takes the row's totals and tokens while the others list.
 template <int DT, uint32_t N>
 __global__ __launch_bounds__(kTopWaves * 64) void alternatives_kernel(ScoreLaunch a) {
@@ -404,62 +476,48 @@ __global__ __launch_bounds__(kTopWaves * 64) void alternatives_kernel(ScoreLaunc
   const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
   const float *maxima = a.maxima + (uint64_t)row * a.groups;
   uint32_t key[N];
-  if (tid < 256) {
+  RowWave<DT> totals;
+  if (tid < kListThreads) {
     float m[N];
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) m[i] = *element(maxima, min(i * 256 + tid, a.groups - 1));
+    for (uint32_t i = 0; i < N; ++i)
+      m[i] = *element(maxima, min(i * kListThreads + tid, a.groups - 1));
     uint32_t best = 0;
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i) {
-      key[i] = i * 256 + tid < a.groups ? listed_key(m[i]) : 0u;
+      key[i] = i * kListThreads + tid < a.groups ? listed_key(m[i]) : 0u;
       best = max(best, key[i]);
     }
-    if (k <= kQuadTop) {
-      best = max(best, xor_u32<1>(best));
+    best = max(best, xor_u32<1>(best));
+    if (k <= kShortTop) {
       best = max(best, xor_u32<2>(best));
-      if (tid % 4 == 0) s.unit[tid / 4] = best;
+      best = max(best, xor_u32<4>(best));
+      if (tid % 8 == 0) s.unit[tid / 8] = best;
     } else {
-      s.unit[tid] = best;
+      if (tid % 2 == 0) s.unit[tid / 2] = best;
     }
+  } else {
+    totals.load(a, row);
   }
   if (tid == 0) s.crowded = 0;
   __syncthreads();
-  if (tid >= 256) {
-    const float inv_t = inverse_temperature(a, row);
-    const MaxSum total = row_total(a, row, row_part(a, row), inv_t * kLog2e);
-    const RowScore score{total.m, inv_t, logf(total.s)};
-    if (tid == 256) s.score = score;
-    put_tokens<DT>(a, row, x, score);
-  } else if (k <= kQuadTop) {
+  if (tid >= kListThreads) {
+    const RowScore score = totals.put(a, row, x);
+    if (tid == kListThreads) s.score = score;
+  } else if (k <= kShortTop) {
     list_wave<DT, N, 1>(s, a, x, key);
   } else {
     list_wave<DT, N, 4>(s, a, x, key);
   }
   __syncthreads();
-  uint32_t listed;
+  uint32_t listed = 0;
   if (!s.crowded) {
-    // Every item's place is the number of items ahead of it: four lanes an item,
-    // a wave's list each.
-    const uint32_t c0 = s.count[0], c1 = c0 + s.count[1], c2 = c1 + s.count[2];
-    listed = c2 + s.count[3];
-    const RowScore score = s.score;
-    const uint32_t own = s.count[tid % 4];
-    const uint64_t *list = s.item[tid % 4];
-    for (uint32_t first = 0; first < listed; first += kTopWaves * 16) {
-      const uint32_t i = first + tid / 4;
-      const uint32_t w = (i >= c0) + (i >= c1) + (i >= c2);
-      const uint32_t at = i - (w == 0 ? 0u : w == 1 ? c0 : w == 2 ? c1 : c2);
-      const uint64_t item = i < listed ? s.item[w][at] : 0ull;
-      uint32_t place = 0;
-#pragma unroll 1
-      for (uint32_t j = 0; j < own; j += 8) {
 #pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) place += list[j + e] > item ? 1u : 0u;
-      }
-      place += xor_u32<1>(place);
-      place += xor_u32<2>(place);
-      if (item && place < k && tid % 4 == 0) put_best(a, row, place, item, score);
-    }
+    for (uint32_t w = 0; w < kListWaves; ++w) listed += s.count[w];
+    if (k <= kShortTop)
+      place_items<1>(s, a, row, listed);
+    else
+      place_items<3>(s, a, row, listed);
   } else {
     listed = crowded_best<DT, N>(s, a, row, x, maxima);
   }
@@ -592,15 +650,15 @@ __global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
 template <int DT>
 void launch_alternatives(const ScoreLaunch &a, hipStream_t stream) {
   const dim3 rows(a.row_count), block(kTopWaves * 64);
-  const uint32_t each = (a.groups + 255) / 256;
-  if (each <= 4)
+  const uint32_t each = (a.groups + kListThreads - 1) / kListThreads;
+  if (each <= 2)
+    hipLaunchKernelGGL((alternatives_kernel<DT, 2>), rows, block, 0, stream, a);
+  else if (each <= 4)
     hipLaunchKernelGGL((alternatives_kernel<DT, 4>), rows, block, 0, stream, a);
+  else if (each <= 6)
+    hipLaunchKernelGGL((alternatives_kernel<DT, 6>), rows, block, 0, stream, a);
   else if (each <= 8)
     hipLaunchKernelGGL((alternatives_kernel<DT, 8>), rows, block, 0, stream, a);
-  else if (each <= 12)
-    hipLaunchKernelGGL((alternatives_kernel<DT, 12>), rows, block, 0, stream, a);
-  else if (each <= 16)
-    hipLaunchKernelGGL((alternatives_kernel<DT, 16>), rows, block, 0, stream, a);
   else
     hipLaunchKernelGGL((alternatives_kernel<DT, kMostItems>), rows, block, 0, stream, a);
 }
