@@ -36,6 +36,9 @@ __device__ __forceinline__ float list_weight(float mass, const MaxSum &total) {
   return mass == 0.0f || total.s == 0.0f ? 0.0f : mass / total.s;
 }
 
+constexpr uint32_t kHolderBits = 11, kHolders = 1u << kHolderBits;
+static_assert(kTeacherTokens <= 256, "a slot is a byte");
+
 // A row's list, worked out by one wave, SLOTS slots a lane: slot i * 64 + lane
 // is element i of its lane.
 template <int DT, uint32_t SLOTS>
@@ -45,10 +48,10 @@ struct Teacher {
   bool valid[SLOTS];  // a token, and its first slot
   float mass;
 
-  // `listed` is LDS for 64 * SLOTS ids.
+  // `holder` is LDS of kHolders bytes.
   __device__ __forceinline__ void load(const ScoreLaunch &a, uint32_t row,
                                        const typename Logits<DT>::Element *x, float inv_t,
-                                       uint32_t *listed) {
+                                       uint8_t *holder) {
     const uint32_t lane = threadIdx.x & 63u, K = a.teacher_count;
     float value[SLOTS];
 #pragma unroll
@@ -62,16 +65,8 @@ struct Teacher {
       }
       valid[i] = id[i] < a.vocabulary;
       logit[i] = valid[i] ? logit_value(x[id[i]]) : 0.0f;
-      listed[k] = id[i];
     }
-    __builtin_amdgcn_wave_barrier();  // the wave's own LDS, in order
-#pragma unroll 8
-    for (uint32_t k = 0; k < K; ++k) {
-      const uint32_t other = listed[k];
-#pragma unroll
-      for (uint32_t i = 0; i < SLOTS; ++i)
-        valid[i] = valid[i] && !(k < i * 64 + lane && other == id[i]);
-    }
+    keep_first(holder);
     float first = -__builtin_inff();
 #pragma unroll
     for (uint32_t i = 0; i < SLOTS; ++i) {
@@ -100,6 +95,39 @@ struct Teacher {
       mass += p[i];
     }
     mass = wave_sum_f32(mass);
+  }
+
+  // Drops the slots whose token an earlier one lists. Every slot writes itself
+  // down at its token's place in a table: all but one of those that share a token
+  // then find another one there, as few others do, and each such token is looked
+  // up among all slots. (Comparing every slot with every one before it took 98
+  // slots a row 5 us.)
+  __device__ __forceinline__ void keep_first(uint8_t *holder) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const auto place = [&](uint32_t i) { return id[i] * 2654435761u >> (32 - kHolderBits); };
+#pragma unroll
+    for (uint32_t i = 0; i < SLOTS; ++i)
+      if (valid[i]) holder[place(i)] = (uint8_t)(i * 64 + lane);
+    __builtin_amdgcn_wave_barrier();  // the wave's own LDS, in order
+    uint64_t look[SLOTS];
+#pragma unroll
+    for (uint32_t i = 0; i < SLOTS; ++i)
+      look[i] = ballot(valid[i] && holder[place(i)] != (uint8_t)(i * 64 + lane));
+#pragma unroll
+    for (uint32_t i = 0; i < SLOTS; ++i) {
+      while (look[i]) {
+        const uint32_t token = readlane_u32(id[i], __builtin_ctzll(look[i]));
+        bool first = true;
+#pragma unroll
+        for (uint32_t j = 0; j < SLOTS; ++j) {
+          const bool same = valid[j] && id[j] == token;
+          const uint64_t lanes = ballot(same);
+          valid[j] = valid[j] && !(same && !(first && lane == (uint32_t)__builtin_ctzll(lanes)));
+          first = first && !lanes;
+          look[j] &= ~lanes;
+        }
+      }
+    }
   }
 
   // The row's outputs, and what the backward pass takes: the maximum, the
@@ -132,13 +160,13 @@ struct Teacher {
 
 template <int DT, uint32_t SLOTS>
 __global__ __launch_bounds__(64) void distill_loss_kernel(ScoreLaunch a) {
-  __shared__ uint32_t listed[64 * SLOTS];
+  __shared__ uint8_t holder[kHolders];
   const uint32_t row = blockIdx.x;
   const auto *x = row_of<DT>(a.logits, (uint64_t)row * a.stride);
   const float inv_t = 1.0f / a.temperature;
   const MaxSum part = row_part(a, row);
   Teacher<DT, SLOTS> t;
-  t.load(a, row, x, inv_t, listed);
+  t.load(a, row, x, inv_t, holder);
   const MaxSum total = row_total(a, row, part, inv_t * kLog2e);
   t.put(a, row, total, RowScore{total.m, inv_t, logf(total.s)});
 }
@@ -159,7 +187,7 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
   constexpr uint32_t VEC = Logits<DT>::VEC, SLAB = kStepThreads * VEC, QUAD = kQuad * SLAB,
                      HELD = kHeld<SLOTS>;
   using Words = typename Logits<DT>::Words;
-  __shared__ uint32_t listed[64 * SLOTS];
+  __shared__ uint8_t holder[kHolders];
   __shared__ MaxSum part[kStepWaves];
   __shared__ float mass;
   const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63u, row = blockIdx.x;
@@ -184,7 +212,7 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
   // The first wave works the list out while the row arrives.
   Teacher<DT, SLOTS> t;
   if (wave == 0) {
-    t.load(a, row, z, inv_t, listed);
+    t.load(a, row, z, inv_t, holder);
     if (lane == 0) mass = t.mass;
   }
   MaxSum run{-__builtin_inff(), 0.0f};

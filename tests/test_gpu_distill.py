@@ -107,6 +107,25 @@ def test_losses_and_gradients(V, dtype, normalize, T):
         assert not got["grad"][3].any() and not got["grad"][7].any() and got["loss"][7] == 0
 
 
+# Lists of which most or all slots repeat a token, and of tokens apart by
+# multiples of powers of two.
+@pytest.mark.parametrize("K", [2, 63, 64, 65, 200, 256])
+@pytest.mark.parametrize("mode", ["separate", "step"])
+def test_a_token_counts_at_its_first_slot(K, mode):
+    rng = np.random.default_rng(K)
+    V, rows = 70001, 6
+    z = rng.normal(0, 3, (rows, V)).astype(np.float32)
+    ids = np.stack([np.full(K, 17), rng.integers(0, 3, K), rng.integers(0, max(2, K // 2), K),
+                    rng.integers(0, 68, K) * 1024, rng.choice(V, K, replace=False),
+                    np.repeat(rng.choice(V, K, replace=False), 2)[:K]]).astype(np.uint32)
+    ids[3, K // 2] = NO
+    values = rng.normal(0, 1, (rows, K)).astype(np.float32)
+    g = np.ones(rows, np.float32)
+    for normalize in (True, False):
+        v = values if normalize else values - 8
+        check(z, ids, v, 1.5, normalize, g, "f32", run(z, ids, v, 1.5, normalize, g, "f32", mode))
+
+
 def test_cross_entropy_is_a_list_of_one():
     rng = np.random.default_rng(3)
     z = rng.normal(0, 3, (4, 9001)).astype(np.float32)
