@@ -73,8 +73,8 @@ constexpr uint32_t kWaveItems = 512;
 // Lists of up to this many alternatives are cut by the best groups of 64 units of
 // eight lanes, longer ones by those of 256 pairs: a cut by fewer units is
 // quicker to find and lists more groups (64 rows x 151,936 in f32: 5 alternatives
-// 15.2 us by quads, 16.8 by threads; 20 16.3 and 16.8; 33 17.7 and 18.2; 48 20.9
-// and 19.0).
+// 14.3 us by the larger units, 16.0 by pairs; 20 15.3 and 16.7; 33 16.4 and 17.4;
+// 48 19.8 and 17.9).
 constexpr uint32_t kShortTop = 32;
 
 struct TopLds {
@@ -220,8 +220,8 @@ __device__ __forceinline__ uint32_t block_kth_key(TopLds &s, const uint32_t (&ke
   return keys < k ? 0u : block_kth_largest(s, key, search_between(least, most), k, phase);
 }
 
-// The block's `k` best of M keys a thread, each with an id (0 is no
-// key), to put(place, key, id) of their threads, in no order; returns how many.
+// The block's `k` best of M keys a thread, each with an id (0 is no key), to
+// put(place, key, id) of their threads, in no order; returns how many.
 // Whatever the ties: the k-th key, then the k-th of the ids that have it.
 template <uint32_t M, int ID_BITS, class Id, class Put>
 __device__ __forceinline__ uint32_t pick_best(TopLds &s, const uint32_t (&key)[M], uint32_t k,
@@ -256,8 +256,8 @@ __device__ __forceinline__ void put_best(const ScoreLaunch &a, uint32_t row, uin
 // equal maxima, as of a constant row, one masked by a lowest value down to fewer
 // than k tokens, or one that falls from its first token on): its k best groups,
 // then their k best tokens. Returns how many there are. 64 rows x 151,936 in
-// f32, constant: 20 alternatives 32 us, 128 of them 35, and masked by the lowest
-// value 57 and 62 (in random order 14 and 24; in k rounds of a maximum each 67
+// f32, constant: 20 alternatives 32 us, 128 of them 36, and masked by the lowest
+// value 60 and 65 (in random order 13 and 21; in k rounds of a maximum each 67
 // and 975).
 template <int DT, uint32_t N>
 __device__ __forceinline__ uint32_t crowded_best(TopLds &s, const ScoreLaunch &a, uint32_t row,
@@ -643,21 +643,13 @@ __global__ __launch_bounds__(256) void score_kernel(ScoreLaunch a) {
   }
 }
 
-// The groups a thread takes of a row at most, in steps: the kernel asks for all of
-// its places, there or not, at 0.1 us each four (64 rows x 32,000 tokens, 2 groups
-// a thread: 10.3 us with 4 places, 10.8 with 10, 11.2 with 16 and 12.0 with 32; x
-// 100,003, 7 groups: 14.1 with 8, 14.6 with 16 and 15.6 with 32).
+// The places for groups that a thread holds: it asks for all of them, there or
+// not (64 rows x 32,000 tokens, a group a thread: 10.3 us with 8 places, 10.9 with
+// 16; x 151,936, five of them: 15.5 and 15.9; with 6 or 2 no less).
 template <int DT>
 void launch_alternatives(const ScoreLaunch &a, hipStream_t stream) {
   const dim3 rows(a.row_count), block(kTopWaves * 64);
-  const uint32_t each = (a.groups + kListThreads - 1) / kListThreads;
-  if (each <= 2)
-    hipLaunchKernelGGL((alternatives_kernel<DT, 2>), rows, block, 0, stream, a);
-  else if (each <= 4)
-    hipLaunchKernelGGL((alternatives_kernel<DT, 4>), rows, block, 0, stream, a);
-  else if (each <= 6)
-    hipLaunchKernelGGL((alternatives_kernel<DT, 6>), rows, block, 0, stream, a);
-  else if (each <= 8)
+  if (a.groups <= 8 * kListThreads)
     hipLaunchKernelGGL((alternatives_kernel<DT, 8>), rows, block, 0, stream, a);
   else
     hipLaunchKernelGGL((alternatives_kernel<DT, kMostItems>), rows, block, 0, stream, a);

@@ -375,9 +375,9 @@ int jf_process_logits(jf_scorer *s, const jf_process_args *a, void *stream) {
 // ---- the pass over a row -----------------------------------------------------
 
 // The vectors a thread takes of a row at a time, two while four would leave the
-// GPU with few blocks (20 alternatives of one f32 row x 151,936: 9.1 us against
-// 9.6, of 64 rows 17.3 against 16.2; of 8 bf16 rows 10.8 against 11.1, of 64
-// rows 14.8 against 14.5; gradients of 32 bf16 rows 4.4 against 5.2).
+// GPU with few blocks (20 alternatives of one f32 row x 151,936: 8.4 us against
+// 8.8, of 64 rows 17.4 against 15.5; of 8 bf16 rows 9.9 against 10.0, of 64 rows
+// 15.0 against 14.7; gradients of 32 bf16 rows x 100,003 4.6 against 5.2).
 static uint32_t chunk_vectors(uint32_t rows, uint32_t vocabulary, uint32_t dtype) {
   const uint64_t tokens = (uint64_t)rows * vocabulary;
   return tokens <= (dtype == JF_DTYPE_F32 ? 1u << 20 : 8u << 20) ? 2 : 4;
