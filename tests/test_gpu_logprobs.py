@@ -142,6 +142,19 @@ def test_orders_that_crowd_the_best(how, top, V):
     both(x, "bf16", top=top)
 
 
+# Zeros of both signs are equal; subnormal logits keep their order.
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("top", [1, 20, 64, 128])
+def test_zeros_and_subnormals(dtype, top):
+    rng = np.random.default_rng(top)
+    V = 9000
+    x = np.stack([rng.normal(0, 1e-39, V), np.where(rng.random(V) < 0.5, 0.0, -0.0),
+                  np.where(rng.random(V) < 0.99, -1e-39, -0.0),
+                  np.where(rng.random(V) < 0.002, 1e-39, -3.0)]).astype(np.float32)
+    tokens = rng.integers(0, V, (4, 1)).astype(np.uint32)
+    both(x, dtype, tokens=tokens, top=top)
+
+
 # Masks of the lowest value that leave fewer tokens than are listed, as many and more.
 @pytest.mark.parametrize("V", [300, 30000, 151936])
 @pytest.mark.parametrize("top", [20, 128])
