@@ -475,15 +475,16 @@ static int check_distill(const jf_scorer *s, const jf_distill_args *a, bool forw
 }
 
 // Whether a training step takes its rows whole, a block each, in one launch. A
-// short row is done before three launches would be (32,000 tokens bf16: 7.5 us
-// against 13.6 at 16 rows, 14.9 against 24.8 at 512). A long one keeps its block
-// busy longer than the rows' chunks spread over the GPU would take, unless there
-// are rows for every CU: with 4 KB of a row for each row (151,936 bf16, 64 rows
-// 21.3 us against 17.7 and 128 rows 22.7 against 25.9; fp32, 128 rows 44.3
-// against 42.6 and 256 rows 74.9 against 77.8).
+// short row is done before three launches would be (72,256 tokens, one bf16 row
+// 11.1 us against 11.5, 64 rows 12.0 against 13.1, 512 rows 27 against 41). A long
+// one keeps its block busy longer than the rows' chunks spread over the GPU take
+// (100,003 f32, one row 14.6 against 11.6; 151,936 bf16, 64 rows 21.5 against
+// 15.8), unless rows keep nearly half of the CUs busy (96 rows 22.1 against 20.0,
+// 128 rows 23.1 against 24.5) or, of the longest, most (248,320 f32, 128 rows 65.2
+// against 60.7, 192 rows 105.6 against 92.9; bf16, 128 rows 34.9 against 35.6).
 static bool whole_rows(uint32_t rows, uint32_t vocabulary, uint32_t dtype) {
   const size_t row_bytes = vocabulary * element_size(dtype);
-  return row_bytes <= (128u << 10) || rows >= row_bytes / 4096;
+  return vocabulary <= 72u << 10 || rows >= std::max<size_t>(112, row_bytes / 5120);
 }
 
 static int distill(jf_scorer *s, const jf_distill_args *a, bool forward, bool backward,

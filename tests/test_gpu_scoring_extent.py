@@ -92,7 +92,7 @@ def test_more_rows_than_a_launch():
     s.close()
 
 
-@pytest.mark.parametrize("rows", [1, 2, 140])
+@pytest.mark.parametrize("rows", [1, 2, 140, 410])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_largest_vocabulary(rows, dtype):
     """524,288 tokens: few rows by chunks, many by whole rows."""
