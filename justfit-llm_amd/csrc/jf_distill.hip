@@ -10,7 +10,7 @@
 // lane that holds the token subtracts p in registers and every element is
 // stored once (also where the gradient overwrites the logits).
 //
-// Both at once, for many rows: a block takes a whole row, reads it for m and S,
+// Both at once, for short rows and for many: a block takes a whole row, reads it for m and S,
 // and takes it again for the gradient, a third of a 300 KB row from registers,
 // the rest from the caches. What the caches serve counts as well (their fabric
 // carries about 6 TB/s, read and written), so what is held is time: 2048 rows x
