@@ -191,9 +191,16 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
   __shared__ MaxSum part[kStepWaves];
   __shared__ float mass;
   const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63u, row = blockIdx.x;
-  const uint32_t V = a.vocabulary, quads = V / QUAD;
-  const auto *z = row_of<DT>(a.logits, (uint64_t)row * a.stride);
-  auto *dz = row_of<DT>(g.grad, (uint64_t)row * g.grad_stride);
+  const auto *logits = row_of<DT>(a.logits, (uint64_t)row * a.stride);
+  auto *grad = row_of<DT>(g.grad, (uint64_t)row * g.grad_stride);
+  // Vectors count from the gradient's last line before the row, `before` elements
+  // ahead of it, so that every store covers whole lines: a row that starts within
+  // one is stored in parts of lines otherwise (2048 rows x 151,935 bf16: 324 us,
+  // 271 so). Nothing ahead of the row is read or written.
+  const uint32_t before = (uint32_t)((uintptr_t)grad % 128 / sizeof(*grad));
+  const auto *z = logits - before;
+  auto *dz = grad - before;
+  const uint32_t V = before + a.vocabulary, quads = V / QUAD;
   const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
   const float scale = g.grad_loss[(uint64_t)row * g.grad_loss_stride] * inv_t;
   const auto load = [&](uint32_t quad, LogitWords (&w)[kQuad]) {
@@ -204,15 +211,26 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
   // `rest`: the vectors past the last whole quad.
   LogitWords held[HELD][kQuad], rest[kQuad];
 #pragma unroll
-  for (uint32_t q = 0; q < HELD; ++q)
-    if (q < quads) load(q, held[q]);
+  for (uint32_t q = 0; q < HELD; ++q) {
+    if (q >= quads) break;
+    if (q == 0 && tid * VEC < before) {
+      // The row's first line: the first vectors of its first wave.
+      held[0][0] = load_words<DT>(z, tid * VEC, V, kPastMinusInfinity<DT>, before);
+#pragma unroll
+      for (uint32_t j = 1; j < kQuad; ++j)
+        held[0][j] = *(const Words *)(z + j * SLAB + tid * VEC);
+    } else {
+      load(q, held[q]);
+    }
+  }
 #pragma unroll
   for (uint32_t j = 0; j < kQuad; ++j)
-    rest[j] = load_words<DT>(z, quads * QUAD + j * SLAB + tid * VEC, V, kPastMinusInfinity<DT>);
+    rest[j] = load_words<DT>(z, quads * QUAD + j * SLAB + tid * VEC, V, kPastMinusInfinity<DT>,
+                             before);
   // The first wave works the list out while the row arrives.
   Teacher<DT, SLOTS> t;
   if (wave == 0) {
-    t.load(a, row, z, inv_t, holder);
+    t.load(a, row, logits, inv_t, holder);
     if (lane == 0) mass = t.mass;
   }
   MaxSum run{-__builtin_inff(), 0.0f};
@@ -256,9 +274,14 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
   };
   const auto put = [&](uint32_t quad, const LogitWords (&w)[kQuad]) {
 #pragma unroll
-    for (uint32_t j = 0; j < kQuad; ++j)
-      __builtin_nontemporal_store(gradient(w[j]),
-                                  (Words *)(dz + quad * QUAD + j * SLAB + tid * VEC));
+    for (uint32_t j = 0; j < kQuad; ++j) {
+      const uint32_t token = quad * QUAD + j * SLAB + tid * VEC;
+      const LogitWords d = gradient(w[j]);
+      if (j == 0 && token < before)
+        store_words<DT>(dz, token, V, d, before);
+      else
+        __builtin_nontemporal_store(d, (Words *)(dz + token));
+    }
   };
   // The quads read again come first, the last read before the others.
   for (uint32_t q = quads; q-- > HELD;) {
@@ -272,7 +295,7 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
 #pragma unroll
   for (uint32_t j = 0; j < kQuad; ++j) {
     const uint32_t token = quads * QUAD + j * SLAB + tid * VEC;
-    if (token < V) store_words<DT>(dz, token, V, gradient(rest[j]));
+    if (token < V) store_words<DT>(dz, token, V, gradient(rest[j]), before);
   }
   if (wave == 0) t.put(a, row, total, RowScore{total.m, inv_t, logf(total.s)});
   // The listed tokens' elements anew, once every store above has completed.
@@ -281,7 +304,7 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
   if (wave == 0 && scale != 0.0f) {
 #pragma unroll
     for (uint32_t i = 0; i < SLOTS; ++i)
-      if (t.valid[i]) dz[t.id[i]] = logit_of<DT>(pulled(t.logit[i]) - scale * t.p[i]);
+      if (t.valid[i]) grad[t.id[i]] = logit_of<DT>(pulled(t.logit[i]) - scale * t.p[i]);
   }
 }
 

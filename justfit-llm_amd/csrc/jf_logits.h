@@ -85,23 +85,28 @@ __device__ __forceinline__ LogitWords pack(const float (&v)[Logits<DT>::VEC]) {
   return w;
 }
 
-// The vector at `token` of a row of `vocabulary` tokens; those past its end
-// hold the bits `past`.
+// The vector at `token` of a row of `vocabulary` tokens, of which the first
+// `before` are none; those and the ones past its end hold the bits `past`.
 template <int DT>
 __device__ __forceinline__ LogitWords load_words(const typename Logits<DT>::Element *row,
                                                  uint32_t token, uint32_t vocabulary,
-                                                 uint32_t past) {
-  if (token + Logits<DT>::VEC <= vocabulary) return *(const typename Logits<DT>::Words *)(row + token);
+                                                 uint32_t past, uint32_t before = 0) {
+  if (token >= before && token + Logits<DT>::VEC <= vocabulary)
+    return *(const typename Logits<DT>::Words *)(row + token);
+  const auto at = [&](uint32_t t) -> uint32_t {
+    if (t < before || t >= vocabulary) return past;
+    if constexpr (DT == 0)
+      return f2u(row[t]);
+    else
+      return row[t];
+  };
   LogitWords w;
 #pragma unroll
   for (uint32_t e = 0; e < 4; ++e) {
-    if constexpr (DT == 0) {
-      w[e] = token + e < vocabulary ? f2u(row[token + e]) : past;
-    } else {
-      const uint32_t lo = token + 2 * e < vocabulary ? row[token + 2 * e] : past;
-      const uint32_t hi = token + 2 * e + 1 < vocabulary ? row[token + 2 * e + 1] : past;
-      w[e] = lo | hi << 16;
-    }
+    if constexpr (DT == 0)
+      w[e] = at(token + e);
+    else
+      w[e] = at(token + 2 * e) | at(token + 2 * e + 1) << 16;
   }
   return w;
 }
@@ -128,17 +133,18 @@ template <int DT>
 constexpr uint32_t kPastMinusInfinity = DT == 0 ? 0xff800000u : 0xff80u;
 
 // The values of a vector into tokens [token, token + VEC) of a row, those
-// past its end left out.
+// past its end and its first `before` left out.
 template <int DT>
 __device__ __forceinline__ void store_words(typename Logits<DT>::Element *row, uint32_t token,
-                                            uint32_t vocabulary, const LogitWords &w) {
-  if (token + Logits<DT>::VEC <= vocabulary) {
+                                            uint32_t vocabulary, const LogitWords &w,
+                                            uint32_t before = 0) {
+  if (token >= before && token + Logits<DT>::VEC <= vocabulary) {
     *(typename Logits<DT>::Words *)(row + token) = w;
     return;
   }
 #pragma unroll
   for (uint32_t e = 0; e < Logits<DT>::VEC; ++e)
-    if (token + e < vocabulary) {
+    if (token + e >= before && token + e < vocabulary) {
       if constexpr (DT == 0)
         row[token + e] = u2f(w[e]);
       else

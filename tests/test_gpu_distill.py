@@ -126,6 +126,25 @@ def test_a_token_counts_at_its_first_slot(K, mode):
         check(z, ids, v, 1.5, normalize, g, "f32", run(z, ids, v, 1.5, normalize, g, "f32", mode))
 
 
+# Rows that start anywhere in a line, over more tokens than a block holds; the
+# gradient's rows start elsewhere than the logits' but in place.
+@pytest.mark.parametrize("V", [73001, 73727, 65536])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("mode", ["step", "in place"])
+@pytest.mark.parametrize("K", [5, 70])
+def test_whole_rows_at_any_alignment(V, dtype, mode, K):
+    rng = np.random.default_rng(V + K)
+    z = rng.normal(0, 3, (5, V)).astype(np.float32)
+    if dtype == "bf16":
+        z = bf16(z)
+    ids, values = lists(rng, z, K, True, 2.0)
+    ids[:, 0] = 0, 1, V - 1, 2, 70
+    g = rng.normal(0, 1, 5).astype(np.float32)
+    for pad, lead in ((0, 0), (1, 1), (7, 33)):
+        got = run(z, ids, values, 2.0, True, g, dtype, mode, pad, lead)
+        check(z, ids, values, 2.0, True, g, dtype, got)
+
+
 def test_cross_entropy_is_a_list_of_one():
     rng = np.random.default_rng(3)
     z = rng.normal(0, 3, (4, 9001)).astype(np.float32)
