@@ -50,16 +50,20 @@ struct ProcessLds {
 
 // VEC tokens of a row of type DT as a lane loads or stores them: 16 bytes, or 8
 // bytes of bf16 where the other side is f32, so that a wave's loads and its
-// stores both cover whole lines.
-template <int DT, uint32_t VEC>
+// stores both cover whole lines. BELOW: a token may be below 0, modulo 2^32; there
+// is nothing, as past the vocabulary.
+template <int DT, uint32_t VEC, bool BELOW>
 struct Tokens {
   using Element = typename Logits<DT>::Element;
   static constexpr uint32_t WORDS = VEC * sizeof(Element) / 4;
   typedef uint32_t Words __attribute__((ext_vector_type(WORDS)));
   typedef Words WordsAt __attribute__((aligned(sizeof(Element))));
 
+  static __device__ __forceinline__ bool within(uint32_t token, uint32_t V) {
+    return (!BELOW || token < V) && token + VEC <= V;
+  }
   static __device__ __forceinline__ Words load(const Element *row, uint32_t token, uint32_t V) {
-    if (token + VEC <= V) return *(const WordsAt *)(row + token);
+    if (within(token, V)) return *(const WordsAt *)(row + token);
     Words w{};
 #pragma unroll
     for (uint32_t e = 0; e < VEC; ++e)
@@ -73,7 +77,7 @@ struct Tokens {
   }
   template <bool NT>
   static __device__ __forceinline__ void store(Element *row, uint32_t token, uint32_t V, Words w) {
-    if (token + VEC <= V) {
+    if (within(token, V)) {
       if constexpr (NT)
         __builtin_nontemporal_store(w, (WordsAt *)(row + token));
       else
@@ -124,32 +128,46 @@ template <class List>
 __device__ __forceinline__ uint32_t place_at(const List &l, uint32_t at) {
   return l.first[at >> 5] + __popc(l.bits[at >> 5] & ((1u << (at & 31u)) - 1u));
 }
-// Entry i of a list's chunk: its bit, and its place if it begins a word.
+// Entry i of a list, token `at` of the chunk: its bit, and its place if it begins
+// a word.
 template <class List>
-__device__ __forceinline__ void mark(List &l, const PenaltyEntry *list, uint32_t i,
-                                     uint32_t token, uint32_t base) {
-  const uint32_t at = token - base;
+__device__ __forceinline__ void mark(List &l, const PenaltyEntry *list, uint32_t i, uint32_t at,
+                                     uint32_t base) {
   atomicOr(&l.bits[at >> 5], 1u << (at & 31u));
   if (i == 0 || (list[i - 1].token - base) >> 5 != at >> 5) l.first[at >> 5] = (uint16_t)i;
 }
 
+// How a call's outputs are stored: kPast: past the caches (nontemporal); kLines:
+// also in whole lines, of rows that start within one.
+enum Stores { kCached, kPast, kLines };
+
 // A chunk of N vectors a thread.
-template <int DI, int DO, uint32_t N, bool NT>
+template <int DI, int DO, uint32_t N, Stores STORES>
 __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
   constexpr uint32_t VEC = DI == 1 && DO == 1 ? 8 : 4, SLAB = 256 * VEC, CHUNK = N * SLAB;
   constexpr uint32_t ALL = (1u << VEC) - 1u;
   static_assert(CHUNK % kPenaltyBucket == 0 && CHUNK / 32 <= 256);
-  using In = Tokens<DI, VEC>;
-  using Out = Tokens<DO, VEC>;
+  constexpr bool NT = STORES != kCached, BELOW = STORES == kLines;
+  using In = Tokens<DI, VEC, BELOW>;
+  using Out = Tokens<DO, VEC, BELOW>;
   __shared__ ProcessLds<CHUNK> s;
   const uint32_t tid = threadIdx.x;
   const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks;
-  const uint32_t base = chunk * CHUNK, V = a.vocabulary;
+  const uint32_t V = a.vocabulary;
   const auto *x = row_of<DI>(a.logits, (uint64_t)row * a.stride);
   auto *y = row_of<DO>(a.out, (uint64_t)row * a.out_stride);
+  // Whole lines: chunks count from the output's last line before the row; the
+  // first one's `base` is then below 0, modulo 2^32.
+  const uint32_t before = BELOW ? (uint32_t)((uintptr_t)y % 128 / sizeof(*y)) : 0;
+  const uint32_t base = chunk * CHUNK - before;
+  if (BELOW && chunk && base >= V) return;  // not every row reaches the last chunk
+  // Whether any token of a vector is the row's.
+  const auto inside = [&](uint32_t token) {
+    return token < V || (BELOW && 0u - token < VEC);
+  };
   typename In::Words w[N];
   const auto load_all = [&] {
-    if (base + CHUNK <= V) {
+    if ((!BELOW || base < V) && base + CHUNK <= V) {
 #pragma unroll
       for (uint32_t j = 0; j < N; ++j)
         w[j] = *(const typename In::WordsAt *)(x + base + j * SLAB + tid * VEC);
@@ -168,8 +186,8 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
   if (whole && !early) load_all();
 
   uint32_t pen0 = 0, pens = 0, bias0 = 0, biases = 0;
-  const uint32_t b0 = chunk * (CHUNK / kPenaltyBucket);
-  const uint32_t b1 = min(b0 + CHUNK / kPenaltyBucket, a.buckets);
+  const uint32_t b0 = (BELOW && !chunk ? 0 : base) / kPenaltyBucket;
+  const uint32_t b1 = min((base + CHUNK + kPenaltyBucket - 1) / kPenaltyBucket, a.buckets);
   if (p.penalty_row != kNoRow) {
     const uint32_t *off = a.pen_offsets + (uint64_t)p.penalty_row * (a.buckets + 1);
     pen0 = off[b0];
@@ -183,14 +201,23 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
   const bool has_word = tid < CHUNK / 32;
   if (has_word) s.penalty.bits[tid] = s.bias.bits[tid] = s.extra_bits[tid] = 0;
   if (masked && has_word) {
-    // Tokens past the vocabulary are never stored; words past it not read.
-    const uint32_t word = base / 32 + tid;
+    // Tokens outside the vocabulary are never stored; words outside it not read.
     uint32_t bits = 0xffffffffu;
-    if ((p.flags & kProcessMasked) && word < (V + 31) / 32)
-      bits = a.masks[(uint64_t)p.mask_row * a.mask_stride + word];
+    if (p.flags & kProcessMasked) {
+      const uint32_t *mask = a.masks + (uint64_t)p.mask_row * a.mask_stride;
+      const uint32_t words = (V + 31) / 32;
+      const int32_t token = (int32_t)(base + tid * 32);
+      const uint32_t word = (uint32_t)(token >> 5), shift = token & 31;
+      bits = word < words ? mask[word] : 0xffffffffu;
+      if (BELOW && shift) {
+        const uint32_t next = word + 1 < words ? mask[word + 1] : 0xffffffffu;
+        bits = bits >> shift | next << (32 - shift);
+      }
+    }
     if (p.flags & kProcessStops) {
-      if (a.stop0 / 32 == word) bits &= ~(1u << (a.stop0 % 32));
-      if (a.stop1 / 32 == word) bits &= ~(1u << (a.stop1 % 32));
+      const uint32_t at0 = a.stop0 - base, at1 = a.stop1 - base;
+      if (at0 >> 5 == tid) bits &= ~(1u << (at0 & 31u));
+      if (at1 >> 5 == tid) bits &= ~(1u << (at1 & 31u));
     }
     s.admitted[tid] = bits;
   }
@@ -202,7 +229,7 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
     for (uint32_t j = 0; j < N; ++j) {
       const uint32_t at = j * SLAB + tid * VEC;
       w[j] = typename In::Words{};
-      if (base + at < V && bits_at<VEC>(s.admitted, at)) w[j] = In::load(x, base + at, V);
+      if (inside(base + at) && bits_at<VEC>(s.admitted, at)) w[j] = In::load(x, base + at, V);
     }
   }
   const PenaltyEntry *pen_list =
@@ -216,14 +243,18 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
   };
   for (uint32_t i = tid; i < biases; i += 256) {
     const PenaltyEntry e = bias_list[i];
-    mark(s.bias, bias_list, i, e.token, base);
+    const uint32_t at = e.token - base;
+    if (BELOW && at >= CHUNK) continue;  // of a bucket that the chunk shares
+    mark(s.bias, bias_list, i, at, base);
     if (i < kStaged) s.bias.value[i] = u2f(e.word);
   }
   for (uint32_t i = tid; i < pens; i += 256) {
     const PenaltyEntry e = pen_list[i];
-    mark(s.penalty, pen_list, i, e.token, base);
+    const uint32_t at = e.token - base;
+    if (BELOW && at >= CHUNK) continue;
+    mark(s.penalty, pen_list, i, at, base);
     // A dropped token's value is never taken, nor its logit read.
-    if (i < kStaged && !(masked && !bit_at(s.admitted, e.token - base)))
+    if (i < kStaged && !(masked && !bit_at(s.admitted, at)))
       s.penalty.value[i] = penalized(e, logit_value(x[e.token]));
   }
   if (p.extra_count) {
@@ -251,7 +282,7 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
     for (uint32_t j = 0; j < N; ++j) {
       const uint32_t at = j * SLAB + tid * VEC;
       w[j] = typename In::Words{};
-      if (base + at >= V) continue;
+      if (!inside(base + at)) continue;
       const uint32_t admitted = masked ? bits_at<VEC>(s.admitted, at) : ALL;
       if (admitted && (admitted != ALL || edited_at(at)))
         w[j] = In::load(x, base + at, V);
@@ -262,7 +293,7 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
 #pragma unroll
   for (uint32_t j = 0; j < N; ++j) {
     const uint32_t at = j * SLAB + tid * VEC, token = base + at;
-    if (token >= V) continue;
+    if (!inside(token)) continue;
     const uint32_t admitted = masked ? bits_at<VEC>(s.admitted, at) : ALL;
     const uint32_t edited = edited_at(at) & admitted;
     if (a.in_place && !edited && admitted == ALL) continue;
@@ -305,18 +336,30 @@ __global__ __launch_bounds__(256) void process_kernel(ProcessLaunch a) {
 // masked rows x 248,320 bf16 take 28.7 us so, 46.5 otherwise, and 67.3 or 67.6
 // with a pass that reads them behind; 64 rows x 151,936 in f32, 39 MB, 15.0 or
 // 16.3, and 26.0 or 26.5. A smaller output is found there by its reader: 16 such
-// rows 6.6 or 7.3, but 14.7 or 14.2 with the reader.
+// rows 6.6 or 7.3, but 14.7 or 14.2 with the reader. Such stores of parts of lines
+// are dear: rows that start within a line take them whole at the price of masks
+// that shift and vectors that begin below the row (256 masked rows x 248,319 bf16
+// 34.9 us without, 31.2 so; but 256 bf16 rows x 151,936 to f32, aligned, 40.4
+// without, 44.3 so).
 constexpr uint64_t kCachedOutput = 24u << 20;
 
 template <int DI, int DO, uint32_t CHUNK>
 void launch_chunks(ProcessLaunch a, hipStream_t stream) {
   constexpr uint32_t N = CHUNK / (256 * (DI == 1 && DO == 1 ? 8 : 4));
-  a.chunks = (a.vocabulary + CHUNK - 1) / CHUNK;
+  constexpr uint32_t SIZE = sizeof(typename Logits<DO>::Element);
+  const bool past = (uint64_t)a.row_count * a.vocabulary * SIZE > kCachedOutput;
+  const bool lines = past && ((uintptr_t)a.out % 128 != 0 ||
+                              (a.row_count > 1 && a.out_stride * SIZE % 128 != 0));
+  // A row that starts within a line may reach a chunk more.
+  const uint32_t before = lines ? 128 / SIZE - 1 : 0;
+  a.chunks = (a.vocabulary + before + CHUNK - 1) / CHUNK;
   const dim3 grid(a.row_count * a.chunks), block(256);
-  if ((uint64_t)a.row_count * a.vocabulary * sizeof(typename Logits<DO>::Element) > kCachedOutput)
-    hipLaunchKernelGGL((process_kernel<DI, DO, N, true>), grid, block, 0, stream, a);
+  if (lines)
+    hipLaunchKernelGGL((process_kernel<DI, DO, N, kLines>), grid, block, 0, stream, a);
+  else if (past)
+    hipLaunchKernelGGL((process_kernel<DI, DO, N, kPast>), grid, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((process_kernel<DI, DO, N, false>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((process_kernel<DI, DO, N, kCached>), grid, block, 0, stream, a);
 }
 
 // Small chunks while there are few, for blocks on every CU (16 rows x 151,936:

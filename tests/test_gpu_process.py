@@ -34,7 +34,7 @@ POLICIES = [dict(), dict(repetition=1.3), dict(presence=0.7, frequency=0.2),
 
 
 def _run(V, rows, dtype, out_dtype, pad=0, lead=0, out_pad=0, in_place=False, seed=0, x=None,
-         biases=7, extras=True, history=900):
+         biases=7, extras=True, history=900, kinds=POLICIES):
     """Every row its own policy; returns nothing, checks every element."""
     import torch
     print(f"process V={V} rows={rows} {dtype}->{out_dtype} pad={pad} lead={lead} "
@@ -44,7 +44,7 @@ def _run(V, rows, dtype, out_dtype, pad=0, lead=0, out_pad=0, in_place=False, se
         x = rng.normal(0, 4, (rows, V)).astype(np.float32)
     if dtype == "bf16":
         x = bf16(x)
-    policies = [J.policy(**POLICIES[r % len(POLICIES)]) for r in range(rows)]
+    policies = [J.policy(**kinds[r % len(kinds)]) for r in range(rows)]
     stops = (V // 2, V - 1)
     n = max(2, min(2 * V, history))
     table = J.PenaltyTable(V, rows, n + 8)
@@ -115,6 +115,38 @@ def test_processed_logits(V, dtype, out):
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_in_place(V, dtype):
     _run(V, 9, dtype, dtype, pad=3, lead=1, in_place=True)
+
+
+# Outputs that go past the caches, from rows that start anywhere in a line.
+@pytest.mark.parametrize("V,rows,dtype,out,in_place", [
+    (50021, 130, "f32", "f32", False), (50021, 130, "bf16", "f32", False),
+    (50021, 260, "bf16", "bf16", False), (50021, 260, "f32", "bf16", False),
+    (50021, 130, "f32", "f32", True), (50021, 260, "bf16", "bf16", True),
+    (8191, 800, "bf16", "f32", False), (65536, 200, "bf16", "bf16", False)])
+def test_large_outputs_at_any_alignment(V, rows, dtype, out, in_place):
+    _run(V, rows, dtype, out, pad=3, lead=V % 7, out_pad=V % 4, in_place=in_place)
+
+
+@pytest.mark.parametrize("dtype,out,in_place", [
+    ("f32", "f32", False), ("bf16", "f32", False), ("bf16", "bf16", False), ("bf16", "bf16", True)])
+def test_large_masked_outputs_at_any_alignment(dtype, out, in_place):
+    _run(50021, 340, dtype, out, pad=3, lead=5, out_pad=1, in_place=in_place,
+         kinds=[k for k in POLICIES if k.get("constrained") or k.get("exclude_stop")])
+
+
+@pytest.mark.parametrize("V,rows", [(2, 3300000), (3, 2200000), (7, 1000000), (40, 160000)])
+def test_many_short_rows(V, rows):
+    import torch
+    buf = torch.full((rows * V + 64,), 5.0, device="cuda")
+    out = buf[33:33 + rows * V].view(rows, V)
+    t = torch.randn((rows, V), device="cuda")
+    s = J.Scorer(V, rows)
+    s.process(t, [J.policy(exclude_stop=True)] * rows, out, stop_tokens=(1, NO))
+    want = t.clone()
+    want[:, 1] = -float("inf")
+    assert torch.equal(out, want)
+    assert bool((buf[:33] == 5).all()) and bool((buf[33 + rows * V:] == 5).all())
+    s.close()
 
 
 @pytest.mark.parametrize("biases,history", [(700, 900), (3001, 900), (10, 12000), (2500, 12000)])
