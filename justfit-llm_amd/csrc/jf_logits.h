@@ -110,22 +110,22 @@ __device__ __forceinline__ LogitWords load_words(const typename Logits<DT>::Elem
   }
   return w;
 }
-// A thread's vectors of the chunk of N slabs at `base`. One branch for the
+// A thread's vectors of the chunk of N slabs at `base`, likewise. One branch for the
 // chunk: with one a vector the compiler keeps every vector's ways apart in
 // registers.
 template <int DT, uint32_t N>
 __device__ __forceinline__ void load_chunk(const typename Logits<DT>::Element *row, uint32_t base,
                                            uint32_t vocabulary, uint32_t past,
-                                           LogitWords (&w)[N]) {
+                                           LogitWords (&w)[N], uint32_t before = 0) {
   const uint32_t token = base + threadIdx.x * Logits<DT>::VEC;
-  if (base + N * kSlab<DT> <= vocabulary) {
+  if (base >= before && base + N * kSlab<DT> <= vocabulary) {
 #pragma unroll
     for (uint32_t j = 0; j < N; ++j)
       w[j] = *(const typename Logits<DT>::Words *)(row + token + j * kSlab<DT>);
   } else {
 #pragma unroll
     for (uint32_t j = 0; j < N; ++j)
-      w[j] = load_words<DT>(row, token + j * kSlab<DT>, vocabulary, past);
+      w[j] = load_words<DT>(row, token + j * kSlab<DT>, vocabulary, past, before);
   }
 }
 // The bits of -infinity for `past`.

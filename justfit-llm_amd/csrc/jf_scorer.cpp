@@ -522,7 +522,6 @@ static int distill(jf_scorer *s, const jf_distill_args *a, bool forward, bool ba
       G.row_count = n;
       G.vocabulary = s->vocabulary;
       G.vectors = L.vectors;
-      G.chunks = L.segments;
       G.grad_loss = a->grad_loss + r * a->grad_loss_stride;
       G.grad_loss_stride = a->grad_loss_stride;
     }

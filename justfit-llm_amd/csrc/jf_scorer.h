@@ -100,7 +100,7 @@ struct DistillGradLaunch {
   uint64_t grad_stride;
   uint32_t row_count, vocabulary;
   uint32_t vectors;  // a thread: 2 or 4
-  uint32_t chunks;   // blocks a row
+  uint32_t chunks;   // blocks a row: the launch's own
   float temperature;
   const uint32_t *teacher_ids;
   uint64_t teacher_stride;
