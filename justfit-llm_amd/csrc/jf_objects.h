@@ -167,6 +167,14 @@ inline int check_device(int device) {
   return JF_OK;
 }
 
+// Whether what is enqueued on `stream` goes into a graph now.
+inline int is_capturing(hipStream_t stream, bool &capturing) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  JF_HIP(hipStreamIsCapturing(stream, &status), "capture status");
+  capturing = status != hipStreamCaptureStatusNone;
+  return JF_OK;
+}
+
 }  // namespace jf::host
 
 // Fixed penalty slots a chunk at most (two per thread of the fast kernel).

@@ -323,6 +323,13 @@ int jf_process_logits(jf_scorer *s, const jf_process_args *a, void *stream) {
     const size_t bytes = s->host_rows.size() * sizeof(jf::ProcessRow);
     if (s->last_rows.size() < s->host_rows.size() ||
         std::memcmp(s->last_rows.data(), s->host_rows.data(), bytes) != 0) {
+      // A replay would upload what the pinned buffer holds by then.
+      bool capturing;
+      rc = is_capturing((hipStream_t)stream, capturing);
+      if (rc != JF_OK) return rc;
+      if (capturing)
+        return fail(JF_ERR_LOGIC, "a captured call repeats the rows of the scorer's last call; "
+                                  "issue it once before");
       s->last_rows.clear();
       rc = s->staging.upload(s->rows, s->host_rows.data(), bytes, (hipStream_t)stream);
       if (rc != JF_OK) return rc;

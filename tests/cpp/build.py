@@ -1,7 +1,8 @@
 """Builds the C++ test programs into tests/cpp/_build: sampling_mirror, the
 driver of the C++ operator mirror, against the in-tree libjf_sampler.so, and
-launch_plan, the library's host objects over recording launchers (build the
-library first)."""
+launch_plan, the library's host objects over recording launchers, and
+libscorer_host.so, the scorer's over a recording device as well (build the library
+first)."""
 import os
 import subprocess
 import sys
@@ -12,6 +13,7 @@ LIBDIR = os.path.join(REPO, "justfit-llm_amd", "jf_sampler")
 OBJ = os.path.join(REPO, "justfit-llm_amd", "_build")
 OUT = os.path.join(HERE, "_build", "sampling_mirror")
 PLAN = os.path.join(HERE, "_build", "launch_plan")
+SCORER = os.path.join(HERE, "_build", "libscorer_host.so")
 
 
 def _compile(source, out, link, verbose):
@@ -38,6 +40,10 @@ def build(verbose=True):
     _compile("launch_plan.cpp", PLAN,
              ["-x", "none"] + [os.path.join(OBJ, n + ".o")
                                for n in ("jf_sampler.cpp", "jf_host.cpp")], verbose)
+    _compile("scorer_host.cpp", SCORER,
+             ["-x", "none"] + [os.path.join(OBJ, n + ".o")
+                               for n in ("jf_scorer.cpp", "jf_host.cpp")] +
+             ["-shared", "-fPIC", "-Wl,-Bsymbolic"], verbose)
     return OUT
 
 
