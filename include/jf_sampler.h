@@ -601,8 +601,9 @@ int jf_bias_table_set(jf_bias_table *table, uint32_t row,
  * stride: then only edited and dropped tokens are written. Otherwise the two
  * share no element. Row records are uploaded when they differ from the last
  * call's (as jf_sample's). A call that repeats them may be captured into a HIP
- * graph (another fails with JF_ERR_LOGIC there); its replays read the records
- * that the scorer's last call left. */
+ * graph (another fails with JF_ERR_LOGIC there): its replays read those records
+ * whatever the scorer is called with since, which keeps 48 bytes a row of
+ * max_rows until the scorer is destroyed, and the tables' rows as they are then. */
 typedef struct jf_process_args {
   uint32_t rows;
   uint32_t dtype;

@@ -167,8 +167,11 @@ inline int check_device(int device) {
   return JF_OK;
 }
 
-// Whether what is enqueued on `stream` goes into a graph now.
+// Whether what is enqueued on `stream` goes into a graph now; the null stream's
+// never does.
 inline int is_capturing(hipStream_t stream, bool &capturing) {
+  capturing = false;
+  if (!stream) return JF_OK;
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   JF_HIP(hipStreamIsCapturing(stream, &status), "capture status");
   capturing = status != hipStreamCaptureStatusNone;

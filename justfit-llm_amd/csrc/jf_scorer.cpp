@@ -74,6 +74,10 @@ struct jf_scorer {
   uint64_t workspace_bytes = 0;
   std::vector<jf::ProcessRow> last_rows;  // what the device's rows hold
   std::vector<jf::ProcessRow> host_rows;  // the call's rows, reused across calls
+  // A captured call's masks, tables and launches go with its records, which its
+  // replays read: they stay as they are, and other records go elsewhere.
+  bool rows_captured = false;                    // `rows` are such
+  std::vector<jf::ProcessRow *> captured_rows;  // earlier ones, [max_rows] each
   StagingRing staging;
 };
 
@@ -178,6 +182,7 @@ int jf_scorer_destroy(jf_scorer *s) {
   if (!s) return JF_OK;
   s->staging.release();
   (void)hipFree(s->rows);
+  for (jf::ProcessRow *rows : s->captured_rows) (void)hipFree(rows);
   (void)hipFree(s->partials);
   (void)hipFree(s->aheads);
   (void)hipFree(s->maxima);
@@ -242,6 +247,19 @@ static int check_rows(const jf_scorer *s, uint32_t rows, uint32_t dtype, const v
 }
 
 // ---- processed logits --------------------------------------------------------
+
+// Leaves the records that a captured call reads to its replays.
+static int leave_captured_rows(jf_scorer *s) {
+  s->captured_rows.reserve(s->captured_rows.size() + 1);
+  jf::ProcessRow *fresh;
+  const int rc = device_alloc(&fresh, s->max_rows, "row records");
+  if (rc != JF_OK) return rc;
+  s->captured_rows.push_back(s->rows);
+  s->rows = fresh;
+  s->rows_captured = false;
+  s->workspace_bytes += s->max_rows * sizeof(jf::ProcessRow);
+  return JF_OK;
+}
 
 static int fill_process_rows(const jf_scorer *s, const jf_process_args *a,
                              std::vector<jf::ProcessRow> &rows) {
@@ -314,6 +332,9 @@ int jf_process_logits(jf_scorer *s, const jf_process_args *a, void *stream) {
       (a->out_dtype != a->dtype || (a->rows > 1 && a->out_stride != a->logits_stride)))
     return fail(JF_ERR_INVALID_ARGUMENT,
                 "logits processed in place keep their dtype and row stride");
+  bool capturing;
+  rc = is_capturing((hipStream_t)stream, capturing);
+  if (rc != JF_OK) return rc;
   try {
     s->host_rows.clear();
     rc = fill_process_rows(s, a, s->host_rows);
@@ -324,13 +345,11 @@ int jf_process_logits(jf_scorer *s, const jf_process_args *a, void *stream) {
     if (s->last_rows.size() < s->host_rows.size() ||
         std::memcmp(s->last_rows.data(), s->host_rows.data(), bytes) != 0) {
       // A replay would upload what the pinned buffer holds by then.
-      bool capturing;
-      rc = is_capturing((hipStream_t)stream, capturing);
-      if (rc != JF_OK) return rc;
       if (capturing)
         return fail(JF_ERR_LOGIC, "a captured call repeats the rows of the scorer's last call; "
                                   "issue it once before");
       s->last_rows.clear();
+      if (s->rows_captured && (rc = leave_captured_rows(s)) != JF_OK) return rc;
       rc = s->staging.upload(s->rows, s->host_rows.data(), bytes, (hipStream_t)stream);
       if (rc != JF_OK) return rc;
       s->last_rows = s->host_rows;
@@ -339,6 +358,7 @@ int jf_process_logits(jf_scorer *s, const jf_process_args *a, void *stream) {
     s->last_rows.clear();
     return fail(JF_ERR_NO_MEMORY, "row record allocation failed");
   }
+  s->rows_captured |= capturing;
   const uint64_t stride = a->rows > 1 ? a->logits_stride : s->vocabulary;
   const uint64_t out_stride = a->rows > 1 ? a->out_stride : s->vocabulary;
   const uint32_t most = launch_rows(s->vocabulary);

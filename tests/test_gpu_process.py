@@ -355,3 +355,69 @@ def test_refusals():
     # Nothing above reached the output.
     assert not out.any()
     s.close()
+
+
+@pytest.mark.parametrize("rows", [3, 70])
+def test_a_graph_replays_its_own_rows_whatever_the_scorer_does_since(rows):
+    """Captured without masks and tables and with them; calls of the other kind, of
+    fewer and of more rows come between, and each replay equals the eager call."""
+    import torch
+    V, rng = 6000, np.random.default_rng(12)
+    x = rng.normal(0, 3, (rows, V)).astype(np.float32)
+    _, masks = _masks(rng, rows, V)
+    t, _ = device_rows(x, "f32")
+    table, bias = J.PenaltyTable(V, rows, 40), J.BiasTable(V, rows, 9)
+    for r in range(rows):
+        table.rebuild(r, rng.integers(0, V, 30), 15, None, True)
+        bias.set(r, rng.choice(V, 9, replace=False), rng.normal(0, 3, 9))
+    m = torch.from_numpy(masks.view(np.int32)).cuda()
+    s = J.Scorer(V, rows)
+    edited = dict(masks=m, penalties=table, penalty_rows=range(rows), biases=bias,
+                  bias_rows=range(rows))
+    kinds = [([J.policy()] * rows, {}),
+             ([J.policy(constrained=True, presence=0.5)] * rows, edited),
+             ([J.policy(repetition=1.2)] * rows, dict(edited, masks=None)),
+             ([J.policy(constrained=True)] * rows, dict(masks=m))]
+    outs = [torch.zeros((rows, V), device="cuda") for _ in kinds]
+    records = [s.process_args(t, p, o, **kw) for (p, kw), o in zip(kinds, outs)]
+    stream, wants, graphs = torch.cuda.Stream(), [], []
+    for (a, _), out in zip(records, outs):
+        s.launch_process(a)
+        wants.append(host(out))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            s.launch_process(a)
+        graphs.append(graph)
+    few_out = torch.zeros((2, V), device="cuda")
+    few = s.process_args(t[:2], [J.policy(exclude_stop=True), J.policy(constrained=True)], few_out,
+                         masks=m)
+    for turn in range(3):
+        for n, (graph, out) in enumerate(zip(graphs, outs)):
+            for i in (few[0], records[(n + 1 + turn) % 4][0]):
+                s.launch_process(i)
+            torch.cuda.synchronize()
+            for o in outs:
+                o.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            np.testing.assert_array_equal(host(out), wants[n])
+            assert not any(bool(o.any()) for k, o in enumerate(outs) if k != n)
+    # A call with records of its own is refused inside a capture, and the scorer
+    # goes on.
+    s.launch_process(records[1][0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(J.JfError) as e:
+            s.launch_process(few[0])
+        s.launch_process(records[1][0])
+    assert e.value.code == J.JF_ERR_LOGIC
+    s.launch_process(few[0])
+    assert few_out.any()
+    torch.cuda.synchronize()
+    outs[1].zero_()
+    graph.replay()
+    np.testing.assert_array_equal(host(outs[1]), wants[1])
+    del graph, graphs, few_out
+    s.close()

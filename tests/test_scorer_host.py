@@ -12,6 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "cpp", "_build", "libscorer_host.so")
 vp, u32 = ctypes.c_void_p, ctypes.c_uint32
 LOGITS, OUT, MASKS = 1 << 30, 2 << 30, 3 << 30  # addresses that nothing reads
+STREAM = vp(64)
 
 
 class Host:
@@ -60,7 +61,7 @@ class Host:
         a.stop_token_0 = a.stop_token_1 = J.JF_NO_TOKEN
         for name, value in fields.items():
             setattr(a, name, value)
-        rc = self.lib.jf_process_logits(self.scorer, ctypes.byref(a), None)
+        rc = self.lib.jf_process_logits(self.scorer, ctypes.byref(a), STREAM)
         return rc, self.log()
 
     def refused(self, rc, code, message):
@@ -90,3 +91,46 @@ def test_a_captured_call_brings_no_new_row_records():
         h.capturing(False)
         rc, log = h.process([MASKED] * 2)
         assert rc == 0 and kinds(log)[-2:] == ["copy", "process"]
+
+
+def test_captured_calls_keep_their_row_records():
+    """A captured call has its masks and tables fixed, so its replays have to read
+    the records that go with them, whatever the scorer is called with since."""
+    with Host() as h:
+        records = next(e["at"] for e in h.created if e["what"] == "malloc")
+
+        def call(policies, capture=False):
+            h.capturing(capture)
+            rc, log = h.process(policies)
+            h.capturing(False)
+            assert rc == 0
+            assert not capture or kinds(log) == ["process"]
+            uploads = [e for e in log if e["what"] == "copy"]
+            for e in uploads:
+                held[e["to"]] = bytes.fromhex(e["held"])
+            (used,) = [e["rows"] for e in log if e["what"] == "process"]
+            return used, held[used][:48 * len(policies)]
+
+        held, graphs = {}, []
+        for policies in ([PLAIN] * 2, [MASKED, PLAIN], [MASKED] * 4, [PLAIN] * 2):
+            eager = call(policies)
+            graphs.append(call(policies, capture=True))
+            assert graphs[-1] == eager
+            # Calls with and without new records behind the captured one.
+            for other in (policies, [PLAIN, MASKED, MASKED], [MASKED], policies):
+                call(other)
+                for used, then in graphs:
+                    assert held[used][:len(then)] == then
+        # Calls that nothing captured share one place.
+        places = len(held)
+        for policies in ([PLAIN], [MASKED], [PLAIN] * 4):
+            call(policies)
+        assert len(held) == places == 1 + len(graphs) and records in held
+        # Counted, and freed with the scorer.
+        h.lib.jf_scorer_workspace_bytes.restype = ctypes.c_uint64
+        bytes_before = sum(e["bytes"] for e in h.created if e["what"] == "malloc")
+        assert h.lib.jf_scorer_workspace_bytes(h.scorer) == bytes_before + 4 * 4 * 48
+        h.lib.jf_scorer_destroy(h.scorer)
+        h.scorer = vp()
+        freed = {e["at"] for e in h.log() if e["what"] == "free"}
+        assert set(held) <= freed
