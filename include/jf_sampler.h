@@ -585,7 +585,8 @@ int jf_bias_table_create(uint32_t vocabulary, uint32_t rows,
 int jf_bias_table_destroy(jf_bias_table *table);
 /* Replaces row `row` by `count` host pairs in any order (0 clears it); uploads
  * on `stream`. A token outside the vocabulary or given twice, or a bias that
- * is NaN or +infinity, fails before the row changes. */
+ * is NaN or +infinity, fails before the row changes, and so does a stream that
+ * is being captured (JF_ERR_LOGIC). */
 int jf_bias_table_set(jf_bias_table *table, uint32_t row,
                       const uint32_t *tokens, const float *biases,
                       uint64_t count, void *stream);

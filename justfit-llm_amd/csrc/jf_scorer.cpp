@@ -139,6 +139,11 @@ int jf_bias_table_set(jf_bias_table *t, uint32_t row, const uint32_t *tokens, co
     return fail(JF_ERR_INVALID_ARGUMENT, "biases exceed the table row");
   int rc = check_device(t->device);
   if (rc != JF_OK) return rc;
+  // A replay would upload what the pinned buffers hold by then.
+  bool capturing;
+  rc = is_capturing((hipStream_t)stream, capturing);
+  if (rc != JF_OK) return rc;
+  if (capturing) return fail(JF_ERR_LOGIC, "a bias row's upload cannot be captured");
   try {
     std::vector<std::pair<uint32_t, float>> sorted(count);
     for (uint64_t i = 0; i < count; ++i) {

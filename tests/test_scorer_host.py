@@ -134,3 +134,23 @@ def test_captured_calls_keep_their_row_records():
         h.scorer = vp()
         freed = {e["at"] for e in h.log() if e["what"] == "free"}
         assert set(held) <= freed
+
+
+def test_biases_are_not_set_inside_a_capture():
+    with Host() as h:
+        table = vp()
+        assert h.lib.jf_bias_table_create(1000, 2, 4, ctypes.byref(table)) == 0
+        h.log()
+        tokens, biases = (u32 * 2)(3, 9), (ctypes.c_float * 2)(1.0, 2.0)
+        args = (table, 1, tokens, biases, ctypes.c_uint64(2), STREAM)
+        h.capturing(True)
+        h.refused(h.lib.jf_bias_table_set(*args), J.JF_ERR_LOGIC, "captured")
+        assert not h.log()
+        # The row is as it was, and may be used.
+        rc, _ = h.process([PLAIN], biases=table, bias_rows=(u32 * 1)(1))
+        assert rc == J.JF_ERR_LOGIC  # its records are new
+        h.capturing(False)
+        assert h.process([PLAIN], biases=table, bias_rows=(u32 * 1)(1))[0] == 0
+        assert h.lib.jf_bias_table_set(*args) == 0
+        assert kinds(h.log()) == ["copy", "copy"]
+        h.lib.jf_bias_table_destroy(table)
