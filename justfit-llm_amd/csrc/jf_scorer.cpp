@@ -286,6 +286,8 @@ static int fill_process_rows(const jf_scorer *s, const jf_process_args *a,
         return fail(JF_ERR_INVALID_ARGUMENT, "penalized lane has no penalty table row");
       if (a->penalties->vocabulary != s->vocabulary)
         return fail(JF_ERR_INVALID_ARGUMENT, "penalty table vocabulary differs");
+      if (a->penalties->device != s->device)
+        return fail(JF_ERR_INVALID_ARGUMENT, "penalty table is on another device");
       if (a->penalties->stale[a->penalty_rows[r]])
         return fail(JF_ERR_LOGIC, "penalty table row is out of date after a failed update; "
                                   "rebuild it");
@@ -311,6 +313,8 @@ static int fill_process_rows(const jf_scorer *s, const jf_process_args *a,
         return fail(JF_ERR_INVALID_ARGUMENT, "biased row has no bias table row");
       if (a->biases->vocabulary != s->vocabulary)
         return fail(JF_ERR_INVALID_ARGUMENT, "bias table vocabulary differs");
+      if (a->biases->device != s->device)
+        return fail(JF_ERR_INVALID_ARGUMENT, "bias table is on another device");
       if (a->biases->stale[a->bias_rows[r]])
         return fail(JF_ERR_LOGIC, "bias table row is out of date after a failed update; set it");
       row.bias_row = a->bias_rows[r];

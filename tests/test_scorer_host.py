@@ -154,3 +154,26 @@ def test_biases_are_not_set_inside_a_capture():
         assert h.lib.jf_bias_table_set(*args) == 0
         assert kinds(h.log()) == ["copy", "copy"]
         h.lib.jf_bias_table_destroy(table)
+
+
+def test_tables_of_another_device_are_refused():
+    with Host() as h:
+        biases = vp()
+        h.device(1)
+        assert h.lib.jf_bias_table_create(1000, 1, 4, ctypes.byref(biases)) == 0
+        h.device(0)
+        h.lib.fake_penalty_table.restype = vp
+        penalties = [vp(h.lib.fake_penalty_table(1000, device)) for device in (0, 1)]
+        row = (u32 * 1)(0)
+        h.log()
+        rc, log = h.process([PLAIN], biases=biases, bias_rows=row)
+        h.refused(rc, J.JF_ERR_INVALID_ARGUMENT, "bias table is on another device")
+        assert not log
+        penalized = [J.policy(presence=1.0)]
+        rc, log = h.process(penalized, penalties=penalties[1], penalty_rows=row)
+        h.refused(rc, J.JF_ERR_INVALID_ARGUMENT, "penalty table is on another device")
+        assert not log
+        assert h.process(penalized, penalties=penalties[0], penalty_rows=row)[0] == 0
+        for table in penalties:
+            h.lib.fake_penalty_table_free(table)
+        h.lib.jf_bias_table_destroy(biases)
