@@ -577,7 +577,7 @@ int jf_scorer_destroy(jf_scorer *scorer);
 uint64_t jf_scorer_workspace_bytes(const jf_scorer *scorer);
 
 /* Requests' logit biases on the device, one row a request, each of at most
- * max_entries distinct tokens. A bias is finite, or -infinity for a ban. */
+ * max_entries distinct tokens of a scorer's vocabulary. A bias is finite, or -infinity for a ban. */
 typedef struct jf_bias_table jf_bias_table;
 
 int jf_bias_table_create(uint32_t vocabulary, uint32_t rows,

@@ -100,6 +100,8 @@ int jf_bias_table_create(uint32_t vocabulary, uint32_t rows, uint32_t max_entrie
   *out = nullptr;
   if (!vocabulary || !rows || !max_entries || max_entries > 0x7fffffffu)
     return fail(JF_ERR_INVALID_ARGUMENT, "invalid bias table geometry");
+  if (vocabulary > kMaxVocabulary)
+    return fail(JF_ERR_INVALID_ARGUMENT, "vocabulary exceeds 524288 tokens");
   jf_bias_table *t = new (std::nothrow) jf_bias_table;
   if (!t) return fail(JF_ERR_NO_MEMORY, "bias table allocation failed");
   t->vocabulary = vocabulary;

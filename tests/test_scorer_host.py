@@ -177,3 +177,16 @@ def test_tables_of_another_device_are_refused():
         for table in penalties:
             h.lib.fake_penalty_table_free(table)
         h.lib.jf_bias_table_destroy(biases)
+
+
+@pytest.mark.parametrize("vocabulary", [524289, 2 ** 32 - 2048, 2 ** 32 - 2047, 2 ** 32 - 1])
+def test_bias_tables_take_no_larger_vocabulary_than_scorers(vocabulary):
+    """Near 2^32 the number of a row's buckets wrapped to none, and setting a row
+    then counted past a vector of one."""
+    with Host() as h:
+        table = vp(1)
+        rc = h.lib.jf_bias_table_create(vocabulary, 1, 1, ctypes.byref(table))
+        h.refused(rc, J.JF_ERR_INVALID_ARGUMENT, "524288 tokens")
+        assert not table.value and not h.log()
+        assert h.lib.jf_bias_table_create(524288, 1, 1, ctypes.byref(table)) == 0
+        h.lib.jf_bias_table_destroy(table)
