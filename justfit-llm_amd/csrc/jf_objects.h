@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cstdint>
 #include <cstring>
 #include <string>
 #include <vector>
@@ -154,6 +155,8 @@ template <class T>
 int device_alloc(T **p, size_t count, const char *what) {
   *p = nullptr;
   if (!count) return JF_OK;
+  if (count > SIZE_MAX / sizeof(T))
+    return fail(JF_ERR_NO_MEMORY, std::string(what) + ": more bytes than 64 bits count");
   JF_HIP(hipMalloc((void **)p, count * sizeof(T)), what);
   return JF_OK;
 }

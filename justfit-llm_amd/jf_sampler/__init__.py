@@ -15,6 +15,7 @@ JF_OK = 0
 JF_ERR_INVALID_ARGUMENT = 1
 JF_ERR_LOGIC = 2
 JF_ERR_DEVICE = 3
+JF_ERR_NO_MEMORY = 4
 JF_NO_TOKEN = 0xFFFFFFFF
 JF_DTYPE_F32 = 0
 JF_DTYPE_BF16 = 1

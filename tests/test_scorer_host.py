@@ -190,3 +190,13 @@ def test_bias_tables_take_no_larger_vocabulary_than_scorers(vocabulary):
         assert not table.value and not h.log()
         assert h.lib.jf_bias_table_create(524288, 1, 1, ctypes.byref(table)) == 0
         h.lib.jf_bias_table_destroy(table)
+
+
+def test_a_bias_table_whose_bytes_pass_64_bits_is_out_of_memory():
+    """2^30 + 1 rows of 2^31 - 1 entries are 2^64 bytes and a few: a table of a few
+    bytes was made."""
+    with Host() as h:
+        table = vp(1)
+        rc = h.lib.jf_bias_table_create(1, (1 << 30) + 1, (1 << 31) - 1, ctypes.byref(table))
+        h.refused(rc, J.JF_ERR_NO_MEMORY, "bias entries")
+        assert not table.value and not h.log()
