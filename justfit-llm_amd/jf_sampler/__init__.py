@@ -680,6 +680,25 @@ def _plain(t, shape, what, floating):
     return _device(t, what)
 
 
+def _check_extra_tokens(t, policies, counts, offsets, stride):
+    """That a tensor of extra tokens holds what the penalized rows take of it,
+    rows by flat places from its first element. Counts and places that the
+    library refuses are left to it."""
+    import torch
+    end = 0
+    for r, p in enumerate(policies):
+        count = int(counts[r])
+        first = (int(offsets[r]) if offsets is not None else r * stride) % 2 ** 64
+        if ((p.repetition != 1 or p.presence != 0 or p.frequency != 0) and 0 < count <= 16
+                and first <= 0xFFFFFFFF - 16):
+            end = max(end, first + count)
+    held = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else 0
+    if end and t.dtype not in (torch.int32, torch.uint32):
+        raise ValueError(f"extra tokens hold {t.dtype}")
+    if end > held:
+        raise ValueError(f"extra tokens of shape {tuple(t.shape)} end before the rows' do")
+
+
 class Scorer:
     """jf_scorer: processed logits, log-probabilities and distillation over
     one vocabulary, up to max_rows rows a call. The *_args methods check
@@ -741,6 +760,8 @@ class Scorer:
                 arr = (ctype * rows)(*[int(v) for v in values])
                 setattr(a, name, arr)
                 keep.append(arr)
+        if extra_tokens is not None and extra_counts is not None:
+            _check_extra_tokens(extra_tokens, pol, extra_counts, extra_offsets, extra_stride)
         return a, keep
 
     def launch_process(self, a, stream=None):
