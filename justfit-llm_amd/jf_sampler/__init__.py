@@ -721,6 +721,7 @@ class Scorer:
                      biases=None, bias_rows=None):
         """Builds a JfProcessArgs (kept-alive host arrays ride along). bias_rows:
         the bias table's row of each row, None for a row without biases."""
+        import torch
         rows = logits.shape[0]
         a = JfProcessArgs()
         a.rows = rows
@@ -730,7 +731,9 @@ class Scorer:
         a.out_stride = out.stride(0)
         if masks is not None:
             used = rows if mask_rows is None else max(mask_rows) + 1
-            if (masks.dim() != 2 or masks.element_size() != 4 or masks.stride(1) != 1
+            if masks.dtype not in (torch.int32, torch.uint32):
+                raise ValueError(f"masks hold {masks.dtype}")
+            if (masks.dim() != 2 or masks.stride(1) != 1
                     or masks.shape[0] < used or masks.shape[1] * 32 < self.vocabulary
                     or (mask_rows is not None and min(mask_rows) < 0)):
                 raise ValueError(f"masks of shape {tuple(masks.shape)} do not cover the rows")

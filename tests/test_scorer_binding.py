@@ -75,3 +75,12 @@ def test_extra_tokens_that_no_row_reads():
     extras(none, policies=[J.policy()] * ROWS, extra_counts=[9] * ROWS, extra_stride=16)
     for counts, offsets in (([17, 0, 0], None), ([0, 0, 1], [0, 0, 1 << 32]), ([0, -1, 0], None)):
         extras(none, extra_counts=counts, extra_offsets=offsets, extra_stride=16)
+
+
+def test_masks_are_32_bit_words():
+    x = on(torch.zeros((ROWS, V)))
+    for dtype in (torch.float32, torch.int64, torch.int16):
+        with pytest.raises(ValueError, match="masks"):
+            scorer().process_args(x, PENALIZED, x, masks=on(torch.zeros((ROWS, 8), dtype=dtype)))
+    for dtype in (torch.int32, torch.uint32):
+        scorer().process_args(x, PENALIZED, x, masks=on(torch.zeros((ROWS, 4), dtype=dtype)))
