@@ -652,34 +652,6 @@ def _dtype(t, what):
     raise ValueError(f"{what} are f32 or bf16, not {t.dtype}")
 
 
-def _device(t, what):
-    """The address of a tensor in device memory."""
-    if not t.is_cuda:
-        raise ValueError(f"{what} are on {t.device}, not on the GPU")
-    return t.data_ptr()
-
-
-def _rows(t, vocabulary, rows, what):
-    """The address of a [rows, vocabulary] tensor of contiguous rows."""
-    if t.dim() != 2 or t.shape[1] != vocabulary or (rows is not None and t.shape[0] != rows):
-        raise ValueError(f"{what} have shape {tuple(t.shape)}")
-    if vocabulary > 1 and t.stride(1) != 1:
-        raise ValueError(f"{what} have no contiguous rows")
-    return _device(t, what)
-
-
-def _plain(t, shape, what, floating):
-    """The address of an optional contiguous f32 (or 32-bit id) tensor."""
-    import torch
-    if t is None:
-        return None
-    if tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{what} is no contiguous tensor of shape {shape}")
-    if t.dtype not in ((torch.float32,) if floating else (torch.int32, torch.uint32)):
-        raise ValueError(f"{what} holds {t.dtype}")
-    return _device(t, what)
-
-
 def _check_extra_tokens(t, policies, counts, offsets, stride):
     """That a tensor of extra tokens holds what the penalized rows take of it,
     rows by flat places from its first element. Counts and places that the
@@ -706,14 +678,44 @@ class Scorer:
     addresses, so its tensors have to outlive it (host arrays ride along)."""
 
     def __init__(self, vocabulary, max_rows):
+        import torch
         h = c_vp()
         check(lib().jf_scorer_create(vocabulary, max_rows, ctypes.byref(h)))
         self.handle = h
         self.vocabulary = vocabulary
         self.max_rows = max_rows
+        self.device = torch.cuda.current_device()
 
     def workspace_bytes(self):
         return lib().jf_scorer_workspace_bytes(self.handle)
+
+    def _device(self, t, what):
+        """The address of a tensor in the scorer's device memory."""
+        if not t.is_cuda:
+            raise ValueError(f"{what} are on {t.device}, not on the GPU")
+        if t.get_device() != self.device:
+            raise ValueError(f"{what} are on {t.device}, not on cuda:{self.device}")
+        return t.data_ptr()
+
+    def _rows(self, t, rows, what):
+        """The address of a [rows, vocabulary] tensor of contiguous rows."""
+        if t.dim() != 2 or t.shape[1] != self.vocabulary or (rows is not None
+                                                             and t.shape[0] != rows):
+            raise ValueError(f"{what} have shape {tuple(t.shape)}")
+        if self.vocabulary > 1 and t.stride(1) != 1:
+            raise ValueError(f"{what} have no contiguous rows")
+        return self._device(t, what)
+
+    def _plain(self, t, shape, what, floating):
+        """The address of an optional contiguous f32 (or 32-bit id) tensor."""
+        import torch
+        if t is None:
+            return None
+        if tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{what} is no contiguous tensor of shape {shape}")
+        if t.dtype not in ((torch.float32,) if floating else (torch.int32, torch.uint32)):
+            raise ValueError(f"{what} holds {t.dtype}")
+        return self._device(t, what)
 
     def process_args(self, logits, policies, out, *, masks=None, mask_rows=None,
                      stop_tokens=(JF_NO_TOKEN, JF_NO_TOKEN), penalties=None, penalty_rows=None,
@@ -726,8 +728,8 @@ class Scorer:
         a = JfProcessArgs()
         a.rows = rows
         a.dtype, a.out_dtype = _dtype(logits, "logits"), _dtype(out, "processed logits")
-        a.logits, a.logits_stride = _rows(logits, self.vocabulary, None, "logits"), logits.stride(0)
-        a.out = _rows(out, self.vocabulary, rows, "processed logits")
+        a.logits, a.logits_stride = self._rows(logits, None, "logits"), logits.stride(0)
+        a.out = self._rows(out, rows, "processed logits")
         a.out_stride = out.stride(0)
         if masks is not None:
             used = rows if mask_rows is None else max(mask_rows) + 1
@@ -737,7 +739,7 @@ class Scorer:
                     or masks.shape[0] < used or masks.shape[1] * 32 < self.vocabulary
                     or (mask_rows is not None and min(mask_rows) < 0)):
                 raise ValueError(f"masks of shape {tuple(masks.shape)} do not cover the rows")
-            a.masks = _device(masks, "masks")
+            a.masks = self._device(masks, "masks")
             a.mask_stride = masks.stride(0)
         pol = (JfPolicy * rows)(*policies)
         a.policies = pol
@@ -746,7 +748,7 @@ class Scorer:
         if penalties is not None:
             a.penalties = penalties.handle
         if extra_tokens is not None:
-            a.extra_tokens = _device(extra_tokens, "extra tokens")
+            a.extra_tokens = self._device(extra_tokens, "extra tokens")
             a.extra_stride = extra_stride
         if biases is not None:
             a.biases = biases.handle
@@ -783,19 +785,19 @@ class Scorer:
         rows = logits.shape[0]
         a = JfLogprobsArgs()
         a.rows, a.dtype = rows, _dtype(logits, "logits")
-        a.logits, a.logits_stride = _rows(logits, self.vocabulary, None, "logits"), logits.stride(0)
-        a.temperatures = _plain(temperatures, (rows,), "temperatures", True)
+        a.logits, a.logits_stride = self._rows(logits, None, "logits"), logits.stride(0)
+        a.temperatures = self._plain(temperatures, (rows,), "temperatures", True)
         if tokens is not None:
             a.token_count = tokens.shape[1]
-            a.tokens = _plain(tokens, (rows, a.token_count), "tokens", False)
+            a.tokens = self._plain(tokens, (rows, a.token_count), "tokens", False)
             a.token_stride = a.token_count
-        a.out_logprobs = _plain(logprobs, (rows, a.token_count), "logprobs", True)
-        a.out_lse = _plain(lse, (rows,), "lse", True)
-        a.out_ranks = _plain(ranks, (rows,), "ranks", False)
+        a.out_logprobs = self._plain(logprobs, (rows, a.token_count), "logprobs", True)
+        a.out_lse = self._plain(lse, (rows,), "lse", True)
+        a.out_ranks = self._plain(ranks, (rows,), "ranks", False)
         if top_ids is not None:
             a.top = top_ids.shape[1]
-            a.out_top_ids = _plain(top_ids, (rows, a.top), "top_ids", False)
-        a.out_top_logprobs = _plain(top_logprobs, (rows, a.top), "top_logprobs", True)
+            a.out_top_ids = self._plain(top_ids, (rows, a.top), "top_ids", False)
+        a.out_top_logprobs = self._plain(top_logprobs, (rows, a.top), "top_logprobs", True)
         return a
 
     def launch_logprobs(self, a, stream=None):
@@ -814,24 +816,24 @@ class Scorer:
         rows, k = teacher_ids.shape
         a = JfDistillArgs()
         a.rows, a.dtype = rows, _dtype(logits, "logits")
-        a.logits, a.logits_stride = _rows(logits, self.vocabulary, rows, "logits"), logits.stride(0)
+        a.logits, a.logits_stride = self._rows(logits, rows, "logits"), logits.stride(0)
         a.temperature, a.normalize = temperature, 1 if normalize else 0
-        a.teacher_ids = _plain(teacher_ids, (rows, k), "teacher_ids", False)
-        a.teacher_values = _plain(teacher_values, (rows, k), "teacher_values", True)
+        a.teacher_ids = self._plain(teacher_ids, (rows, k), "teacher_ids", False)
+        a.teacher_values = self._plain(teacher_values, (rows, k), "teacher_values", True)
         a.teacher_stride = a.teacher_count = k
-        a.out_loss = _plain(loss, (rows,), "loss", True)
-        a.out_lse = _plain(lse, (rows,), "lse", True)
-        a.saved = _plain(saved, (rows, 2 + k), "saved", True)
+        a.out_loss = self._plain(loss, (rows,), "loss", True)
+        a.out_lse = self._plain(lse, (rows,), "lse", True)
+        a.saved = self._plain(saved, (rows, 2 + k), "saved", True)
         if grad_loss is not None:
             import torch
             if tuple(grad_loss.shape) != (rows,) or grad_loss.dtype != torch.float32:
                 raise ValueError(f"grad_loss is no f32 tensor of {rows} rows")
-            a.grad_loss = _device(grad_loss, "loss gradients")
+            a.grad_loss = self._device(grad_loss, "loss gradients")
             a.grad_loss_stride = grad_loss.stride(0)
         if grad is not None:
             if grad.dtype != logits.dtype:
                 raise ValueError("gradients have the logits' dtype")
-            a.grad, a.grad_stride = _rows(grad, self.vocabulary, rows, "gradients"), grad.stride(0)
+            a.grad, a.grad_stride = self._rows(grad, rows, "gradients"), grad.stride(0)
         return a
 
     def launch_distill(self, a, stream=None):

@@ -84,3 +84,28 @@ def test_masks_are_32_bit_words():
             scorer().process_args(x, PENALIZED, x, masks=on(torch.zeros((ROWS, 8), dtype=dtype)))
     for dtype in (torch.int32, torch.uint32):
         scorer().process_args(x, PENALIZED, x, masks=on(torch.zeros((ROWS, 4), dtype=dtype)))
+
+
+def test_tensors_are_on_the_scorers_gpu():
+    """A tensor of another GPU: its address means nothing on the scorer's, and a
+    trainer's current stream there is not the one that the tensor's work is on."""
+    def t(*shape, dtype=torch.float32):
+        return on(torch.zeros(shape, dtype=dtype))
+    i32 = torch.int32
+    x, ids, values = t(ROWS, V), t(ROWS, 2, dtype=i32), t(ROWS, 2)
+    s = scorer()
+    calls = ((s.process_args, dict(logits=x, policies=PENALIZED, out=x, masks=t(ROWS, 4, dtype=i32),
+                                   extra_tokens=t(8, dtype=i32))),
+             (s.logprobs_args, dict(logits=x, tokens=ids, temperatures=t(ROWS), lse=t(ROWS),
+                                    logprobs=values, ranks=t(ROWS, dtype=i32), top_ids=ids,
+                                    top_logprobs=values)),
+             (s.distill_args, dict(logits=x, teacher_ids=ids, teacher_values=values, loss=t(ROWS),
+                                   lse=t(ROWS), saved=t(ROWS, 4), grad_loss=t(ROWS), grad=x)))
+    for build, kw in calls:
+        build(**kw)
+        for name, value in kw.items():
+            if torch.is_tensor(value):
+                with pytest.raises(ValueError, match="cuda:1, not on cuda:0"):
+                    build(**dict(kw, **{name: on(value.clone(), 1)}))
+                with pytest.raises(ValueError, match="not on the GPU"):
+                    build(**dict(kw, **{name: torch.zeros(value.shape, dtype=value.dtype)}))
