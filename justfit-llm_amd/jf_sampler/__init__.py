@@ -660,7 +660,7 @@ def _check_extra_tokens(t, policies, counts, offsets, stride):
     end = 0
     for r, p in enumerate(policies):
         count = int(counts[r])
-        first = (int(offsets[r]) if offsets is not None else r * stride) % 2 ** 64
+        first = (int(offsets[r]) if offsets is not None else r * int(stride)) % 2 ** 64
         if ((p.repetition != 1 or p.presence != 0 or p.frequency != 0) and 0 < count <= 16
                 and first <= 0xFFFFFFFF - 16):
             end = max(end, first + count)

@@ -109,3 +109,12 @@ def test_tensors_are_on_the_scorers_gpu():
                     build(**dict(kw, **{name: on(value.clone(), 1)}))
                 with pytest.raises(ValueError, match="not on the GPU"):
                     build(**dict(kw, **{name: torch.zeros(value.shape, dtype=value.dtype)}))
+
+
+def test_numpy_counts_offsets_and_strides():
+    import numpy as np
+    tokens = on(torch.zeros(8, dtype=torch.int32))
+    extras(tokens, extra_counts=np.array([1, 0, 2]), extra_stride=np.int64(2))
+    extras(tokens, extra_counts=np.array([1, 0, 2]), extra_offsets=np.array([0, 0, 6]))
+    with pytest.raises(ValueError, match="extra tokens"):
+        extras(tokens, extra_counts=np.array([1, 0, 2]), extra_stride=np.int64(4))
