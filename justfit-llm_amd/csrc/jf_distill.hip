@@ -67,19 +67,20 @@ struct Teacher {
       logit[i] = valid[i] ? logit_value(x[id[i]]) : 0.0f;
     }
     keep_first(holder);
-    float first = -__builtin_inff();
+    float most = -__builtin_inff();
 #pragma unroll
     for (uint32_t i = 0; i < SLOTS; ++i) {
       log_p[i] = valid[i] ? value[i] : -__builtin_inff();
-      if (a.normalize) log_p[i] *= inv_t;
-      first = __builtin_fmaxf(first, log_p[i]);
+      most = __builtin_fmaxf(most, log_p[i]);
     }
     if (a.normalize) {
-      first = finite_reference(wave_max_f32(first));
+      // Apart from the largest before the scale: their common offset costs no
+      // bits, and u / T may pass the range.
+      most = finite_reference(wave_max_f32(most));
       float sum = 0.0f;
 #pragma unroll
       for (uint32_t i = 0; i < SLOTS; ++i) {
-        log_p[i] -= first;
+        log_p[i] = (log_p[i] - most) * inv_t;
         sum += expf(log_p[i]);
       }
       sum = logf(wave_sum_f32(sum));
