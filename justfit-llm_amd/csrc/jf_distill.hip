@@ -305,7 +305,7 @@ __global__ __launch_bounds__(kStepThreads, 4) void distill_step_kernel(ScoreLaun
   if (wave == 0 && scale != 0.0f) {
 #pragma unroll
     for (uint32_t i = 0; i < SLOTS; ++i)
-      if (t.valid[i]) grad[t.id[i]] = logit_of<DT>(pulled(t.logit[i]) - scale * t.p[i]);
+      if (!(t.p[i] <= 0.0f)) grad[t.id[i]] = logit_of<DT>(pulled(t.logit[i]) - scale * t.p[i]);
   }
 }
 
@@ -342,7 +342,8 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillGradLaunch a) 
     const uint32_t id = a.teacher_ids[(uint64_t)row * a.teacher_stride + tid];
     const uint32_t at = id + before - base;
     const float p = saved[2 + tid];
-    if (at < CHUNK && id < a.vocabulary && p >= 0.0f) {
+    // A token of no probability has no share, also of a gradient that is not finite.
+    if (at < CHUNK && id < a.vocabulary && !(p <= 0.0f)) {
       share[tid] = scale * p;
       slot[at] = (uint8_t)tid;
       atomicOr(&listed[at >> 5], 1u << (at & 31u));

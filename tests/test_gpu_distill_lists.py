@@ -101,3 +101,38 @@ def test_lists_without_mass():
     np.testing.assert_array_equal(p[1], [0, 1])
     assert abs(loss[1] - np.log(50)) <= 64 * U * np.log(50)
     assert np.isnan(loss[2]) and np.isnan(grad[2]).all()
+
+
+@pytest.mark.parametrize("V", [3000, 80003])
+@pytest.mark.parametrize("g", [np.nan, np.inf, -np.inf, 2.0])
+@pytest.mark.parametrize("mode", ["separate", "step"])
+def test_tokens_without_probability_have_no_share_of_the_loss_gradient(V, g, mode):
+    """No slot of rows 0 and 1 has probability: no gradient, whatever comes in. In
+    row 2 one has: the others' gradients are g / T times q, as any token's.
+    Short rows by whole rows, long ones by chunks."""
+    rng = np.random.default_rng(4)
+    z = rng.normal(0, 1, (3, V)).astype(np.float32)
+    ids = np.tile([5, 70, V - 1], (3, 1))
+    values = np.float32([[-np.inf] * 3, [-np.inf, -300, -np.inf], [-1, -np.inf, -np.inf]])
+    import torch
+    t, _ = device_rows(z, "f32")
+    loss, saved = torch.full((3,), 7.0).cuda(), torch.full((3, 5), 7.0).cuda()
+    grad, gl = torch.full((3, V), 7.0).cuda(), torch.full((3,), g).cuda()
+    d_ids, d_values = torch.from_numpy(ids.astype(np.int32)).cuda(), torch.from_numpy(values).cuda()
+    s = J.Scorer(V, 3)
+    kw = dict(normalize=False, saved=saved)
+    if mode == "step":
+        s.launch_distill_step(s.distill_args(t, d_ids, d_values, loss=loss, grad_loss=gl,
+                                             grad=grad, **kw))
+    else:
+        s.launch_distill(s.distill_args(t, d_ids, d_values, loss=loss, **kw))
+        s.launch_distill_backward(s.distill_args(t, d_ids, None, grad_loss=gl, grad=grad, **kw))
+    got = host(grad)
+    assert not host(loss)[:2].any() and not got[:2].any()
+    if g == 2.0:
+        _, want, _, bound = distill_plain(z[2], ids[2], values[2], 1.0, False)
+        assert np.all(np.abs(got[2] - 2 * want) <= 2 * bound + 8 * U * np.abs(want))
+    else:
+        # The listed token takes g (q - p), inf - inf in the order it is worked out in.
+        np.testing.assert_array_equal(np.delete(got[2], 5), np.full(V - 1, g))
+    s.close()
