@@ -49,3 +49,24 @@ def test_list_buffers_may_be_filled_anew_before_the_backward_pass(normalize, ref
             assert abs(float(loss[r]) - want_loss) <= loss_bound + U * abs(want_loss)
             assert np.all(excess(got[r], grad, bound + 4 * U * np.abs(grad) + 1e-37, "f32") <= 1)
     s.close()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_an_empty_batch_has_no_losses_and_an_empty_gradient(dtype):
+    """A packed batch none of whose tokens is trained on."""
+    import torch
+    from jf_sampler.train import distill_loss
+    V, K = 500, 4
+    s = J.Scorer(V, 8)
+    leaf = torch.randn((3, V), device="cuda", dtype=getattr(torch, dtype)).requires_grad_(True)
+    ids, values = torch.zeros((0, K), dtype=torch.int32).cuda(), torch.zeros((0, K)).cuda()
+    loss = distill_loss(s, leaf[:0], ids, values)
+    assert loss.shape == (0,) and loss.dtype == torch.float32 and loss.is_cuda
+    loss.sum().backward()
+    assert leaf.grad.shape == (3, V) and leaf.grad.dtype == leaf.dtype and not leaf.grad.any()
+    # Its tensors are looked at all the same.
+    for bad in ((leaf[:0, :9], ids, values), (leaf[:1], ids, values), (leaf[:0], ids.long(), values),
+                (leaf[:0], ids, values[:, :2]), (leaf[:0], ids[:, :0], values[:, :0])):
+        with pytest.raises(ValueError):
+            distill_loss(s, *bad)
+    s.close()
