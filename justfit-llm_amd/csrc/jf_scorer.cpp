@@ -67,7 +67,7 @@ struct jf_scorer {
   uint32_t max_rows = 0;
   int device = 0;
   jf::ProcessRow *rows = nullptr;  // [max_rows]
-  float2 *partials = nullptr;      // a chunk each, row by row
+  float2 *partials = nullptr;      // a chunk each, row by row, of one launch
   uint32_t *aheads = nullptr;      // likewise
   float *maxima = nullptr;         // those of min(max_rows, kTopRows) rows' chunks
   float *saved = nullptr;          // [min(max_rows, kSavedRows)][2 + kTeacherTokens]
@@ -213,8 +213,9 @@ int jf_scorer_create(uint32_t vocabulary, uint32_t max_rows, jf_scorer **out) {
   int rc = JF_OK;
   const hipError_t e = hipGetDevice(&s->device);
   if (e != hipSuccess) rc = hip_fail(e, "hipGetDevice");
-  // The rows' blocks and groups, whatever the chunk.
-  const uint64_t parts = (uint64_t)max_rows * blocks_of(vocabulary, kLeastChunk);
+  // The blocks and groups of one launch's rows, whatever the chunk.
+  const uint64_t parts = (uint64_t)std::min(max_rows, launch_rows(vocabulary)) *
+                         blocks_of(vocabulary, kLeastChunk);
   const uint64_t maxima = (uint64_t)std::min(max_rows, jf::kTopRows) *
                           blocks_of(vocabulary, kMostChunk) * (kMostChunk / jf::kScoreGroup);
   const uint64_t saved = (uint64_t)std::min(max_rows, kSavedRows) * (2 + jf::kTeacherTokens);

@@ -200,3 +200,65 @@ def test_a_bias_table_whose_bytes_pass_64_bits_is_out_of_memory():
         rc = h.lib.jf_bias_table_create(1, (1 << 30) + 1, (1 << 31) - 1, ctypes.byref(table))
         h.refused(rc, J.JF_ERR_NO_MEMORY, "bias entries")
         assert not table.value and not h.log()
+
+
+def scratch(h):
+    """{address: bytes} of the scorer's device memory."""
+    return {e["at"]: e["bytes"] for e in h.created if e["what"] == "malloc"}
+
+
+def score(h, rows, dtype=0, top=0):
+    a = J.JfLogprobsArgs()
+    a.rows, a.dtype, a.logits, a.logits_stride = rows, dtype, LOGITS, h.vocabulary
+    a.out_lse = OUT
+    if top:
+        a.top, a.out_top_ids, a.out_top_logprobs = top, OUT, OUT
+    assert h.lib.jf_logprobs(h.scorer, ctypes.byref(a), STREAM) == 0
+    return h.log()
+
+
+def distill(h, rows, dtype=0, call="jf_distill_step", saved=None):
+    a = J.JfDistillArgs()
+    a.rows, a.dtype, a.logits, a.logits_stride = rows, dtype, LOGITS, h.vocabulary
+    a.temperature, a.teacher_ids, a.teacher_values = 1.0, MASKS, MASKS
+    a.teacher_stride = a.teacher_count = 256
+    a.out_loss, a.grad_loss, a.grad, a.grad_stride = OUT, OUT, OUT, h.vocabulary
+    a.saved = saved
+    assert getattr(h.lib, call)(h.scorer, ctypes.byref(a), STREAM) == 0
+    return h.log()
+
+
+@pytest.mark.parametrize("vocabulary", [1, 3, 2048, 2049, 32000, 73728, 73729, 151936, 262144,
+                                        524288])
+def test_scratch_holds_what_every_launch_takes(vocabulary):
+    for max_rows in (1, 5, 111, 112, 409, 513, 65536, 4194304):
+        with Host(vocabulary, max_rows) as h:
+            held = scratch(h)
+            for rows in sorted({1, 2, 100, 111, 112, 148, 296, 408, 409, 512, 513, 20000, 55189,
+                                max_rows}):
+                if rows > max_rows:
+                    continue
+                for dtype in (0, 1):
+                    for log in (score(h, rows, dtype), score(h, rows, dtype, top=128),
+                                distill(h, rows, dtype), distill(h, rows, dtype, "jf_distill")):
+                        for e in log:
+                            if "segments" in e:
+                                parts = e["row_count"] * e["segments"]
+                                assert 8 * parts <= held[e["partials"]], (max_rows, rows, e)
+                                assert 4 * parts <= held[e["aheads"]], (max_rows, rows, e)
+                                if e["top"]:
+                                    assert 4 * e["row_count"] * e["groups"] <= held[e["maxima"]]
+                            if e["what"] in ("loss", "grad") and e["saved"]:
+                                assert 4 * e["row_count"] * 258 <= held[e["saved"]], (max_rows, e)
+
+
+def test_scratch_of_rows_is_that_of_one_launch():
+    """Its launches follow one another on the same parts. One launch over 151,936
+    tokens takes 55,188 rows at most, in chunks of at least 2,048 tokens."""
+    with Host(151936, 4194304) as h:
+        parts = 55188 * 75
+        sizes = sorted(scratch(h).values())
+        assert sizes.count(8 * parts) == 1 and sizes.count(4 * parts) == 1
+        assert max(score(h, 4194304), key=lambda e: e["row_count"])["row_count"] == 55188
+    with Host(1000, 8) as h:
+        assert {8 * 8, 4 * 8} <= set(scratch(h).values())
