@@ -30,14 +30,27 @@ constexpr uint64_t kMaxTokens = 1ull << 33;
 constexpr uint32_t kLeastChunk = jf::chunk_tokens(JF_DTYPE_F32, 2);
 constexpr uint32_t kMostChunk = jf::chunk_tokens(JF_DTYPE_BF16, 4);
 uint32_t blocks_of(uint32_t vocabulary, uint32_t chunk) { return (vocabulary + chunk - 1) / chunk; }
-// Rows of one training step's launches at most where the scorer holds what the
-// forward pass saves.
-constexpr uint32_t kSavedRows = 65536;
 // Rows of one launch at most.
 uint32_t launch_rows(uint32_t vocabulary) {
   return (uint32_t)(kMaxTokens / ((uint64_t)blocks_of(vocabulary, kMostChunk) * kMostChunk));
 }
 size_t element_size(uint32_t dtype) { return dtype == JF_DTYPE_F32 ? 4 : 2; }
+
+// The rows from which a training step takes them whole, a block each, in one
+// launch. A short row is done before three launches would be (72,256 tokens, one
+// bf16 row 11.1 us against 11.5, 64 rows 12.0 against 13.1, 512 rows 27 against 41).
+// A long one keeps its block busy longer than the rows' chunks spread over the GPU
+// take (100,003 f32, one row 14.6 against 11.6; 151,936 bf16, 64 rows 21.5 against
+// 15.8), unless rows keep nearly half of the CUs busy (96 rows 22.1 against 20.0,
+// 128 rows 23.1 against 24.5) or, of the longest, most (248,320 f32, 128 rows 65.2
+// against 60.7, 192 rows 105.6 against 92.9; bf16, 128 rows 34.9 against 35.6).
+uint32_t whole_rows(uint32_t vocabulary, uint32_t dtype) {
+  const uint32_t row_bytes = vocabulary * (uint32_t)element_size(dtype);
+  return vocabulary <= 72u << 10 ? 1 : std::max(112u, row_bytes / 5120);
+}
+// Those of steps by chunks at most: the scorer holds what their forward pass saves
+// where the caller does not.
+uint32_t chunked_rows(uint32_t vocabulary) { return whole_rows(vocabulary, JF_DTYPE_F32) - 1; }
 
 const void *rows_at(const void *p, uint64_t row, uint64_t stride, uint32_t dtype) {
   return (const uint8_t *)p + row * stride * element_size(dtype);
@@ -70,7 +83,7 @@ struct jf_scorer {
   float2 *partials = nullptr;      // a chunk each, row by row, of one launch
   uint32_t *aheads = nullptr;      // likewise
   float *maxima = nullptr;         // those of min(max_rows, kTopRows) rows' chunks
-  float *saved = nullptr;          // [min(max_rows, kSavedRows)][2 + kTeacherTokens]
+  float *saved = nullptr;          // [min(max_rows, chunked_rows)][2 + kTeacherTokens]
   uint64_t workspace_bytes = 0;
   std::vector<jf::ProcessRow> last_rows;  // what the device's rows hold
   std::vector<jf::ProcessRow> host_rows;  // the call's rows, reused across calls
@@ -218,7 +231,8 @@ int jf_scorer_create(uint32_t vocabulary, uint32_t max_rows, jf_scorer **out) {
                          blocks_of(vocabulary, kLeastChunk);
   const uint64_t maxima = (uint64_t)std::min(max_rows, jf::kTopRows) *
                           blocks_of(vocabulary, kMostChunk) * (kMostChunk / jf::kScoreGroup);
-  const uint64_t saved = (uint64_t)std::min(max_rows, kSavedRows) * (2 + jf::kTeacherTokens);
+  const uint64_t saved =
+      (uint64_t)std::min(max_rows, chunked_rows(vocabulary)) * (2 + jf::kTeacherTokens);
   if (rc == JF_OK) rc = device_alloc(&s->rows, max_rows, "row records");
   if (rc == JF_OK) rc = device_alloc(&s->partials, parts, "row partials");
   if (rc == JF_OK) rc = device_alloc(&s->aheads, parts, "rank partials");
@@ -513,19 +527,6 @@ static int check_distill(const jf_scorer *s, const jf_distill_args *a, bool forw
   return JF_OK;
 }
 
-// Whether a training step takes its rows whole, a block each, in one launch. A
-// short row is done before three launches would be (72,256 tokens, one bf16 row
-// 11.1 us against 11.5, 64 rows 12.0 against 13.1, 512 rows 27 against 41). A long
-// one keeps its block busy longer than the rows' chunks spread over the GPU take
-// (100,003 f32, one row 14.6 against 11.6; 151,936 bf16, 64 rows 21.5 against
-// 15.8), unless rows keep nearly half of the CUs busy (96 rows 22.1 against 20.0,
-// 128 rows 23.1 against 24.5) or, of the longest, most (248,320 f32, 128 rows 65.2
-// against 60.7, 192 rows 105.6 against 92.9; bf16, 128 rows 34.9 against 35.6).
-static bool whole_rows(uint32_t rows, uint32_t vocabulary, uint32_t dtype) {
-  const size_t row_bytes = vocabulary * element_size(dtype);
-  return vocabulary <= 72u << 10 || rows >= std::max<size_t>(112, row_bytes / 5120);
-}
-
 static int distill(jf_scorer *s, const jf_distill_args *a, bool forward, bool backward,
                    void *stream) {
   if (!s || !a) return fail(JF_ERR_INVALID_ARGUMENT, "null scorer or arguments");
@@ -534,8 +535,7 @@ static int distill(jf_scorer *s, const jf_distill_args *a, bool forward, bool ba
   const uint64_t stride = a->rows > 1 ? a->logits_stride : s->vocabulary;
   const uint64_t grad_stride = a->rows > 1 ? a->grad_stride : s->vocabulary;
   const uint32_t K = a->teacher_count;
-  uint32_t most = launch_rows(s->vocabulary);
-  if (forward && backward && !a->saved) most = std::min(most, kSavedRows);
+  const uint32_t most = launch_rows(s->vocabulary);
   for (uint32_t r = 0; r < a->rows; r += most) {
     const uint32_t n = std::min(most, a->rows - r);
     float *saved = a->saved ? a->saved + (uint64_t)r * (2 + K) : backward ? s->saved : nullptr;
@@ -565,7 +565,7 @@ static int distill(jf_scorer *s, const jf_distill_args *a, bool forward, bool ba
       G.grad_loss_stride = a->grad_loss_stride;
     }
     int e = hipSuccess;
-    if (forward && backward && whole_rows(n, s->vocabulary, a->dtype)) {
+    if (forward && backward && n >= whole_rows(s->vocabulary, a->dtype)) {
       L.saved = a->saved ? saved : nullptr;
       e = jf::launch_distill_step(L, G, a->dtype, stream);
     } else {

@@ -262,3 +262,30 @@ def test_scratch_of_rows_is_that_of_one_launch():
         assert max(score(h, 4194304), key=lambda e: e["row_count"])["row_count"] == 55188
     with Host(1000, 8) as h:
         assert {8 * 8, 4 * 8} <= set(scratch(h).values())
+
+
+def test_distillation_records_are_those_of_steps_by_chunks():
+    """Only steps of fewer rows than are taken whole keep them in the scorer: none
+    of short rows, fewer than 112 or a row's f32 bytes / 5120 of long ones."""
+    for vocabulary, rows in ((1000, 0), (73728, 0), (73729, 111), (151936, 117), (524288, 408)):
+        for max_rows in (5, 4194304):
+            with Host(vocabulary, max_rows) as h:
+                size = min(rows, max_rows) * 258 * 4
+                held = scratch(h)
+                saved = {e["saved"] for n in range(1, min(rows, max_rows) + 1)
+                         for e in distill(h, n) if e["what"] == "grad"}
+                assert [held[at] for at in saved] == [size] * bool(rows)
+                # That is all: rows, parts and maxima beside it.
+                used = {e[name] for log in (score(h, 1, top=1), h.process([PLAIN])[1]) for e in log
+                        for name in ("rows", "partials", "aheads", "maxima") if name in e}
+                assert set(held) == used | saved
+                h.lib.jf_scorer_workspace_bytes.restype = ctypes.c_uint64
+                assert h.lib.jf_scorer_workspace_bytes(h.scorer) == sum(held.values())
+
+
+def test_steps_of_whole_rows_are_one_launch():
+    with Host(1000, 200000) as h:
+        assert [e["row_count"] for e in distill(h, 200000)] == [200000]
+    with Host(151936, 200000) as h:
+        assert [(e["what"], e["row_count"]) for e in distill(h, 55188 + 117)] == [
+            ("step", 55188), ("score", 117), ("loss", 117), ("grad", 117)]
