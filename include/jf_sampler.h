@@ -577,7 +577,8 @@ int jf_scorer_destroy(jf_scorer *scorer);
 uint64_t jf_scorer_workspace_bytes(const jf_scorer *scorer);
 
 /* Requests' logit biases on the device, one row a request, each of at most
- * max_entries distinct tokens of a scorer's vocabulary. A bias is finite, or -infinity for a ban. */
+ * max_entries distinct tokens of a scorer's vocabulary. A bias is finite, or
+ * -infinity for a ban. */
 typedef struct jf_bias_table jf_bias_table;
 
 int jf_bias_table_create(uint32_t vocabulary, uint32_t rows,
@@ -684,11 +685,11 @@ int jf_logprobs(jf_scorer *scorer, const jf_logprobs_args *args, void *stream);
  * (terms of p_k = 0 are 0; a factor of T^2 is the caller's, in grad_loss). The
  * list and T get no gradient. A list of one token with normalize is cross
  * entropy with that token.
- * A row with no listed probability has loss 0; its gradient, and that of a row
- * whose grad_loss is 0, is 0 whatever its logits. A listed token of logit
- * -infinity with p > 0 makes the loss +infinity (its gradient stays finite);
- * a student row that leaves nothing has q = 0 everywhere. NaN or +infinity in
- * a row makes its loss and gradient NaN.
+ * A row with no listed probability has loss 0; its gradient is 0 whatever its
+ * logits and grad_loss, and that of a row whose grad_loss is 0 whatever its
+ * logits. A listed token of logit -infinity with p > 0 makes the loss +infinity
+ * (its gradient stays finite); a student row that leaves nothing has q = 0
+ * everywhere. NaN or +infinity in a row makes its loss and gradient NaN.
  *
  * jf_distill: the losses (and out_lse, the rows' logsumexp of logits / T, when
  * set), and what the backward pass takes into `saved` when set:

@@ -12,7 +12,7 @@
 // The finish is a launch of its own, 4 to 6 us for few rows: a block that
 // counts the row's others in and finishes behind the last of them makes every
 // block publish its part first, and 1024 losses of 151,936 took 105 us so, 59
-// in two launches.
+// in two launches. (Not timed for a few rows.)
 //
 // The best tokens without a second pass. The pass also keeps the maximum of
 // every group of 64 consecutive tokens. The k best tokens of a row, in the
