@@ -747,7 +747,8 @@ int jf_distill_step(jf_scorer *scorer, const jf_distill_args *args,
  * logits themselves with the same stride, otherwise the two share no element. An output
  * of a row may take the place of the same row's input (a preference loss's not that of
  * its tokens, nor in a step of its loss gradients: refused), and shares no other element.
- * Everything else is constant: only the logits get a gradient. */
+ * Everything else is constant: only the logits get a gradient. Where a loss's gradient
+ * is 0, its rows' gradients are 0 whatever their logits, NaN among them. */
 
 /* With r = exp(lp - old), A the advantage, c = reference - lp and H the entropy of
  * q (all of row r):
@@ -757,9 +758,9 @@ int jf_distill_step(jf_scorer *scorer, const jf_distill_args *args,
  *                 * (G ([j = a] - q_j) + entropy_weight q_j (ln q_j + H))
  * with G = -r A where the bound does not hold r back (also exactly at it), else 0,
  * plus kl_weight (1 - exp(c)). Without old_logprobs a row's own are taken, r = 1.
- * Without a reference there is no KL term. A row whose loss gradient is 0 has
- * gradient 0 whatever its logits, and so has, with entropy_weight 0, one of G = 0.
- * The optional outputs are a row's lp, its KL term exp(c) - c - 1, and H. */
+ * Without a reference there is no KL term. With entropy_weight 0 a row of G = 0 has
+ * gradient 0 whatever its logits and its loss gradient. The optional outputs are a
+ * row's lp, its KL term exp(c) - c - 1, and H. */
 typedef struct jf_clipped_args {
   uint32_t rows;
   uint32_t dtype;

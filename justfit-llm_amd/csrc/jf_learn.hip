@@ -503,7 +503,8 @@ struct Slopes {
   __device__ __forceinline__ Slopes(const LearnedRow &r, float scale, float c, float entropy_weight)
       : m(r.x), c(c), share(scale * r.z) {
     const float weight = scale * r.y;
-    any = weight != 0.0f;
+    // A loss that nothing follows from has no gradient, also where its row's sum is NaN.
+    any = scale != 0.0f && weight != 0.0f;
     // p_j (h (t_j - E) - G) as e_j (flat + steep u_j), u_j the exponents of 2.
     flat = ENTROPY ? -weight * (r.z + entropy_weight * r.w) : -share * r.y;
     steep = ENTROPY ? weight * entropy_weight * kLn2 : 0.0f;
