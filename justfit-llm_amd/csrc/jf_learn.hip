@@ -576,6 +576,9 @@ __global__ __launch_bounds__(THREADS, 4) void clipped_step_kernel(LearnLaunch a,
       store_words<DT>(dz, at, V, d, before);
   };
   if (token >= a.vocabulary) {
+    // Every wave has the token before the row's numbers are written, which may take its
+    // place: a wave that found 0 there would learn from the row.
+    __syncthreads();
     if (tid == 0 && block == 0) put_nothing(a, row);
     const LogitWords zero{};
     for (uint32_t at = block * SLAB + tid * VEC; at < V; at += blocks * SLAB) put(at, zero);
@@ -700,6 +703,8 @@ __global__ __launch_bounds__(THREADS, 6) void learn_rows_kernel(LearnLaunch a) {
   const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63u, row = blockIdx.x;
   const uint32_t token = a.tokens[row];
   if (token >= a.vocabulary) {
+    // As in a step: every wave has the token before the row's numbers may take its place.
+    __syncthreads();
     if (tid) return;
     if constexpr (PAIRS)
       put_no_pair(a, row);
