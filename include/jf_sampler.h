@@ -758,9 +758,10 @@ int jf_distill_step(jf_scorer *scorer, const jf_distill_args *args,
  *                 * (G ([j = a] - q_j) + entropy_weight q_j (ln q_j + H))
  * with G = -r A where the bound does not hold r back (also exactly at it), else 0,
  * plus kl_weight (1 - exp(c)). Without old_logprobs a row's own are taken, r = 1.
- * Without a reference there is no KL term. With entropy_weight 0 a row of G = 0 has
- * gradient 0 whatever its logits and its loss gradient. The optional outputs are a
- * row's lp, its KL term exp(c) - c - 1, and H. */
+ * Without a reference there is no KL term. A row of NaN lp has a NaN loss, also for
+ * r = 1. With entropy_weight 0 a row of G = 0 has gradient 0 whatever its logits and
+ * its loss gradient. The optional outputs are a row's lp, its KL term
+ * exp(c) - c - 1, and H. */
 typedef struct jf_clipped_args {
   uint32_t rows;
   uint32_t dtype;

@@ -297,7 +297,8 @@ __device__ __forceinline__ LearnedRow clipped_row(const LearnLaunch &a, uint32_t
   }
   const LearnedRow record = make_float4(total.m, inv, (float)slope, mean);
   if (put) {
-    a.out_loss[row] = (float)loss;
+    // Also where no ratio has made it so: a trainer looks for NaN in its losses.
+    a.out_loss[row] = lp != lp ? (float)lp : (float)loss;
     if (a.out_logprobs) a.out_logprobs[row] = (float)lp;
     if (a.saved) a.saved[row] = record;
   }
