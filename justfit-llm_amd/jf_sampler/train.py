@@ -52,6 +52,14 @@ def distill_loss(scorer, logits, teacher_ids, teacher_values, temperature=1.0, n
                               bool(normalize))
 
 
+def _count_writes(tensors):
+    """Counts what the library has written through addresses as torch counts its own writes
+    in place, so that a graph that has saved one of the tensors refuses its backward pass.
+    Inference tensors have no such count."""
+    torch.autograd.graph.increment_version(
+        [t for t in tensors if t is not None and not t.is_inference()])
+
+
 def _rows_saved(logits):
     return torch.empty((logits.shape[0], 4), dtype=torch.float32, device=logits.device)
 
@@ -66,6 +74,7 @@ class _ClippedLoss(torch.autograd.Function):
             raise ValueError("advantages are missing")
         if loss.numel():
             scorer.launch_clipped(args)
+            _count_writes(options[k] for k in ("logprobs", "kl", "entropy"))
         # The tokens as they are now: a trainer's buffers may hold the next batch's by
         # the backward pass.
         if ctx.needs_input_grad[0]:
@@ -112,6 +121,7 @@ class _PreferenceLoss(torch.autograd.Function):
         args = scorer.preference_args(logits, tokens, offsets, loss=loss, saved=saved, **options)
         if saved.numel():
             scorer.launch_preference(args)
+            _count_writes(options[k] for k in ("scores", "logprobs"))
         else:
             # Pairs without any token.
             for t in (loss, options["scores"]):
@@ -161,4 +171,5 @@ def clip_gradients(clipper, parameters, max_norm, order=2.0):
     norm = torch.empty((), dtype=torch.float32, device=torch.device("cuda", clipper.device))
     clipper.launch_clip(clipper.args(gradients, norm=norm, max_norm=float(max_norm),
                                      order=float(order)))
+    _count_writes(gradients)
     return norm
