@@ -860,8 +860,9 @@ uint64_t jf_clipper_workspace_bytes(const jf_clipper *clipper);
 
 /* One tensor's gradient: `count` elements (0: none) in a row, at any element's
  * alignment, and where the clipped ones go: `out` NULL, or `grad` itself with its
- * dtype, for in place. No written element is another tensor's, the norm's, or read
- * elsewhere in the call: refused otherwise. */
+ * dtype, for in place. Where gradients are written, no written element is another
+ * tensor's, the norm's, or read elsewhere in the call: refused otherwise. A norm alone is
+ * written once all gradients have been read, also where it is an element of theirs. */
 typedef struct jf_gradient {
   void *grad;         /* device */
   void *out;          /* device, or NULL */
