@@ -8,7 +8,7 @@
 // gradient, and the order of blocks costs no bits that a norm in fp32 has.
 //
 // Memory bounds both: 500M bf16 elements in 290 tensors, norm 174 us (6 TB/s without
-// the launches beside it), norm and clipping 522. Blocks take chunks by turns, so that
+// the launches beside it), norm and clipping 526. Blocks take chunks by turns, so that
 // all of them read at one place of memory (a run of chunks a block: 602 us), which makes
 // every chunk one of another tensor: the table is in LDS, where looking a chunk up
 // costs little, and the next chunk's loads are out while one is worked on.

@@ -175,14 +175,17 @@ uint32_t step_blocks(uint32_t rows, const jf_clipped_args *a) {
     return 1;
   return rows <= 4 ? 8 : rows <= 24 ? 4 : 2;
 }
-// Whether a step takes rows whole, with KL term and entropies: always where a row is short
-// (one f32 row x 32,000 in eight blocks 7.2 us, 8.3 by chunks, x 40,000 8.1 against 7.9, 16
-// rows 9.5 against 8.6), and from where the rows keep the CUs busy (f32 x 48,000, 64 rows
-// 13.8 against 12.9, 128 rows 14.9 against 16.8; x 151,936, 96 rows 33.0 against 32.9, 128
-// rows 37.6 against 42.4; of the longest 192 95 against 91, 256 112 against 118; bf16 x
-// 64,000, 64 rows 14.3 against 12.9, 128 rows 15.3 against 15.1; x 100,003, 160 rows 25.7
-// against 23.2, 200 rows 26.5 against 26.2, and without entropies 192 rows 21.9 against
-// 24.4).
+// Whether a step takes rows whole: always where a row is short (one f32 row x 32,000 with
+// entropies in eight blocks 7.2 us, 8.3 by chunks, x 40,000 8.1 against 7.9, 16 rows 9.5
+// against 8.6), and from where the rows keep the CUs busy. Entropies cost whole rows more
+// than chunks, so that one rule for both comes late without them and, by up to 5%, early
+// with them. Whole against chunks, without and with entropies: f32 x 48,000, 64 rows 11.3
+// against 10.1, 12.7 against 11.1; 96 rows 12.1, 13.7; 14.0, 14.8; x 100,003, 80 rows 20.2,
+// 20.5; 23.8, 22.7; 96 rows 20.8, 22.5; 24.3, 24.5; x 151,936, 96 rows 28.5, 31.9; 33.0,
+// 32.8; of the longest, with them, 192 rows 95, 91; 256 rows 112, 118. bf16 x 64,000, 112
+// rows 11.8, 12.9; 14.5, 14.4; 128 rows 12.0, 13.6; 14.7, 15.1; x 100,003, 160 rows 21.2,
+// 21.3; 25.5, 23.3; 176 rows 21.7, 22.6; 25.9, 24.6; 200 rows 22.1, 24.2; 26.4, 26.2; x
+// 151,936, 176 rows 28.3, 31.4; 33.8, 33.1.
 bool whole_step(uint32_t rows, uint32_t vocabulary, uint32_t dtype) {
   const bool bf16 = dtype == JF_DTYPE_BF16;
   if (vocabulary <= 36u << 10) return true;
